@@ -44,6 +44,7 @@ extern "C" {
 #define PK_F16 0
 #define PK_BF16 1
 #define PK_F32 2 /* output only: un-rounded result for parity checks */
+#define PK_I8 3  /* cache storage only: signed 8-bit codes with one scale per row */
 
 /* Q/K scale granularity (reference: qk_quantization="per_warp" | "per_thread",
  * attention/kernels/qk_quantization/int8/sage/reference.py:20-74) */
@@ -184,6 +185,115 @@ PK_API int pk_debug_stalled_wait(const pk_problem* p, int sage, int skip_key_til
  *     Nothing needs clearing between calls: each call overwrites every partial it reads.
  * Results are bit-identical to the k_mean / v_mean views of pk_piper_prepare with center_value=1. */
 PK_API int pk_kv_means_static(const pk_problem* p, float* k_mean, float* v_mean);
+
+/* ------------------------------------------------------------------------------------------
+ * Sliding-window attention with sink tokens, and attention over a paged K/V cache.  These have
+ * no counterpart in the reference project; 16-bit inputs, no quantisation of Q or of the
+ * probabilities.  The entry points follow the rules at the top of this file.
+ * ------------------------------------------------------------------------------------------ */
+
+/* out[i] = sum_j softmax_j(scale * q_i.k_j) v_j over the keys that row i sees.  Row i stands at
+ * position p = i + kv_len - q_len and sees key j when j <= p and (p - j < window or j < sinks) and
+ * j < lengths[b].  Rows that see nothing, rows with p < 0 and rows with p >= lengths[b] are zero.
+ * heads is a multiple of kv_heads: query head h reads key head h / (heads / kv_heads). */
+typedef struct pk_window_problem {
+  int32_t batch, heads, kv_heads, q_len, kv_len, head_dim; /* head_dim 64 or 128 */
+  int32_t dtype;                                           /* PK_F16 | PK_BF16: q, k, v and out */
+  int32_t window;                                          /* >= 1 */
+  int32_t sinks;                                           /* >= 0 */
+  float scale;                                             /* finite and > 0 */
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch, head, sequence (elements) */
+  const int32_t* lengths;                        /* [batch] device, or NULL: kv_len everywhere */
+  void* out;                                     /* contiguous [batch, heads, q_len, head_dim], 16-byte aligned */
+  void* workspace;                               /* device scratch, 256-byte aligned */
+  uint64_t workspace_bytes;
+  int32_t device;
+  void* stream;
+} pk_window_problem;
+
+PK_API int pk_window_workspace_bytes(const pk_window_problem* p, uint64_t* bytes);
+PK_API int pk_window_attention_fwd(const pk_window_problem* p);
+
+/* A paged cache: `batch` sequences whose rows lie in pages of page_size rows.  Every array is
+ * contiguous device memory that the caller owns; the library keeps nothing.
+ *   keys, values [layers, pages, kv_heads, page_size, head_dim]; PK_I8 also key_scales,
+ *   value_scales [layers, pages, kv_heads, page_size] f32 (value = code * scale, scale >= 0)
+ *   table [batch, width]: page of each page_size rows of a sequence, -1 where there is none
+ *   lengths [batch], starts [batch]: rows [starts, lengths) are the ones added last
+ *   uses [pages]: how many table entries name the page; 0: free
+ *   refused [batch]: set to 1 (0) by extend, fork and compact for a sequence that was left alone
+ *   scratch: 4 * batch + 4 words
+ * Calls on one cache are ordered by their stream; calls on several streams need the caller's events. */
+typedef struct pk_cache {
+  int32_t layers, pages, kv_heads, page_size, head_dim; /* page_size 16, 32, 64, 128 or 256 */
+  int32_t batch, width;                                 /* batch <= 4096 */
+  int32_t dtype;                                        /* PK_F16 | PK_BF16 | PK_I8 */
+  void* keys;
+  void* values;
+  float* key_scales;
+  float* value_scales;
+  int32_t* table;
+  int32_t* lengths;
+  int32_t* starts;
+  int32_t* uses;
+  int32_t* refused;
+  int32_t* scratch;
+  int32_t device;
+  void* stream;
+} pk_cache;
+
+/* Room for counts[b] more rows (negative: none) of every sequence: starts = lengths, lengths +=
+ * counts.  A partly filled last page that other sequences also name is replaced by a copy; when all
+ * of its owners are extended in this call the first of them keeps it.  New pages are the lowest
+ * free ones, in the order of the sequences.  A sequence that would pass width * page_size rows, or
+ * for which the free pages (counted from the first sequence on) do not suffice, is refused: it is
+ * not extended (starts = lengths). */
+PK_API int pk_cache_extend(const pk_cache* c, const int32_t* counts);
+/* Stores rows [starts, lengths) of one layer (or of all: layer = -1): row t of sequence b comes from
+ * key/value[layer, b, :, t], t < tokens; element strides layer, batch, head, token; dtype PK_F16 |
+ * PK_BF16, equal to the cache's unless that is PK_I8.  8-bit rows: scale = max|x| / 127 + 1e-7, code =
+ * rint(x / scale); a row with a value that is not finite gets the scale NaN. */
+PK_API int pk_cache_write(const pk_cache* c, int32_t layer, const void* key, const void* value, const int64_t key_stride[4],
+                          const int64_t value_stride[4], int32_t dtype, int32_t tokens);
+/* Gathers rows first[b] + [0, count) of one layer (or all) into contiguous key/value
+ * [layers, batch, kv_heads, count, head_dim]; dtype PK_F32, or a 16-bit type.  Rows outside
+ * [0, lengths[b]) read as zero. */
+PK_API int pk_cache_read(const pk_cache* c, int32_t layer, const int32_t* first, int32_t count, void* key, void* value, int32_t dtype);
+/* Sequence b becomes what sequence parents[b] was before the call (shares its pages); negative:
+ * empty.  parents[b] >= batch is refused (the sequence stays as it was). */
+PK_API int pk_cache_fork(const pk_cache* c, const int32_t* parents);
+/* Every sequence keeps its first min(length, max(lengths[b], 0)) rows; pages behind them are released. */
+PK_API int pk_cache_truncate(const pk_cache* c, const int32_t* lengths);
+/* Of the rows added last keeps paths[b, i], i < counts[b], in this order: row starts + paths[b, i]
+ * moves to starts + i, the rest is released (as by truncate).  paths is [batch, most]; it must rise
+ * strictly within [0, lengths - starts): a sequence for which it does not, or whose count is not in
+ * [0, min(most, lengths - starts)], is refused and left as it was. */
+PK_API int pk_cache_compact(const pk_cache* c, const int32_t* paths, int64_t path_stride, int32_t most, const int32_t* counts);
+
+/* Attention of `tokens` query tokens per sequence over one layer of a cache.  Token t stands at row
+ * starts[b] + t and is valid below lengths[b] (others: zero).  Without a tree it sees rows j <= its
+ * own.  With tree ([batch, tokens] parents in [-1, t), tokens <= 64; other values count as -1) the
+ * rows from starts[b] on are the drafted tokens: a token sees the context and itself and the tokens
+ * above it.  window (0: none) and sinks apply to positions, a token's being starts[b] + the number
+ * of tokens above it.  q is [batch, heads, tokens, head_dim] of a 16-bit type, the cache's unless that is
+ * PK_I8.  Keys on a page that the table does not name (an entry outside [0, pages)) are not seen. */
+typedef struct pk_cache_query {
+  int32_t heads, tokens, layer, dtype, window, sinks;
+  float scale;
+  const void* q;
+  int64_t q_stride[3];  /* batch, head, token (elements) */
+  const int32_t* tree;  /* or NULL */
+  int64_t tree_stride;  /* elements between batch elements (0: one tree for all) */
+  void* out;            /* contiguous [batch, heads, tokens, head_dim], 16-byte aligned */
+  void* workspace;      /* device scratch, 256-byte aligned */
+  uint64_t workspace_bytes;
+} pk_cache_query;
+
+PK_API int pk_cache_attention_workspace_bytes(const pk_cache* c, const pk_cache_query* q, uint64_t* bytes);
+PK_API int pk_cache_attention_fwd(const pk_cache* c, const pk_cache_query* q);
 
 #ifdef __cplusplus
 }

@@ -13,7 +13,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libpiper_b200.so"
 
 PK_OK = 0
 PK_ERR_BAD_ARG, PK_ERR_UNSUPPORTED_ARCH, PK_ERR_WORKSPACE, PK_ERR_CUDA, PK_ERR_DEVICE_STATUS = 1, 2, 3, 4, 5
-PK_F16, PK_BF16, PK_F32 = 0, 1, 2
+PK_F16, PK_BF16, PK_F32, PK_I8 = 0, 1, 2, 3
 PK_QK_PER_BLOCK, PK_QK_PER_THREAD = 0, 1
 
 EXPORTS = (
@@ -23,6 +23,9 @@ EXPORTS = (
     "pk_device_status", "pk_debug_first_tile", "pk_kv_means_static", "pk_debug_timeline",
     "pk_piper_prepare_kv", "pk_piper_prepare_q", "pk_sage2pp_prepare_kv", "pk_sage2pp_prepare_q",
     "pk_poll_device_fault", "pk_debug_stalled_wait",
+    "pk_window_workspace_bytes", "pk_window_attention_fwd",
+    "pk_cache_extend", "pk_cache_write", "pk_cache_read", "pk_cache_fork", "pk_cache_truncate", "pk_cache_compact",
+    "pk_cache_attention_workspace_bytes", "pk_cache_attention_fwd",
 )
 
 
@@ -49,6 +52,38 @@ class PkViews(C.Structure):
         ("q_row_mul", C.c_void_p), ("k_col_mul", C.c_void_p), ("k_col_add", C.c_void_p),
         ("k_col_inv", C.c_void_p), ("status", C.c_void_p),
         ("sq_pad", C.c_int32), ("sk_pad", C.c_int32),
+    ]
+
+
+class PkWindowProblem(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("q_len", C.c_int32),
+        ("kv_len", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32), ("window", C.c_int32),
+        ("sinks", C.c_int32), ("scale", C.c_float),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+        ("lengths", C.c_void_p), ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("device", C.c_int32), ("stream", C.c_void_p),
+    ]
+
+
+class PkCache(C.Structure):
+    _fields_ = [
+        ("layers", C.c_int32), ("pages", C.c_int32), ("kv_heads", C.c_int32), ("page_size", C.c_int32),
+        ("head_dim", C.c_int32), ("batch", C.c_int32), ("width", C.c_int32), ("dtype", C.c_int32),
+        ("keys", C.c_void_p), ("values", C.c_void_p), ("key_scales", C.c_void_p), ("value_scales", C.c_void_p),
+        ("table", C.c_void_p), ("lengths", C.c_void_p), ("starts", C.c_void_p), ("uses", C.c_void_p),
+        ("refused", C.c_void_p), ("scratch", C.c_void_p),
+        ("device", C.c_int32), ("stream", C.c_void_p),
+    ]
+
+
+class PkCacheQuery(C.Structure):
+    _fields_ = [
+        ("heads", C.c_int32), ("tokens", C.c_int32), ("layer", C.c_int32), ("dtype", C.c_int32),
+        ("window", C.c_int32), ("sinks", C.c_int32), ("scale", C.c_float),
+        ("q", C.c_void_p), ("q_stride", C.c_int64 * 3), ("tree", C.c_void_p), ("tree_stride", C.c_int64),
+        ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
     ]
 
 
@@ -86,6 +121,18 @@ def lib() -> C.CDLL:
         handle.pk_kv_means_static.argtypes = [P, C.c_void_p, C.c_void_p]
         handle.pk_poll_device_fault.argtypes = [C.c_int32, C.POINTER(C.c_int32)]
         handle.pk_debug_stalled_wait.argtypes = [P, C.c_int, C.c_int]
+        W, K, Q = C.POINTER(PkWindowProblem), C.POINTER(PkCache), C.POINTER(PkCacheQuery)
+        ptr, i32, i64 = C.c_void_p, C.c_int32, C.c_int64
+        handle.pk_window_workspace_bytes.argtypes = [W, C.POINTER(C.c_uint64)]
+        handle.pk_window_attention_fwd.argtypes = [W]
+        handle.pk_cache_extend.argtypes = [K, ptr]
+        handle.pk_cache_write.argtypes = [K, i32, ptr, ptr, i64 * 4, i64 * 4, i32, i32]
+        handle.pk_cache_read.argtypes = [K, i32, ptr, i32, ptr, ptr, i32]
+        handle.pk_cache_fork.argtypes = [K, ptr]
+        handle.pk_cache_truncate.argtypes = [K, ptr]
+        handle.pk_cache_compact.argtypes = [K, ptr, i64, i32, ptr]
+        handle.pk_cache_attention_workspace_bytes.argtypes = [K, Q, C.POINTER(C.c_uint64)]
+        handle.pk_cache_attention_fwd.argtypes = [K, Q]
         for name in EXPORTS[2:]:
             getattr(handle, name).restype = C.c_int
         _lib = handle

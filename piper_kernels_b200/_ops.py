@@ -11,6 +11,7 @@ operator registry; all arithmetic happens inside ``libpiper_b200.so``.
 from __future__ import annotations
 
 import ctypes as C
+from typing import Optional
 
 import torch
 
@@ -116,4 +117,34 @@ def sage_attention_2pp_op(query: torch.Tensor, key: torch.Tensor, value: torch.T
 
 @sage_attention_2pp_op.register_fake
 def _(query, key, value, scale, is_causal):
+    return torch.empty_like(query, memory_format=torch.contiguous_format)
+
+
+@torch.library.custom_op("piper_b200::window_attention", mutates_args=())
+def window_attention_op(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, lengths: Optional[torch.Tensor],
+                        window: int, sinks: int, scale: float) -> torch.Tensor:
+    _require_cuda(query, "window_attention")
+    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    device = query.device.index
+    poll_device_fault(device)
+    p = _cabi.PkWindowProblem()
+    p.batch, p.heads, p.q_len, p.head_dim = query.shape
+    p.kv_heads, p.kv_len = key.shape[1], key.shape[2]
+    p.dtype, p.window, p.sinks, p.scale = _DTYPE[query.dtype], window, sinks, scale
+    p.q, p.k, p.v, p.out = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr()
+    p.q_stride, p.k_stride, p.v_stride = ((C.c_int64 * 3)(*t.stride()[:3]) for t in (query, key, value))
+    p.lengths = lengths.data_ptr() if lengths is not None else None
+    p.device, p.stream = device, torch.cuda.current_stream(query.device).cuda_stream
+    n = C.c_uint64(0)
+    lib = _cabi.lib()
+    _cabi.check(lib.pk_window_workspace_bytes(C.byref(p), C.byref(n)))
+    # allocated on the stream that uses it, like the scratch of _run
+    ws = torch.empty(max(1, n.value), dtype=torch.uint8, device=query.device)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), n.value
+    _cabi.check(lib.pk_window_attention_fwd(C.byref(p)))
+    return out
+
+
+@window_attention_op.register_fake
+def _(query, key, value, lengths, window, sinks, scale):
     return torch.empty_like(query, memory_format=torch.contiguous_format)

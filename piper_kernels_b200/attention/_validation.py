@@ -56,3 +56,48 @@ def validate_inputs(op: str, query, key, value, scale, is_causal) -> float:
     if not math.isfinite(converted) or converted <= 0:
         raise ValueError(f"{op} scale must be finite and positive, got {scale}")
     return converted
+
+
+# Checks of the 16-bit operators (window_attention, cache_attention, PageCache), which have no counterpart
+# in the reference; same fragments of messages.
+
+
+def check_rows(op: str, name: str, tensor, ndim: int = 4) -> None:
+    if tensor.ndim != ndim:
+        shape = "[layers, batch, heads, sequence, head_dim]" if ndim == 5 else "[batch, heads, sequence, head_dim]"
+        raise ValueError(f"{op} {name} must have shape {shape}, got {tuple(tensor.shape)}")
+    if tensor.dtype not in SUPPORTED_DTYPES:
+        raise ValueError(f"{op} {name} must use float16 or bfloat16, got {tensor.dtype}")
+    if tensor.layout is not torch.strided:
+        raise ValueError(f"{op} {name} must use strided layout")
+    if tensor.shape[-1] not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"{op} currently supports head dimensions 64 and 128, got {tensor.shape[-1]}")
+    if tensor.stride(-1) != 1:
+        raise ValueError(f"{op} {name}'s head dimension must be contiguous")
+
+
+def check_lengths(op: str, name: str, tensor, batch: int, device, *, optional: bool = True) -> None:
+    """Per-sequence counts: int32 [batch] on the operator's device."""
+    if tensor is None and optional:
+        return
+    if not isinstance(tensor, torch.Tensor) or tensor.dtype is not torch.int32 or tensor.shape != (batch,):
+        got = f"{tensor.dtype} {tuple(tensor.shape)}" if isinstance(tensor, torch.Tensor) else repr(tensor)
+        raise ValueError(f"{op} {name} must be int32 of shape [{batch}], got {got}")
+    if tensor.device != device:
+        raise ValueError(f"{op} {name} must be on {device}, got {tensor.device}")
+    if batch > 1 and tensor.stride(0) != 1:
+        raise ValueError(f"{op} {name} must be contiguous")
+
+
+def check_window(op: str, window, sinks) -> tuple[int, int]:
+    for name, number, least in (("window", window, 1), ("sinks", sinks, 0)):
+        if isinstance(number, bool) or not isinstance(number, int) or number < least:
+            raise ValueError(f"{op} {name} must be an integer of at least {least}, got {number!r}")
+    return min(window, 2**30), min(sinks, 2**30)
+
+
+def check_scale(op: str, scale, head_dim: int) -> float:
+    converted = head_dim**-0.5 if scale is None else float(scale)
+    if not math.isfinite(converted) or converted <= 0:
+        raise ValueError(f"{op} scale must be finite and positive, got {scale}")
+    return converted

@@ -186,30 +186,16 @@ int validate(const pk_problem* p, Algo algo, bool need_workspace) {
   return PK_OK;
 }
 
-namespace {
-
-struct DeviceGuard {
-  int prev = -1;
-  bool switched = false;
-  cudaError_t err = cudaSuccess;
-  explicit DeviceGuard(int dev) {
-    err = cudaGetDevice(&prev);
-    if (err == cudaSuccess && prev != dev) {
-      err = cudaSetDevice(dev);
-      switched = err == cudaSuccess;
-    }
-  }
-  ~DeviceGuard() {
-    if (switched) cudaSetDevice(prev);
-  }
-};
-
-int check_arch(const pk_problem* p) {
-  const int major = device_major(p->device);
-  if (major < 0) return fail(PK_ERR_CUDA, "cannot query device %d", p->device);
-  if (major != 10) return fail(PK_ERR_UNSUPPORTED_ARCH, "device %d has compute capability %d.x; this library is built for sm_100a only", p->device, major);
+int check_arch(int device) {
+  const int major = device_major(device);
+  if (major < 0) return fail(PK_ERR_CUDA, "cannot query device %d", device);
+  if (major != 10) return fail(PK_ERR_UNSUPPORTED_ARCH, "device %d has compute capability %d.x; this library is built for sm_100a only", device, major);
   return PK_OK;
 }
+
+void clear_error() { g_err[0] = 0; }
+
+namespace {
 
 void fill_views(const pk_problem& p, const Layout& L, Algo algo, pk_views* v) {
   memset(v, 0, sizeof(*v));
@@ -246,7 +232,7 @@ int prepare(const pk_problem* p, Algo algo, pk_views* views, int parts = kPrepas
   if (rc) return rc;
   DeviceGuard g(p->device);
   if (g.err != cudaSuccess) return fail(PK_ERR_CUDA, "cudaSetDevice(%d): %s", p->device, cuda_err(g.err));
-  if ((rc = check_arch(p))) return rc;
+  if ((rc = check_arch(p->device))) return rc;
   const Layout L = make_layout(*p, algo);
   if ((rc = launch_prepass(*p, L, algo, static_cast<cudaStream_t>(p->stream), parts))) return rc;
   if (views) fill_views(*p, L, algo, views);
@@ -259,7 +245,7 @@ int run(const pk_problem* p, Algo algo, const DebugDump* dump) {
   if (rc) return rc;
   DeviceGuard g(p->device);
   if (g.err != cudaSuccess) return fail(PK_ERR_CUDA, "cudaSetDevice(%d): %s", p->device, cuda_err(g.err));
-  if ((rc = check_arch(p))) return rc;
+  if ((rc = check_arch(p->device))) return rc;
   const Layout L = make_layout(*p, algo);
   return launch_fused(*p, L, algo, static_cast<cudaStream_t>(p->stream), dump);
 }
@@ -314,7 +300,7 @@ PK_API int pk_kv_means_static(const pk_problem* p, float* k_mean, float* v_mean)
   if (!k_mean || !v_mean) return fail(PK_ERR_BAD_ARG, "pk_kv_means_static: null output pointer");
   DeviceGuard g(p->device);
   if (g.err != cudaSuccess) return fail(PK_ERR_CUDA, "cudaSetDevice(%d): %s", p->device, cuda_err(g.err));
-  if ((rc = check_arch(p))) return rc;
+  if ((rc = check_arch(p->device))) return rc;
   return kv_means_static(*p, k_mean, v_mean);
 }
 

@@ -1,0 +1,736 @@
+// Attention of few query rows per key head (single tokens, chains and trees of drafted tokens, short
+// prompts) over long keys: dense tensors or a paged cache, 16-bit or 8-bit with a scale per row.
+// The formula is in pk_attend.cuh.
+//
+// What bounds it: every K and V row is read once for the few query rows that see it, 4 * rows / 2
+// operations per byte, so device memory does.  The kernel is built to keep copies in flight:
+//   - A producer warp fills a ring of three 64-key stages (K and V, up to 32 KB each) with TMA,
+//     one copy per page; two CTAs per SM keep up to 192 KB on the way.
+//   - The keys of all batch elements and heads form one list of 64-key tiles; every CTA takes an
+//     equal, contiguous share of it, whatever the lengths are (they are read on the device: nothing
+//     about them is known to the host).  The ring runs on across the borders between sequences.
+//   - A sequence that several CTAs share leaves pieces (un-normalised rows, maximum, sum) in the
+//     workspace; a second small kernel joins them.
+// The products use mma.sync: at up to 64 query rows the tensor work is far below the time of the
+// copies, and its fragments can be filled straight from the rows as they lie in memory.  The
+// contraction may visit features and keys in any order, as long as both operands use the same:
+//   - K: a thread takes 16-byte pieces of one key's row as they are; four consecutive features feed
+//     one 16-deep step (the query fragments use the same order).
+//   - V: a thread takes 16-byte pieces of the two keys that share a register and interleaves them
+//     with byte permutes, eight (or sixteen, 8-bit) output features at a time.
+// An 8-bit row's V scale is folded into the exponent: p = 2^(s + log2(scale) - max), and the sum
+// gets p / scale (the way the 8-bit attention of fused_attention.cu treats its key scales), so that
+// p stays in the range of a 16-bit float whatever the scales are.  p is rounded to the query's
+// 16-bit type for the product; maxima, sums and accumulators are 32-bit.
+
+#pragma once
+
+#include "pk_attend.cuh"
+
+namespace pk {
+namespace {
+
+constexpr int kTile = kAttendTile;
+constexpr int kStages = 3;
+constexpr int kConsumers = 128;
+constexpr int kThreads = kConsumers + 32;
+constexpr int kJoinCols = 32;          // output columns that the warps of a CTA join at a time
+constexpr float kRaise = 8.f;          // a row's reference exponent follows its maximum only beyond this
+constexpr int kMaxWorkers = 2 * 148;   // two CTAs per SM
+
+// One group of query rows (batch element, row block; the same for every key head) and the key tiles
+// that any of its rows sees: `ns` tiles of sinks, then the tiles from `first` on.
+struct Span {
+  int b, rb, off, len, ns, first, n;
+  int full_lo, full_hi;  // keys that every row sees
+};
+
+template <bool TREE>
+__device__ __forceinline__ Span span_of(const AttendParams& p, int g, int rows_per_block) {
+  Span s;
+  s.b = g / p.row_blocks;
+  s.rb = g % p.row_blocks;
+  s.len = attend_len(p, s.b);
+  s.off = attend_off(p, s.b, s.len);
+  const int r0 = s.rb * rows_per_block, r1 = min(r0 + rows_per_block, p.rows) - 1;
+  const int t0 = r0 / p.group, t1 = r1 / p.group;
+  int hi, lo;
+  if (TREE) {
+    hi = min(s.len, s.off + p.tokens);
+    lo = s.off - p.window + 1;
+    s.full_hi = min(s.len, s.off);
+    s.full_lo = s.off + p.tokens - p.window;
+  } else {
+    hi = min(s.len, s.off + t1 + 1);
+    lo = s.off + t0 - p.window + 1;
+    s.full_hi = min(s.len, s.off + t0 + 1);
+    s.full_lo = s.off + t1 - p.window + 1;
+  }
+  if (s.off + t0 >= s.len) hi = 0;  // no valid row
+  hi = max(hi, 0);
+  lo = min(max(lo, 0), hi);
+  s.ns = (min(p.sinks, lo) + kTile - 1) / kTile;
+  s.first = max(lo / kTile, s.ns);
+  s.n = s.ns + max(0, (hi + kTile - 1) / kTile - s.first);
+  if (s.n == 0) s.n = 1, s.ns = 0, s.first = 0;  // rows that see nothing still have to be written
+  return s;
+}
+
+// First tile of worker w, when `total` tiles are shared out.
+__device__ __forceinline__ int64_t share_begin(int64_t total, int workers, int w) {
+  return total / workers * w + min(static_cast<int64_t>(w), total % workers);
+}
+__device__ __forceinline__ int owner_of(int64_t total, int workers, int64_t tile) {
+  const int64_t base = total / workers, extra = total % workers, big = extra * (base + 1);
+  return static_cast<int>(tile < big ? tile / (base + 1) : extra + (tile - big) / base);
+}
+
+struct Found {  // a group and the tiles in front of it
+  int64_t before;
+  int group;
+};
+
+// Tiles of the groups in front of `upto`, all key heads; by the whole CTA, threads [0, 128) count.
+
+template <bool TREE>
+__device__ __forceinline__ int64_t sum_tiles(const AttendParams& p, int rows_per_block, int upto, int64_t* red) {
+  int64_t mine = 0;
+  if (threadIdx.x < kConsumers)
+    for (int g = threadIdx.x; g < upto; g += kConsumers) mine += span_of<TREE>(p, g, rows_per_block).n;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if ((threadIdx.x & 31) == 0 && threadIdx.x < kConsumers) red[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  const int64_t sum = red[0] + red[1] + red[2] + red[3];
+  __syncthreads();
+  return sum * p.kv_heads;
+}
+
+// Finds the group that holds tile `at` (0 <= at < total), 128 groups at a time.
+template <bool TREE>
+__device__ __forceinline__ Found find_group(const AttendParams& p, int rows_per_block, int64_t at, int64_t* red, Found* out) {
+  const int groups = p.batch * p.row_blocks, lane = threadIdx.x & 31;
+  int64_t before = 0;
+  if (threadIdx.x == 0) out->group = -1;
+  __syncthreads();
+  for (int g0 = 0; g0 < groups; g0 += kConsumers) {
+    const int g = g0 + threadIdx.x;
+    int64_t n = 0;
+    if (threadIdx.x < kConsumers && g < groups) n = static_cast<int64_t>(span_of<TREE>(p, g, rows_per_block).n) * p.kv_heads;
+    int64_t incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31 && threadIdx.x < kConsumers) red[threadIdx.x >> 5] = incl;
+    __syncthreads();
+    if (threadIdx.x < kConsumers) {
+      int64_t base = before;
+      for (int w = 0; w < (threadIdx.x >> 5); ++w) base += red[w];
+      const int64_t b0 = base + incl - n;
+      if (n > 0 && at >= b0 && at < b0 + n) out->group = g, out->before = b0;
+    }
+    before += red[0] + red[1] + red[2] + red[3];
+    __syncthreads();
+    if (out->group >= 0) break;  // the same for every thread: written before the barrier
+  }
+  return *out;
+}
+
+template <typename T, bool I8, int D, int WM>
+struct Few {
+  static constexpr int WN = 4 / WM;
+  static constexpr int ROWS = 16 * WM;
+  static constexpr int ESZ = I8 ? 1 : 2;
+  static constexpr int ROW_BYTES = D * ESZ;
+  static constexpr int LINE = ROW_BYTES > 128 ? 128 : ROW_BYTES;  // swizzled line
+  static constexpr int HALVES = ROW_BYTES / LINE;
+  static constexpr int KV_BYTES = kTile * ROW_BYTES;
+  static constexpr int SCALE_BYTES = I8 ? 2 * kTile * 4 : 0;
+  static constexpr int STAGE = 2 * KV_BYTES;
+  static constexpr int KEYS = kTile / WN;  // keys of a tile per warp
+  // In a 16-byte shared-memory access eight threads (two key columns x four pieces) are served at
+  // once.  128-byte lines: neighbouring columns are mapped to keys four apart, whose pieces the
+  // swizzle puts into the other half of the banks.  64-byte lines: neighbours are two halves of 128 bytes.
+  static constexpr bool APART = LINE == 128;
+  static constexpr int OFF_JOIN = kStages * STAGE;
+  static constexpr int OFF_SCALE = OFF_JOIN + 4 * 16 * kJoinCols * 4;
+  static constexpr int OFF_ML = OFF_SCALE + kStages * SCALE_BYTES;
+  static constexpr int OFF_TREE = OFF_ML + 4 * 16 * 8;
+  static constexpr int OFF_BAR = OFF_TREE + static_cast<int>(sizeof(TreeMasks));
+  static constexpr int OFF_RED = OFF_BAR + 2 * kStages * 8;
+  static constexpr int OFF_MISC = OFF_RED + 4 * 8 + 24;
+  static constexpr int OFF_THERE = OFF_MISC + 4;  // per stage: which of its pages exist, one bit each
+  static constexpr int SMEM = OFF_THERE + kStages * 4;
+};
+
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1, __half) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two signed bytes of `w` (the bytes that `sel` puts into the low byte of each half) as two 16-bit floats, exactly.
+// f16: 1024 + (byte ^ 0x80) is a bit pattern; minus 1152.
+__device__ __forceinline__ uint32_t two_bytes(uint32_t w, bool high, __half) {
+  const uint32_t u = __byte_perm(w ^ 0x80808080u, 0x64646464u, high ? 0x4342 : 0x4140);
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// bf16: 128 + (byte & 127) and 128 + (byte & 128) are bit patterns; their difference.
+__device__ __forceinline__ uint32_t two_bytes(uint32_t w, bool high, __nv_bfloat16) {
+  const uint32_t u = __byte_perm(w, 0u, high ? 0x4342 : 0x4140);
+  const uint32_t lo = (u & 0x007F007Fu) | 0x43004300u, sg = (u & 0x00800080u) | 0x43004300u;
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&sg));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+
+// Barrier of the 128 consumer threads; true when `good` holds in all of them.
+__device__ __forceinline__ bool join_vote(bool good) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(static_cast<uint32_t>(good))
+      : "memory");
+  return all != 0;
+}
+
+template <bool TREE>
+struct Walk {  // position in the list of tiles
+  Span s;
+  int g, h, tile;
+  template <int ROWS>
+  __device__ __forceinline__ void start(const AttendParams& p, const Found& f, int64_t at) {
+    g = f.group;
+    s = span_of<TREE>(p, g, ROWS);
+    const int64_t rel = at - f.before;
+    h = static_cast<int>(rel / s.n);
+    tile = static_cast<int>(rel % s.n);
+  }
+  template <int ROWS>
+  __device__ __forceinline__ void next(const AttendParams& p) {
+    if (++tile < s.n) return;
+    tile = 0;
+    if (++h < p.kv_heads) return;
+    h = 0;
+    if (++g < p.batch * p.row_blocks) s = span_of<TREE>(p, g, ROWS);
+  }
+  __device__ __forceinline__ int key() const { return (tile < s.ns ? tile : s.first + tile - s.ns) * kTile; }
+};
+
+template <typename T, bool I8, int D, int WM, bool TREE>
+__global__ void __launch_bounds__(kThreads, 2)
+few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttendParams p) {
+  using C = Few<T, I8, D, WM>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  int64_t* red = reinterpret_cast<int64_t*>(smem + C::OFF_RED);
+  Found* found = reinterpret_cast<Found*>(smem + C::OFF_RED + 32);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC);
+  volatile uint32_t* there = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_THERE);
+  const uint32_t bars = base + C::OFF_BAR;  // full[kStages], empty[kStages]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid < 2 * kStages) {
+    mbar_init(bars + 8 * tid, tid < kStages ? 1 : 4);
+    fence_barrier_init();
+  }
+  if (tid == 0) *abort_flag = 0;
+  if (tid == kConsumers) { prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
+  cudaGridDependencySynchronize();
+  __syncthreads();
+
+  const int groups = p.batch * p.row_blocks;
+  const int64_t total = sum_tiles<TREE>(p, C::ROWS, groups, red);
+  const int64_t w0 = share_begin(total, gridDim.x, blockIdx.x), w1 = share_begin(total, gridDim.x, blockIdx.x + 1);
+  if (w0 >= w1) return;
+  const Found f = find_group<TREE>(p, C::ROWS, w0, red, found);
+  Walk<TREE> walk;
+  walk.template start<C::ROWS>(p, f, w0);
+
+  if (warp == kConsumers / 32) {
+    // ---------------------------------------------------------------- producer
+    if (lane == 0) {
+      const int box = p.table ? min(p.page, kTile) : kTile;
+      int last = -1;
+      bool ok = true;
+      for (int64_t w = w0; w < w1; ++w, walk.template next<C::ROWS>(p)) {
+        const int i = static_cast<int>(w - w0), st = i % kStages;
+        if (i >= kStages && !mbar_wait_bounded(bars + 8 * (kStages + st), ((i / kStages) - 1) & 1, abort_flag, 61)) { ok = false; break; }
+        const uint32_t full = bars + 8 * st, dst = base + st * C::STAGE;
+        const int j0 = walk.key();
+        int scale_boxes = 0;
+        if (!p.table) {
+          there[st] = 1u;
+          mbar_expect_tx(full, C::STAGE);
+          tma_load_5d(dst, &tm_k, full, 0, j0, 0, p.k_stride[1] ? walk.h : 0, p.k_stride[0] ? walk.s.b : 0);
+          tma_load_5d(dst + C::KV_BYTES, &tm_v, full, 0, j0, 0, p.v_stride[1] ? walk.h : 0, p.v_stride[0] ? walk.s.b : 0);
+        } else {
+          int pages[kTile / 16];
+          uint32_t mask = 0;
+#pragma unroll
+          for (int x = 0; x < kTile / 16; ++x) {
+            const int j = j0 + x * box;
+            // a page that is not there, or lies behind the sequence, reads as zeros (outside the map)
+            pages[x] = (x * box < kTile && j < walk.s.len) ? attend_page(p, walk.s.b, j) : -1;
+            if (pages[x] >= 0) mask |= 1u << x;
+            if (I8 && pages[x] >= 0) ++scale_boxes;
+          }
+          there[st] = mask;
+          mbar_expect_tx(full, C::STAGE + scale_boxes * 2 * box * 4);
+#pragma unroll
+          for (int x = 0; x < kTile / 16; ++x) {
+            if (x * box >= kTile) break;
+            const int row = (j0 + x * box) & (p.page - 1);
+            const int c4 = pages[x] >= 0 ? p.page_base + pages[x] : 0x7fffffff;
+            tma_load_5d(dst + x * box * C::ROW_BYTES, &tm_k, full, 0, row, 0, walk.h, c4);
+            tma_load_5d(dst + C::KV_BYTES + x * box * C::ROW_BYTES, &tm_v, full, 0, row, 0, walk.h, c4);
+            if (I8 && pages[x] >= 0) {
+              const int64_t at = (static_cast<int64_t>(pages[x]) * p.kv_heads + walk.h) * p.page + row;
+              const uint32_t sdst = base + C::OFF_SCALE + st * C::SCALE_BYTES + x * box * 4;
+              bulk_load(sdst, p.k_scale + at, box * 4, full);
+              bulk_load(sdst + kTile * 4, p.v_scale + at, box * 4, full);
+            }
+          }
+        }
+        last = i;
+      }
+      if (!ok)  // giving up: let the copies that were issued land before the CTA returns
+        for (int i = max(0, last - kStages + 1); i <= last; ++i) mbar_wait_quiet(bars + 8 * (i % kStages), (i / kStages) & 1, 100000);
+    }
+    return;
+  }
+
+  // ------------------------------------------------------------------ consumers
+  const int wm = warp % WM, wn = warp / WM;
+  const int g8 = lane >> 2, c4 = lane & 3;
+  TreeMasks* tm = reinterpret_cast<TreeMasks*>(smem + C::OFF_TREE);
+  float* join = reinterpret_cast<float*>(smem + C::OFF_JOIN);
+  float2* ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
+  // key of column n of an 8-key step
+  auto key_of = [](int n) { return C::APART ? ((n & 1) << 2) | (n >> 1) : n; };
+  constexpr int OT = D / 8;  // output column tiles
+  uint32_t qf[D / 16][4];
+  float o[OT][4], m[2], l[2];
+  RowView view[2];
+  int tree_b = -1;
+  bool ok = true;
+
+  int64_t w = w0;
+  for (int i = 0; ok && w < w1;) {
+    // -------- a new unit: rows [rb * ROWS, ...) of key head h of batch element b
+    const Span s = walk.s;
+    const int h = walk.h, unit_from = walk.tile;
+    if (TREE && s.b != tree_b) {
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // the previous masks have been read
+      if (warp == 0) build_tree(p, s.b, s.off, lane, tm);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      tree_b = s.b;
+    }
+    const T* qrow[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = s.rb * C::ROWS + wm * 16 + g8 + 8 * x, t = r / p.group;
+      view[x] = r < p.rows ? row_view(p, s.off, s.len, t, TREE ? tm : nullptr) : RowView{0, 0, 0};
+      const bool there = r < p.rows;
+      qrow[x] = there ? static_cast<const T*>(p.q) + s.b * p.q_stride[0] + (h * p.group + r % p.group) * p.q_stride[1] + t * p.q_stride[2] : nullptr;
+      m[x] = -INFINITY;
+      l[x] = 0.f;
+    }
+    // query fragments in the order in which K rows are read (16 bytes of a K row at a time)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      constexpr int PIECE = I8 ? 16 : 8;  // features per 16 bytes of K
+#pragma unroll
+      for (int j = 0; j < D / PIECE / 4; ++j) {
+#pragma unroll
+        for (int k = 0; k < PIECE / 8; ++k) {
+          const int d = (j * 4 + c4) * PIECE + k * 8;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (qrow[x]) {
+            if (p.q_vec) {
+              v = *reinterpret_cast<const uint4*>(qrow[x] + d);
+            } else {
+              uint32_t e[8];
+#pragma unroll
+              for (int y = 0; y < 8; ++y) e[y] = *reinterpret_cast<const uint16_t*>(qrow[x] + d + y);
+              v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+            }
+          }
+          const int step = (j * (PIECE / 8) + k) * 2;
+          qf[step][x] = v.x, qf[step][2 + x] = v.y, qf[step + 1][x] = v.z, qf[step + 1][2 + x] = v.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < OT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+
+    const int unit_tiles = static_cast<int>(min(static_cast<int64_t>(s.n - walk.tile), w1 - w));
+    const int box = p.table ? min(p.page, kTile) : kTile;
+    for (int u = 0; u < unit_tiles; ++u, ++i, ++w) {
+      const int st = i % kStages;
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * st, (i / kStages) & 1, abort_flag, 62));
+      if (!ok) break;
+      const int j0 = (unit_from + u < s.ns ? unit_from + u : s.first + unit_from + u - s.ns) * kTile;
+      // Keys on pages that are not there are masked like those that no row may see.
+      const uint32_t held = there[st], all = (1u << (kTile / box)) - 1;
+      const bool full = held == all && ((j0 >= s.full_lo && j0 + kTile <= s.full_hi) || (j0 + kTile <= min(p.sinks, s.full_hi)));
+      const uint32_t kst = base + st * C::STAGE, vst = kst + C::KV_BYTES;
+      const float* sc = reinterpret_cast<const float*>(smem + C::OFF_SCALE + st * C::SCALE_BYTES);
+#pragma unroll 1
+      for (int step = 0; step < C::KEYS / 16; ++step) {
+        const int k0 = wn * C::KEYS + step * 16;  // within the tile
+        if (j0 + k0 >= s.len && !full) continue;  // behind the sequence (the same for the whole warp)
+        const uint32_t off0 = C::HALVES == 2 ? (k0 / box) * (box * C::ROW_BYTES) + (k0 % box) * 128 : k0 * C::LINE;
+        const uint32_t half = box * 128;
+        // ---- scores of 16 keys
+        float sv[2][4];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          sv[nt][0] = sv[nt][1] = sv[nt][2] = sv[nt][3] = 0.f;
+          const int kk = nt * 8 + key_of(g8);
+          const uint32_t row = kst + off0 + kk * C::LINE;
+          const int sw = C::LINE == 128 ? (kk & 7) : ((kk >> 1) & 3);
+#pragma unroll
+          for (int j = 0; j < C::ROW_BYTES / 64; ++j) {
+            const int chunk = j * 4 + c4;
+            const uint32_t a = row + (C::HALVES == 2 ? (chunk >> 3) * half : 0) + (((chunk & (C::LINE / 16 - 1)) ^ sw) << 4);
+            const uint4 v = lds128(a);
+            if (I8) {
+              const uint32_t wv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int y = 0; y < 4; ++y) mma16816(sv[nt], qf[j * 4 + y], two_bytes(wv[y], false, T{}), two_bytes(wv[y], true, T{}), T{});
+            } else {
+              mma16816(sv[nt], qf[j * 2], v.x, v.y, T{});
+              mma16816(sv[nt], qf[j * 2 + 1], v.z, v.w, T{});
+            }
+          }
+        }
+        // ---- to base-2 exponents; column n of the fragment is key key_of(n)
+        float inv[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int kk = (y >> 1) * 8 + key_of(2 * c4 + (y & 1));
+          float mul = p.scale_log2, add = 0.f;
+          if (I8) {
+            // A scale of zero makes a zero row, whose weight still counts: taken as 2^-60.
+            float vs = sc[kTile + k0 + kk];
+            vs = vs < 0x1p-60f ? 0x1p-60f : vs;
+            mul *= sc[k0 + kk];
+            add = __log2f(vs);
+            inv[y] = __frcp_rn(vs);
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float& e = sv[y >> 1][(y & 1) + 2 * x];
+            e = I8 ? fmaf(e, mul, add) : e * mul;
+          }
+        }
+        if (!full) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int j = j0 + k0 + (y >> 1) * 8 + key_of(2 * c4 + (y & 1));
+            const bool in = j < s.len && ((held >> (k0 / box)) & 1);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              if (!in || !sees<TREE>(view[x], j, s.off, p.sinks)) sv[y >> 1][(y & 1) + 2 * x] = -INFINITY;
+          }
+        }
+        // ---- running maximum: the reference exponent moves only when a score exceeds it by more
+        // than kRaise (2^kRaise fits every type); the quotient is the same for any reference
+        float top[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) top[x] = fmaxf(fmaxf(sv[0][2 * x], sv[0][2 * x + 1]), fmaxf(sv[1][2 * x], sv[1][2 * x + 1]));
+        const bool raise = top[0] > m[0] + kRaise || top[1] > m[1] + kRaise;
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float t = top[x];
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+            const float mn = t > m[x] + kRaise ? t : m[x];
+            const float keep = m[x] == mn ? 1.f : ex2_approx(m[x] - mn);
+            m[x] = mn;
+            l[x] *= keep;
+#pragma unroll
+            for (int t2 = 0; t2 < OT; ++t2) o[t2][2 * x] *= keep, o[t2][2 * x + 1] *= keep;
+          }
+        }
+        uint32_t pf[4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float ref = m[x] == -INFINITY ? 0.f : m[x];
+          float e[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            e[y] = ex2_approx(sv[y >> 1][(y & 1) + 2 * x] - ref);
+            l[x] = I8 ? (e[y] != 0.f ? fmaf(e[y], inv[y], l[x]) : l[x]) : l[x] + e[y];
+          }
+          pf[x] = pack2<T>(e[0], e[1]);
+          pf[2 + x] = pack2<T>(e[2], e[3]);
+        }
+        // ---- O += P V
+        int kk[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) kk[y] = (y >> 1) * 8 + key_of(2 * c4 + (y & 1));
+        // Rows behind the sequence are whatever an earlier owner of the page left (a NaN times the
+        // weight 0 is a NaN): they are taken as zeros.
+        const bool ragged = j0 + k0 + 16 > s.len;
+        if (I8) {
+          constexpr int W = D == 128 ? 4 : 2;  // words of a V row per thread
+          uint32_t vw[4][4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const uint32_t row = vst + off0 + kk[y] * C::LINE;
+            if (D == 128) {
+              const uint4 v = lds128(row + ((key_of(g8) ^ (kk[y] & 7)) << 4));
+              vw[y][0] = v.x, vw[y][1] = v.y, vw[y][2] = v.z, vw[y][3] = v.w;
+            } else {
+              const uint2 v = lds64(row + (((g8 >> 1) ^ ((kk[y] >> 1) & 3)) << 4) + (g8 & 1) * 8);
+              vw[y][0] = v.x, vw[y][1] = v.y, vw[y][2] = vw[y][3] = 0;
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < W; ++x) {
+            // bytes of two keys, alternating: a0 b0 a1 b1 / a2 b2 a3 b3
+            const uint32_t lo01 = __byte_perm(vw[0][x], vw[1][x], 0x5140), lo23 = __byte_perm(vw[0][x], vw[1][x], 0x7362);
+            const uint32_t hi01 = __byte_perm(vw[2][x], vw[3][x], 0x5140), hi23 = __byte_perm(vw[2][x], vw[3][x], 0x7362);
+            mma16816(o[x * 4 + 0], pf, two_bytes(lo01, false, T{}), two_bytes(hi01, false, T{}), T{});
+            mma16816(o[x * 4 + 1], pf, two_bytes(lo01, true, T{}), two_bytes(hi01, true, T{}), T{});
+            mma16816(o[x * 4 + 2], pf, two_bytes(lo23, false, T{}), two_bytes(hi23, false, T{}), T{});
+            mma16816(o[x * 4 + 3], pf, two_bytes(lo23, true, T{}), two_bytes(hi23, true, T{}), T{});
+          }
+        } else {
+#pragma unroll
+          for (int hf = 0; hf < D / 64; ++hf) {
+            uint32_t vw[4][4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const uint4 v = lds128(vst + off0 + hf * half + kk[y] * 128 + ((key_of(g8) ^ (kk[y] & 7)) << 4));
+              vw[y][0] = v.x, vw[y][1] = v.y, vw[y][2] = v.z, vw[y][3] = v.w;
+              if (ragged && j0 + k0 + kk[y] >= s.len) vw[y][0] = vw[y][1] = vw[y][2] = vw[y][3] = 0;
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              mma16816(o[hf * 8 + 2 * x], pf, __byte_perm(vw[0][x], vw[1][x], 0x5410), __byte_perm(vw[2][x], vw[3][x], 0x5410), T{});
+              mma16816(o[hf * 8 + 2 * x + 1], pf, __byte_perm(vw[0][x], vw[1][x], 0x7632), __byte_perm(vw[2][x], vw[3][x], 0x7632), T{});
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + 8 * (kStages + st));
+    }
+
+    // -------- join the warps that shared the unit's keys; write rows, or a piece for the join kernel
+    const bool whole = unit_from == 0 && unit_tiles == s.n;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+      if (!ok) l[x] = __int_as_float(0x7FC00000);
+      if (c4 == 0) ml[warp * 16 + g8 + 8 * x] = make_float2(m[x], l[x]);
+    }
+    ok = join_vote(ok && *abort_flag == 0);  // the same answer in every warp: they leave together
+    const int slot = blockIdx.x * 2 + (unit_from == 0 && w - unit_tiles != w0 ? 1 : 0);
+    float* piece = p.partial + static_cast<int64_t>(slot) * C::ROWS * (D + 2);
+    // thread -> (row, four consecutive columns) of the CTA's rows; a row's columns belong to 8 neighbouring threads
+    bool bad[WM];
+#pragma unroll
+    for (int x = 0; x < WM; ++x) bad[x] = false;
+#pragma unroll
+    for (int pass = 0; pass < D / kJoinCols; ++pass) {
+      // stage: [warp][16 rows][32 columns].  The fragment's columns are spread over the row (16-byte
+      // pieces of V rows): this pass takes the output tiles whose features lie in its 32 columns.
+#pragma unroll
+      for (int t = 0; t < OT; ++t) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          int d;
+          if (I8 && D == 128) d = (c4 + 4 * n) * 16 + t;
+          else if (I8) d = (2 * c4 + n) * 8 + t;
+          else d = (t >> 3) * 64 + (c4 + 4 * n) * 8 + (t & 7);
+          if (d / kJoinCols == pass) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) join[(warp * 16 + g8 + 8 * x) * kJoinCols + (d % kJoinCols)] = o[t][n + 2 * x];
+          }
+        }
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+      for (int it = 0; it < WM; ++it) {
+        const int r16 = tid >> 3, col = (tid & 7) * 4;  // rows of warp row `it`
+        const int row = s.rb * C::ROWS + it * 16 + r16;
+        float mx = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < C::WN; ++n) mx = fmaxf(mx, ml[(n * WM + it) * 16 + r16].x);
+#pragma unroll
+        for (int n = 0; n < C::WN; ++n) {
+          const float2 st = ml[(n * WM + it) * 16 + r16];
+          const float wgt = st.x == mx ? 1.f : ex2_approx(st.x - mx);
+          const float4 v = *reinterpret_cast<const float4*>(join + ((n * WM + it) * 16 + r16) * kJoinCols + col);
+          sum = fmaf(st.y, wgt, sum);
+          acc[0] = fmaf(v.x, wgt, acc[0]), acc[1] = fmaf(v.y, wgt, acc[1]), acc[2] = fmaf(v.z, wgt, acc[2]), acc[3] = fmaf(v.w, wgt, acc[3]);
+        }
+        if (row < p.rows) {
+          if (!whole) {
+            float* dst = piece + (it * 16 + r16) * (D + 2);
+            *reinterpret_cast<float2*>(dst + pass * kJoinCols + col) = make_float2(acc[0], acc[1]);
+            *reinterpret_cast<float2*>(dst + pass * kJoinCols + col + 2) = make_float2(acc[2], acc[3]);
+            if (pass == 0 && (tid & 7) == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mx, sum);
+          } else {
+            const int t = row / p.group, idx = s.off + t;
+            const bool valid = idx >= 0 && idx < s.len;
+            const float r = valid && sum != 0.f ? 1.f / sum : 0.f;
+            float v[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              v[y] = r == 0.f ? 0.f : acc[y] * r;
+              bad[it] |= !(fabsf(v[y]) <= 3.0e38f);
+            }
+            T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + row % p.group) * p.tokens + t) * D + pass * kJoinCols + col;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+          }
+        }
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+    }
+#pragma unroll
+    for (int it = 0; it < WM; ++it) {
+      // rows with a value that is not finite, evaluated again from their own keys
+      const uint32_t vote = __ballot_sync(0xffffffffu, bad[it]);
+      __syncwarp();
+#pragma unroll 1
+      for (int r = 0; vote && r < 4; ++r) {
+        if (!(vote & (0xffu << (8 * r)))) continue;
+        const int row = s.rb * C::ROWS + it * 16 + warp * 4 + r;
+        plain_row<T, I8, D>(p, s.b, h, row, s.off, s.len, row_view(p, s.off, s.len, row / p.group, TREE ? tm : nullptr), TREE);
+      }
+    }
+    // the next unit
+    walk.tile = unit_from + unit_tiles - 1;
+    walk.template next<C::ROWS>(p);
+  }
+  if (tid == 0 && *abort_flag != 0 && p.host_status != nullptr) atomicCAS_system(p.host_status, 0, *abort_flag);
+}
+
+// Joins the pieces of every unit that more than one CTA worked on.  One CTA per unit (batch element,
+// row block, key head); units that one CTA finished are left alone.
+template <typename T, bool I8, int D, int WM, bool TREE>
+__global__ void __launch_bounds__(kConsumers) join_kernel(const __grid_constant__ AttendParams p, int workers) {
+  using C = Few<T, I8, D, WM>;
+  __shared__ int64_t red[4];
+  __shared__ TreeMasks tm;
+  const int unit = blockIdx.x, g = unit / p.kv_heads, h = unit % p.kv_heads, groups = p.batch * p.row_blocks;
+  cudaGridDependencySynchronize();
+  const int64_t total = sum_tiles<TREE>(p, C::ROWS, groups, red);
+  int64_t u0 = sum_tiles<TREE>(p, C::ROWS, g, red);
+  const Span s = span_of<TREE>(p, g, C::ROWS);
+  u0 += static_cast<int64_t>(h) * s.n;
+  const int c0 = owner_of(total, workers, u0), c1 = owner_of(total, workers, u0 + s.n - 1);
+  if (c0 == c1) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (TREE) {
+    if (warp == 0) build_tree(p, s.b, s.off, lane, &tm);
+    __syncthreads();
+  }
+  const bool first_second = u0 > share_begin(total, workers, c0);  // its first CTA began with another unit
+  constexpr int E = D / 32;
+  const int r1 = min(p.rows - s.rb * C::ROWS, C::ROWS);
+  for (int r = warp; r < r1; r += kConsumers / 32) {
+    float mx = -INFINITY, sum = 0.f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int c = c0 + lane; c <= c1; c += 32)
+      mx = fmaxf(mx, p.partial[(static_cast<int64_t>(c * 2 + (c == c0 && first_second)) * C::ROWS + r) * (D + 2) + D]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const float* src = p.partial + (static_cast<int64_t>(c * 2 + (c == c0 && first_second)) * C::ROWS + r) * (D + 2);
+      const float2 st = *reinterpret_cast<const float2*>(src + D);
+      const float wgt = st.x == mx ? 1.f : ex2_approx(st.x - mx);
+      sum = fmaf(st.y, wgt, sum);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(src + lane * E + e);
+        acc[e] = fmaf(v.x, wgt, acc[e]);
+        acc[e + 1] = fmaf(v.y, wgt, acc[e + 1]);
+      }
+    }
+    const int row = s.rb * C::ROWS + r, t = row / p.group, idx = s.off + t;
+    const float inv = idx >= 0 && idx < s.len && sum != 0.f ? 1.f / sum : 0.f;
+    T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + row % p.group) * p.tokens + t) * D + lane * E;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float a = inv == 0.f ? 0.f : acc[e] * inv, b = inv == 0.f ? 0.f : acc[e + 1] * inv;
+      bad |= !(fabsf(a) <= 3.0e38f) || !(fabsf(b) <= 3.0e38f);
+      *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(a, b);
+    }
+    __syncwarp();
+    if (__any_sync(0xffffffffu, bad)) plain_row<T, I8, D>(p, s.b, h, row, s.off, s.len, row_view(p, s.off, s.len, t, TREE ? &tm : nullptr), TREE);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------
+template <typename T, bool I8, int D, int WM, bool TREE>
+int launch(AttendParams p, int device, cudaStream_t st) {
+  using C = Few<T, I8, D, WM>;
+  static_assert(C::SMEM <= 113 * 1024, "two CTAs share an SM");
+  p.row_blocks = (p.rows + C::ROWS - 1) / C::ROWS;
+  CUtensorMap tk, tv;
+  int rc;
+  if ((rc = attend_map(&tk, p, p.k, p.k_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < kTile ? p.page : kTile) : kTile))) return rc;
+  if ((rc = attend_map(&tv, p, p.v, p.v_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < kTile ? p.page : kTile) : kTile))) return rc;
+  if ((rc = allow_smem<few_rows_kernel<T, I8, D, WM, TREE>>(C::SMEM, device))) return rc;
+  // No more CTAs than there can be tiles.
+  const int64_t most = static_cast<int64_t>(p.batch) * p.row_blocks * p.kv_heads * (((p.table ? p.width * p.page : p.kv_len) + kTile - 1) / kTile + 1);
+  p.workers = static_cast<int>(most < kMaxWorkers ? most : kMaxWorkers);
+  cudaError_t e = launch_chained(few_rows_kernel<T, I8, D, WM, TREE>, dim3(p.workers), dim3(kThreads), C::SMEM, st, tk, tv, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(PK_ERR_CUDA, "attention kernel launch failed: %s", cuda_err(e));
+  e = launch_chained(join_kernel<T, I8, D, WM, TREE>, dim3(p.batch * p.row_blocks * p.kv_heads), dim3(kConsumers), 0, st, p, p.workers);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(PK_ERR_CUDA, "join kernel launch failed: %s", cuda_err(e));
+  return PK_OK;
+}
+
+template <typename T, bool I8, int D, bool TREE>
+int by_rows(const AttendParams& p, int device, cudaStream_t st) {
+  if (p.rows <= 16) return launch<T, I8, D, 1, TREE>(p, device, st);
+  if (p.rows <= 32) return launch<T, I8, D, 2, TREE>(p, device, st);
+  return launch<T, I8, D, 4, TREE>(p, device, st);
+}
+template <typename T, bool I8, int D>
+int by_tree(const AttendParams& p, int device, cudaStream_t st) {
+  return p.tree ? by_rows<T, I8, D, true>(p, device, st) : by_rows<T, I8, D, false>(p, device, st);
+}
+template <typename T, bool I8>
+int by_dim(const AttendParams& p, int head_dim, int device, cudaStream_t st) {
+  return head_dim == 128 ? by_tree<T, I8, 128>(p, device, st) : by_tree<T, I8, 64>(p, device, st);
+}
+
+}  // namespace
+}  // namespace pk

@@ -1,0 +1,15 @@
+// Few-row attention (few_rows.cuh) for float16 queries.
+#include "few_rows.cuh"
+
+namespace pk {
+
+uint64_t few_rows_workspace(int rows, int head_dim) {
+  const int block = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  return static_cast<uint64_t>(kMaxWorkers) * 2 * block * (head_dim + 2) * sizeof(float);
+}
+
+int launch_few_rows_f16(const AttendParams& p, int head_dim, bool i8, int device, cudaStream_t st) {
+  return i8 ? by_dim<__half, true>(p, head_dim, device, st) : by_dim<__half, false>(p, head_dim, device, st);
+}
+
+}  // namespace pk

@@ -3,6 +3,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <utility>
 #include <stddef.h>
 #include <stdint.h>
@@ -71,6 +72,38 @@ struct DebugDump {
 int32_t* fault_word_device_ptr(int device);
 int launch_fused(const pk_problem& p, const Layout& L, Algo algo, cudaStream_t stream,
                  const DebugDump* dump);
+
+// Lets a kernel use `bytes` of dynamic shared memory on `device` (set once per kernel and device).
+template <auto KERNEL>
+int allow_smem(int bytes, int device) {
+  static std::atomic<bool> done[64];
+  const int dev = (device >= 0 && device < 64) ? device : 0;
+  if (done[dev].load(std::memory_order_acquire)) return PK_OK;
+  const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(PK_ERR_CUDA, "cudaFuncSetAttribute: %s", cuda_err(e));
+  done[dev].store(true, std::memory_order_release);
+  return PK_OK;
+}
+
+// Makes `device` current for a scope.
+struct DeviceGuard {
+  int prev = -1;
+  bool switched = false;
+  cudaError_t err = cudaSuccess;
+  explicit DeviceGuard(int dev) {
+    err = cudaGetDevice(&prev);
+    if (err == cudaSuccess && prev != dev) {
+      err = cudaSetDevice(dev);
+      switched = err == cudaSuccess;
+    }
+  }
+  ~DeviceGuard() {
+    if (switched) cudaSetDevice(prev);
+  }
+};
+int check_arch(int device);
+int validate_cache(const pk_cache* c);
+void clear_error();
 
 template <typename T>
 inline T* at(const pk_problem& p, size_t off) {
