@@ -36,9 +36,9 @@ int encode_map5(CUtensorMap* m, const void* base, const uint64_t dims[5], const 
   return PK_OK;
 }
 
-int attend_map(CUtensorMap* m, const AttendParams& p, const void* base, const int64_t* stride, int line, int lines, int esz, int box) {
+int attend_map(CUtensorMap* m, const AttendParams& p, const void* base, const int64_t* stride, int line, int lines, int esz, int box, int box_lines) {
   const uint64_t row = static_cast<uint64_t>(line) * lines;  // bytes
-  const uint32_t boxes[5] = {static_cast<uint32_t>(line / esz), static_cast<uint32_t>(box), static_cast<uint32_t>(lines), 1, 1};
+  const uint32_t boxes[5] = {static_cast<uint32_t>(line / esz), static_cast<uint32_t>(box), static_cast<uint32_t>(box_lines), 1, 1};
   if (p.table) {
     // the whole pool, so that a page index outside it reads as zeros
     const uint64_t page = row * p.page;
@@ -84,7 +84,17 @@ bool mappable(const void* base, const int64_t* stride, const int64_t* dims) {
 }
 size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-int few_rows(const AttendParams& a, int head_dim, int dtype, bool i8, int device, cudaStream_t st) {
+// Which kernel: the few-row one reads K and V at the speed of memory for up to 64 rows of a key head; more
+// rows are worth the tensor cores' larger tiles.  8-bit caches have the few-row kernel only.
+bool wide(int rows, bool i8) { return !i8 && rows > 64; }
+
+uint64_t attend_workspace(int batch, int kv_heads, int rows, int head_dim, bool i8) {
+  const uint64_t n = wide(rows, i8) ? wide_rows_workspace(batch, kv_heads, rows, head_dim) : few_rows_workspace(rows, head_dim);
+  return n ? n : 256;
+}
+
+int attend(const AttendParams& a, int head_dim, int dtype, bool i8, int device, cudaStream_t st) {
+  if (wide(a.rows, i8)) return dtype == PK_F16 ? launch_wide_rows_f16(a, head_dim, device, st) : launch_wide_rows_bf16(a, head_dim, device, st);
   return dtype == PK_F16 ? launch_few_rows_f16(a, head_dim, i8, device, st) : launch_few_rows_bf16(a, head_dim, i8, device, st);
 }
 
@@ -105,7 +115,7 @@ DenseLayout dense_layout(const pk_window_problem& p) {
   l.v = off;
   if (l.pack_v) off += align256(bytes);
   l.work = off;
-  off += few_rows_workspace(p.heads / p.kv_heads * p.q_len, p.head_dim);
+  off += attend_workspace(p.batch, p.kv_heads, p.heads / p.kv_heads * p.q_len, p.head_dim, false);
   l.total = off;
   return l;
 }
@@ -178,7 +188,7 @@ int validate_query(const pk_cache* c, const pk_cache_query* q, bool launching) {
     if (!q->out || (reinterpret_cast<uintptr_t>(q->out) & 15)) return fail(PK_ERR_BAD_ARG, "cache_attention: output must be a 16-byte aligned device pointer");
     if (!q->workspace || (reinterpret_cast<uintptr_t>(q->workspace) & 255))
       return fail(PK_ERR_WORKSPACE, "cache_attention: workspace must be a 256-byte aligned device pointer");
-    const uint64_t need = few_rows_workspace(q->heads / c->kv_heads * q->tokens, c->head_dim);
+    const uint64_t need = attend_workspace(c->batch, c->kv_heads, q->heads / c->kv_heads * q->tokens, c->head_dim, c->dtype == PK_I8);
     if (q->workspace_bytes < need)
       return fail(PK_ERR_WORKSPACE, "cache_attention: workspace too small: %llu bytes given, %llu needed",
                   static_cast<unsigned long long>(q->workspace_bytes), static_cast<unsigned long long>(need));
@@ -248,7 +258,7 @@ PK_API int pk_window_attention_fwd(const pk_window_problem* pp) {
   a.scale_log2 = p.scale * kLog2e;
   a.partial = reinterpret_cast<float*>(ws + l.work);
   a.host_status = fault_word_device_ptr(p.device);
-  return few_rows(a, p.head_dim, p.dtype, false, p.device, st);
+  return attend(a, p.head_dim, p.dtype, false, p.device, st);
 }
 
 PK_API int pk_cache_attention_workspace_bytes(const pk_cache* c, const pk_cache_query* q, uint64_t* bytes) {
@@ -256,7 +266,7 @@ PK_API int pk_cache_attention_workspace_bytes(const pk_cache* c, const pk_cache_
   if (!bytes) return fail(PK_ERR_BAD_ARG, "null size pointer");
   const int rc = validate_query(c, q, false);
   if (rc) return rc;
-  *bytes = few_rows_workspace(q->heads / c->kv_heads * q->tokens, c->head_dim);
+  *bytes = attend_workspace(c->batch, c->kv_heads, q->heads / c->kv_heads * q->tokens, c->head_dim, c->dtype == PK_I8);
   return PK_OK;
 }
 
@@ -289,7 +299,7 @@ PK_API int pk_cache_attention_fwd(const pk_cache* c, const pk_cache_query* q) {
   a.scale_log2 = q->scale * kLog2e;
   a.partial = static_cast<float*>(q->workspace);
   a.host_status = fault_word_device_ptr(c->device);
-  return few_rows(a, c->head_dim, q->dtype, i8, c->device, st);
+  return attend(a, c->head_dim, q->dtype, i8, c->device, st);
 }
 
 }  // extern "C"

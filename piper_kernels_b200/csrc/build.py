@@ -17,8 +17,8 @@ from pathlib import Path
 CSRC = Path(__file__).resolve().parent
 PKG = CSRC.parent
 LIB = PKG / "libpiper_b200.so"
-SOURCES = ["cabi.cu", "prepass.cu", "fused_attention.cu", "attend.cu", "few_rows_f16.cu", "few_rows_bf16.cu", "cache_pages.cu"]
-HEADERS = ["pk_internal.h", "pk_ptx.cuh", "pk_attend.cuh", "few_rows.cuh", "../../include/piper_b200.h"]
+SOURCES = ["cabi.cu", "prepass.cu", "fused_attention.cu", "attend.cu", "few_rows_f16.cu", "few_rows_bf16.cu", "wide_rows_f16.cu", "wide_rows_bf16.cu", "cache_pages.cu"]
+HEADERS = ["pk_internal.h", "pk_ptx.cuh", "pk_attend.cuh", "few_rows.cuh", "wide_rows.cuh", "../../include/piper_b200.h"]
 
 
 def nvcc_path() -> str:

@@ -30,113 +30,13 @@
 namespace pk {
 namespace {
 
-constexpr int kTile = kAttendTile;
+constexpr int kTile = 64;  // keys per stage
 constexpr int kStages = 3;
 constexpr int kConsumers = 128;
 constexpr int kThreads = kConsumers + 32;
 constexpr int kJoinCols = 32;          // output columns that the warps of a CTA join at a time
 constexpr float kRaise = 8.f;          // a row's reference exponent follows its maximum only beyond this
 constexpr int kMaxWorkers = 2 * 148;   // two CTAs per SM
-
-// One group of query rows (batch element, row block; the same for every key head) and the key tiles
-// that any of its rows sees: `ns` tiles of sinks, then the tiles from `first` on.
-struct Span {
-  int b, rb, off, len, ns, first, n;
-  int full_lo, full_hi;  // keys that every row sees
-};
-
-template <bool TREE>
-__device__ __forceinline__ Span span_of(const AttendParams& p, int g, int rows_per_block) {
-  Span s;
-  s.b = g / p.row_blocks;
-  s.rb = g % p.row_blocks;
-  s.len = attend_len(p, s.b);
-  s.off = attend_off(p, s.b, s.len);
-  const int r0 = s.rb * rows_per_block, r1 = min(r0 + rows_per_block, p.rows) - 1;
-  const int t0 = r0 / p.group, t1 = r1 / p.group;
-  int hi, lo;
-  if (TREE) {
-    hi = min(s.len, s.off + p.tokens);
-    lo = s.off - p.window + 1;
-    s.full_hi = min(s.len, s.off);
-    s.full_lo = s.off + p.tokens - p.window;
-  } else {
-    hi = min(s.len, s.off + t1 + 1);
-    lo = s.off + t0 - p.window + 1;
-    s.full_hi = min(s.len, s.off + t0 + 1);
-    s.full_lo = s.off + t1 - p.window + 1;
-  }
-  if (s.off + t0 >= s.len) hi = 0;  // no valid row
-  hi = max(hi, 0);
-  lo = min(max(lo, 0), hi);
-  s.ns = (min(p.sinks, lo) + kTile - 1) / kTile;
-  s.first = max(lo / kTile, s.ns);
-  s.n = s.ns + max(0, (hi + kTile - 1) / kTile - s.first);
-  if (s.n == 0) s.n = 1, s.ns = 0, s.first = 0;  // rows that see nothing still have to be written
-  return s;
-}
-
-// First tile of worker w, when `total` tiles are shared out.
-__device__ __forceinline__ int64_t share_begin(int64_t total, int workers, int w) {
-  return total / workers * w + min(static_cast<int64_t>(w), total % workers);
-}
-__device__ __forceinline__ int owner_of(int64_t total, int workers, int64_t tile) {
-  const int64_t base = total / workers, extra = total % workers, big = extra * (base + 1);
-  return static_cast<int>(tile < big ? tile / (base + 1) : extra + (tile - big) / base);
-}
-
-struct Found {  // a group and the tiles in front of it
-  int64_t before;
-  int group;
-};
-
-// Tiles of the groups in front of `upto`, all key heads; by the whole CTA, threads [0, 128) count.
-
-template <bool TREE>
-__device__ __forceinline__ int64_t sum_tiles(const AttendParams& p, int rows_per_block, int upto, int64_t* red) {
-  int64_t mine = 0;
-  if (threadIdx.x < kConsumers)
-    for (int g = threadIdx.x; g < upto; g += kConsumers) mine += span_of<TREE>(p, g, rows_per_block).n;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if ((threadIdx.x & 31) == 0 && threadIdx.x < kConsumers) red[threadIdx.x >> 5] = mine;
-  __syncthreads();
-  const int64_t sum = red[0] + red[1] + red[2] + red[3];
-  __syncthreads();
-  return sum * p.kv_heads;
-}
-
-// Finds the group that holds tile `at` (0 <= at < total), 128 groups at a time.
-template <bool TREE>
-__device__ __forceinline__ Found find_group(const AttendParams& p, int rows_per_block, int64_t at, int64_t* red, Found* out) {
-  const int groups = p.batch * p.row_blocks, lane = threadIdx.x & 31;
-  int64_t before = 0;
-  if (threadIdx.x == 0) out->group = -1;
-  __syncthreads();
-  for (int g0 = 0; g0 < groups; g0 += kConsumers) {
-    const int g = g0 + threadIdx.x;
-    int64_t n = 0;
-    if (threadIdx.x < kConsumers && g < groups) n = static_cast<int64_t>(span_of<TREE>(p, g, rows_per_block).n) * p.kv_heads;
-    int64_t incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    if (lane == 31 && threadIdx.x < kConsumers) red[threadIdx.x >> 5] = incl;
-    __syncthreads();
-    if (threadIdx.x < kConsumers) {
-      int64_t base = before;
-      for (int w = 0; w < (threadIdx.x >> 5); ++w) base += red[w];
-      const int64_t b0 = base + incl - n;
-      if (n > 0 && at >= b0 && at < b0 + n) out->group = g, out->before = b0;
-    }
-    before += red[0] + red[1] + red[2] + red[3];
-    __syncthreads();
-    if (out->group >= 0) break;  // the same for every thread: written before the barrier
-  }
-  return *out;
-}
 
 template <typename T, bool I8, int D, int WM>
 struct Few {
@@ -202,41 +102,6 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   return v;
 }
 
-// Barrier of the 128 consumer threads; true when `good` holds in all of them.
-__device__ __forceinline__ bool join_vote(bool good) {
-  uint32_t all;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(all)
-      : "r"(static_cast<uint32_t>(good))
-      : "memory");
-  return all != 0;
-}
-
-template <bool TREE>
-struct Walk {  // position in the list of tiles
-  Span s;
-  int g, h, tile;
-  template <int ROWS>
-  __device__ __forceinline__ void start(const AttendParams& p, const Found& f, int64_t at) {
-    g = f.group;
-    s = span_of<TREE>(p, g, ROWS);
-    const int64_t rel = at - f.before;
-    h = static_cast<int>(rel / s.n);
-    tile = static_cast<int>(rel % s.n);
-  }
-  template <int ROWS>
-  __device__ __forceinline__ void next(const AttendParams& p) {
-    if (++tile < s.n) return;
-    tile = 0;
-    if (++h < p.kv_heads) return;
-    h = 0;
-    if (++g < p.batch * p.row_blocks) s = span_of<TREE>(p, g, ROWS);
-  }
-  __device__ __forceinline__ int key() const { return (tile < s.ns ? tile : s.first + tile - s.ns) * kTile; }
-};
-
 template <typename T, bool I8, int D, int WM, bool TREE>
 __global__ void __launch_bounds__(kThreads, 2)
 few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttendParams p) {
@@ -260,12 +125,12 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   __syncthreads();
 
   const int groups = p.batch * p.row_blocks;
-  const int64_t total = sum_tiles<TREE>(p, C::ROWS, groups, red);
+  const int64_t total = sum_tiles<TREE, kTile, C::ROWS>(p, groups, red);
   const int64_t w0 = share_begin(total, gridDim.x, blockIdx.x), w1 = share_begin(total, gridDim.x, blockIdx.x + 1);
   if (w0 >= w1) return;
-  const Found f = find_group<TREE>(p, C::ROWS, w0, red, found);
-  Walk<TREE> walk;
-  walk.template start<C::ROWS>(p, f, w0);
+  const Found f = find_group<TREE, kTile, C::ROWS>(p, w0, red, found);
+  Walk<TREE, kTile, C::ROWS> walk;
+  walk.start(p, f, w0);
 
   if (warp == kConsumers / 32) {
     // ---------------------------------------------------------------- producer
@@ -273,7 +138,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       const int box = p.table ? min(p.page, kTile) : kTile;
       int last = -1;
       bool ok = true;
-      for (int64_t w = w0; w < w1; ++w, walk.template next<C::ROWS>(p)) {
+      for (int64_t w = w0; w < w1; ++w, walk.next(p)) {
         const int i = static_cast<int>(w - w0), st = i % kStages;
         if (i >= kStages && !mbar_wait_bounded(bars + 8 * (kStages + st), ((i / kStages) - 1) & 1, abort_flag, 61)) { ok = false; break; }
         const uint32_t full = bars + 8 * st, dst = base + st * C::STAGE;
@@ -550,7 +415,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       if (!ok) l[x] = __int_as_float(0x7FC00000);
       if (c4 == 0) ml[warp * 16 + g8 + 8 * x] = make_float2(m[x], l[x]);
     }
-    ok = join_vote(ok && *abort_flag == 0);  // the same answer in every warp: they leave together
+    ok = vote_barrier(1, ok && *abort_flag == 0);  // the same answer in every warp: they leave together
     const int slot = blockIdx.x * 2 + (unit_from == 0 && w - unit_tiles != w0 ? 1 : 0);
     float* piece = p.partial + static_cast<int64_t>(slot) * C::ROWS * (D + 2);
     // thread -> (row, four consecutive columns) of the CTA's rows; a row's columns belong to 8 neighbouring threads
@@ -628,68 +493,9 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     }
     // the next unit
     walk.tile = unit_from + unit_tiles - 1;
-    walk.template next<C::ROWS>(p);
+    walk.next(p);
   }
   if (tid == 0 && *abort_flag != 0 && p.host_status != nullptr) atomicCAS_system(p.host_status, 0, *abort_flag);
-}
-
-// Joins the pieces of every unit that more than one CTA worked on.  One CTA per unit (batch element,
-// row block, key head); units that one CTA finished are left alone.
-template <typename T, bool I8, int D, int WM, bool TREE>
-__global__ void __launch_bounds__(kConsumers) join_kernel(const __grid_constant__ AttendParams p, int workers) {
-  using C = Few<T, I8, D, WM>;
-  __shared__ int64_t red[4];
-  __shared__ TreeMasks tm;
-  const int unit = blockIdx.x, g = unit / p.kv_heads, h = unit % p.kv_heads, groups = p.batch * p.row_blocks;
-  cudaGridDependencySynchronize();
-  const int64_t total = sum_tiles<TREE>(p, C::ROWS, groups, red);
-  int64_t u0 = sum_tiles<TREE>(p, C::ROWS, g, red);
-  const Span s = span_of<TREE>(p, g, C::ROWS);
-  u0 += static_cast<int64_t>(h) * s.n;
-  const int c0 = owner_of(total, workers, u0), c1 = owner_of(total, workers, u0 + s.n - 1);
-  if (c0 == c1) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (TREE) {
-    if (warp == 0) build_tree(p, s.b, s.off, lane, &tm);
-    __syncthreads();
-  }
-  const bool first_second = u0 > share_begin(total, workers, c0);  // its first CTA began with another unit
-  constexpr int E = D / 32;
-  const int r1 = min(p.rows - s.rb * C::ROWS, C::ROWS);
-  for (int r = warp; r < r1; r += kConsumers / 32) {
-    float mx = -INFINITY, sum = 0.f, acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int c = c0 + lane; c <= c1; c += 32)
-      mx = fmaxf(mx, p.partial[(static_cast<int64_t>(c * 2 + (c == c0 && first_second)) * C::ROWS + r) * (D + 2) + D]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const float* src = p.partial + (static_cast<int64_t>(c * 2 + (c == c0 && first_second)) * C::ROWS + r) * (D + 2);
-      const float2 st = *reinterpret_cast<const float2*>(src + D);
-      const float wgt = st.x == mx ? 1.f : ex2_approx(st.x - mx);
-      sum = fmaf(st.y, wgt, sum);
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(src + lane * E + e);
-        acc[e] = fmaf(v.x, wgt, acc[e]);
-        acc[e + 1] = fmaf(v.y, wgt, acc[e + 1]);
-      }
-    }
-    const int row = s.rb * C::ROWS + r, t = row / p.group, idx = s.off + t;
-    const float inv = idx >= 0 && idx < s.len && sum != 0.f ? 1.f / sum : 0.f;
-    T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + row % p.group) * p.tokens + t) * D + lane * E;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float a = inv == 0.f ? 0.f : acc[e] * inv, b = inv == 0.f ? 0.f : acc[e + 1] * inv;
-      bad |= !(fabsf(a) <= 3.0e38f) || !(fabsf(b) <= 3.0e38f);
-      *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(a, b);
-    }
-    __syncwarp();
-    if (__any_sync(0xffffffffu, bad)) plain_row<T, I8, D>(p, s.b, h, row, s.off, s.len, row_view(p, s.off, s.len, t, TREE ? &tm : nullptr), TREE);
-  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -702,8 +508,8 @@ int launch(AttendParams p, int device, cudaStream_t st) {
   p.row_blocks = (p.rows + C::ROWS - 1) / C::ROWS;
   CUtensorMap tk, tv;
   int rc;
-  if ((rc = attend_map(&tk, p, p.k, p.k_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < kTile ? p.page : kTile) : kTile))) return rc;
-  if ((rc = attend_map(&tv, p, p.v, p.v_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < kTile ? p.page : kTile) : kTile))) return rc;
+  if ((rc = attend_map(&tk, p, p.k, p.k_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < kTile ? p.page : kTile) : kTile, C::HALVES))) return rc;
+  if ((rc = attend_map(&tv, p, p.v, p.v_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < kTile ? p.page : kTile) : kTile, C::HALVES))) return rc;
   if ((rc = allow_smem<few_rows_kernel<T, I8, D, WM, TREE>>(C::SMEM, device))) return rc;
   // No more CTAs than there can be tiles.
   const int64_t most = static_cast<int64_t>(p.batch) * p.row_blocks * p.kv_heads * (((p.table ? p.width * p.page : p.kv_len) + kTile - 1) / kTile + 1);
@@ -711,7 +517,7 @@ int launch(AttendParams p, int device, cudaStream_t st) {
   cudaError_t e = launch_chained(few_rows_kernel<T, I8, D, WM, TREE>, dim3(p.workers), dim3(kThreads), C::SMEM, st, tk, tv, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "attention kernel launch failed: %s", cuda_err(e));
-  e = launch_chained(join_kernel<T, I8, D, WM, TREE>, dim3(p.batch * p.row_blocks * p.kv_heads), dim3(kConsumers), 0, st, p, p.workers);
+  e = launch_chained(join_kernel<T, I8, D, TREE, kTile, C::ROWS>, dim3(p.batch * p.row_blocks * p.kv_heads), dim3(kConsumers), 0, st, p, p.workers);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "join kernel launch failed: %s", cuda_err(e));
   return PK_OK;

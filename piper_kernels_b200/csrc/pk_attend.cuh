@@ -1,4 +1,4 @@
-// What the 16-bit attention kernels (few_rows.cuh) share: the problem they are
+// What the 16-bit attention kernels (few_rows.cuh, wide_rows.cuh) share: the problem they are
 // given, which keys a query row sees, and the plain evaluation of one row.
 //
 // Both operators are one formula.  Batch element b holds len(b) keys; query token t stands at
@@ -20,7 +20,6 @@
 
 namespace pk {
 
-constexpr int kAttendTile = 64;      // keys per step of the few-row kernel
 constexpr int kMaxTreeTokens = 64;   // a token's visible drafted tokens are one 64-bit mask
 constexpr int kNoWindow = 1 << 30;   // larger than any index
 
@@ -114,6 +113,18 @@ __device__ __forceinline__ void build_tree(const AttendParams& p, int b, int off
     tm->sees[t] = keep;
   }
   __syncwarp();
+}
+
+// Barrier `id` of 128 threads; true when `good` holds in all of them.
+__device__ __forceinline__ bool vote_barrier(int id, bool good) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(id), "r"(static_cast<uint32_t>(good))
+      : "memory");
+  return all != 0;
 }
 
 // What one query row sees: keys below `lim`, those above `low` or below the sinks; in a tree also
@@ -229,13 +240,202 @@ __device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, in
   for (int e = 0; e < E; ++e) out[e] = from_f32<T>(l == 0.f ? 0.f : acc[e] / l);
 }
 
-// Copy map of K or V: [line, key, lines of a row, head, batch element or page], boxes of `box` keys.
+// ---------------------------------------------------------------------------------------
+// Sharing the work: the keys of all groups of query rows and key heads form one list of TILE-key
+// tiles, of which every CTA takes an equal, contiguous part.
+// ---------------------------------------------------------------------------------------
+// One group of query rows (batch element, row block; the same for every key head) and the key tiles
+// that any of its rows sees: `ns` tiles of sinks, then the tiles from `first` on.
+struct Span {
+  int b, rb, off, len, ns, first, n;
+  int full_lo, full_hi;  // keys that every row sees
+};
+
+template <bool TREE, int TILE, int ROWS>
+__device__ __forceinline__ Span span_of(const AttendParams& p, int g) {
+  Span s;
+  s.b = g / p.row_blocks;
+  s.rb = g % p.row_blocks;
+  s.len = attend_len(p, s.b);
+  s.off = attend_off(p, s.b, s.len);
+  const int r0 = s.rb * ROWS, r1 = min(r0 + ROWS, p.rows) - 1;
+  const int t0 = r0 / p.group, t1 = r1 / p.group;
+  int hi, lo;
+  if (TREE) {
+    hi = min(s.len, s.off + p.tokens);
+    lo = s.off - p.window + 1;
+    s.full_hi = min(s.len, s.off);
+    s.full_lo = s.off + p.tokens - p.window;
+  } else {
+    hi = min(s.len, s.off + t1 + 1);
+    lo = s.off + t0 - p.window + 1;
+    s.full_hi = min(s.len, s.off + t0 + 1);
+    s.full_lo = s.off + t1 - p.window + 1;
+  }
+  if (s.off + t0 >= s.len) hi = 0;  // no valid row
+  hi = max(hi, 0);
+  lo = min(max(lo, 0), hi);
+  s.ns = (min(p.sinks, lo) + TILE - 1) / TILE;
+  s.first = max(lo / TILE, s.ns);
+  s.n = s.ns + max(0, (hi + TILE - 1) / TILE - s.first);
+  if (s.n == 0) s.n = 1, s.ns = 0, s.first = 0;  // rows that see nothing still have to be written
+  return s;
+}
+
+// First tile of worker w, when `total` tiles are shared out.
+__device__ __forceinline__ int64_t share_begin(int64_t total, int workers, int w) {
+  return total / workers * w + min(static_cast<int64_t>(w), total % workers);
+}
+__device__ __forceinline__ int owner_of(int64_t total, int workers, int64_t tile) {
+  const int64_t base = total / workers, extra = total % workers, big = extra * (base + 1);
+  return static_cast<int>(tile < big ? tile / (base + 1) : extra + (tile - big) / base);
+}
+
+constexpr int kCounters = 128;  // threads that count tiles
+
+struct Found {  // a group and the tiles in front of it
+  int64_t before;
+  int group;
+};
+
+// Tiles of the groups in front of `upto`, all key heads; by the whole CTA, threads [0, 128) count.
+template <bool TREE, int TILE, int ROWS>
+__device__ __forceinline__ int64_t sum_tiles(const AttendParams& p, int upto, int64_t* red) {
+  int64_t mine = 0;
+  if (threadIdx.x < kCounters)
+    for (int g = threadIdx.x; g < upto; g += kCounters) mine += span_of<TREE, TILE, ROWS>(p, g).n;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if ((threadIdx.x & 31) == 0 && threadIdx.x < kCounters) red[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  const int64_t sum = red[0] + red[1] + red[2] + red[3];
+  __syncthreads();
+  return sum * p.kv_heads;
+}
+
+// Finds the group that holds tile `at` (0 <= at < total), 128 groups at a time.
+template <bool TREE, int TILE, int ROWS>
+__device__ __forceinline__ Found find_group(const AttendParams& p, int64_t at, int64_t* red, Found* out) {
+  const int groups = p.batch * p.row_blocks, lane = threadIdx.x & 31;
+  int64_t before = 0;
+  if (threadIdx.x == 0) out->group = -1;
+  __syncthreads();
+  for (int g0 = 0; g0 < groups; g0 += kCounters) {
+    const int g = g0 + threadIdx.x;
+    int64_t n = 0;
+    if (threadIdx.x < kCounters && g < groups) n = static_cast<int64_t>(span_of<TREE, TILE, ROWS>(p, g).n) * p.kv_heads;
+    int64_t incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31 && threadIdx.x < kCounters) red[threadIdx.x >> 5] = incl;
+    __syncthreads();
+    if (threadIdx.x < kCounters) {
+      int64_t base = before;
+      for (int w = 0; w < (threadIdx.x >> 5); ++w) base += red[w];
+      const int64_t b0 = base + incl - n;
+      if (n > 0 && at >= b0 && at < b0 + n) out->group = g, out->before = b0;
+    }
+    before += red[0] + red[1] + red[2] + red[3];
+    __syncthreads();
+    if (out->group >= 0) break;  // the same for every thread: written before the barrier
+  }
+  return *out;
+}
+
+template <bool TREE, int TILE, int ROWS>
+struct Walk {  // position in the list of tiles
+  Span s;
+  int g, h, tile;
+  __device__ __forceinline__ void start(const AttendParams& p, const Found& f, int64_t at) {
+    g = f.group;
+    s = span_of<TREE, TILE, ROWS>(p, g);
+    const int64_t rel = at - f.before;
+    h = static_cast<int>(rel / s.n);
+    tile = static_cast<int>(rel % s.n);
+  }
+  __device__ __forceinline__ void next(const AttendParams& p) {
+    if (++tile < s.n) return;
+    tile = 0;
+    if (++h < p.kv_heads) return;
+    h = 0;
+    if (++g < p.batch * p.row_blocks) s = span_of<TREE, TILE, ROWS>(p, g);
+  }
+  __device__ __forceinline__ int key() const { return (tile < s.ns ? tile : s.first + tile - s.ns) * TILE; }
+};
+
+// Joins the pieces of every unit that more than one CTA worked on.  One CTA per unit (batch element,
+// row block, key head); units that one CTA finished are left alone.
+template <typename T, bool I8, int D, bool TREE, int TILE, int ROWS>
+__global__ void __launch_bounds__(kCounters) join_kernel(const __grid_constant__ AttendParams p, int workers) {
+  __shared__ int64_t red[4];
+  __shared__ TreeMasks tm;
+  const int unit = blockIdx.x, g = unit / p.kv_heads, h = unit % p.kv_heads, groups = p.batch * p.row_blocks;
+  cudaGridDependencySynchronize();
+  const int64_t total = sum_tiles<TREE, TILE, ROWS>(p, groups, red);
+  int64_t u0 = sum_tiles<TREE, TILE, ROWS>(p, g, red);
+  const Span s = span_of<TREE, TILE, ROWS>(p, g);
+  u0 += static_cast<int64_t>(h) * s.n;
+  const int c0 = owner_of(total, workers, u0), c1 = owner_of(total, workers, u0 + s.n - 1);
+  if (c0 == c1) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (TREE) {
+    if (warp == 0) build_tree(p, s.b, s.off, lane, &tm);
+    __syncthreads();
+  }
+  const bool first_second = u0 > share_begin(total, workers, c0);  // its first CTA began with another unit
+  constexpr int E = D / 32;
+  const int r1 = min(p.rows - s.rb * ROWS, ROWS);
+  for (int r = warp; r < r1; r += kCounters / 32) {
+    float mx = -INFINITY, sum = 0.f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int c = c0 + lane; c <= c1; c += 32)
+      mx = fmaxf(mx, p.partial[(static_cast<int64_t>(c * 2 + (c == c0 && first_second)) * ROWS + r) * (D + 2) + D]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const float* src = p.partial + (static_cast<int64_t>(c * 2 + (c == c0 && first_second)) * ROWS + r) * (D + 2);
+      const float2 st = *reinterpret_cast<const float2*>(src + D);
+      const float wgt = st.x == mx ? 1.f : ex2_approx(st.x - mx);
+      sum = fmaf(st.y, wgt, sum);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(src + lane * E + e);
+        acc[e] = fmaf(v.x, wgt, acc[e]);
+        acc[e + 1] = fmaf(v.y, wgt, acc[e + 1]);
+      }
+    }
+    const int row = s.rb * ROWS + r, t = row / p.group, idx = s.off + t;
+    const float inv = idx >= 0 && idx < s.len && sum != 0.f ? 1.f / sum : 0.f;
+    T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + row % p.group) * p.tokens + t) * D + lane * E;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float a = inv == 0.f ? 0.f : acc[e] * inv, b = inv == 0.f ? 0.f : acc[e + 1] * inv;
+      bad |= !(fabsf(a) <= 3.0e38f) || !(fabsf(b) <= 3.0e38f);
+      *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(a, b);
+    }
+    __syncwarp();
+    if (__any_sync(0xffffffffu, bad)) plain_row<T, I8, D>(p, s.b, h, row, s.off, s.len, row_view(p, s.off, s.len, t, TREE ? &tm : nullptr), TREE);
+  }
+}
+
+// Copy map of K or V: [line, key, lines of a row, head, batch element or page], boxes of `box` keys and
+// `box_lines` lines.
 // `stride`: dense element strides (batch, head, key); paged caches are contiguous.
-int attend_map(CUtensorMap* m, const AttendParams& p, const void* base, const int64_t* stride, int line, int lines, int esz, int box);
+int attend_map(CUtensorMap* m, const AttendParams& p, const void* base, const int64_t* stride, int line, int lines, int esz, int box, int box_lines);
 
 // few_rows.cuh
 int launch_few_rows_f16(const AttendParams& p, int head_dim, bool i8, int device, cudaStream_t st);
 int launch_few_rows_bf16(const AttendParams& p, int head_dim, bool i8, int device, cudaStream_t st);
 uint64_t few_rows_workspace(int rows, int head_dim);
+// wide_rows.cuh
+int launch_wide_rows_f16(const AttendParams& p, int head_dim, int device, cudaStream_t st);
+int launch_wide_rows_bf16(const AttendParams& p, int head_dim, int device, cudaStream_t st);
+uint64_t wide_rows_workspace(int batch, int kv_heads, int rows, int head_dim);
 
 }  // namespace pk

@@ -1,0 +1,559 @@
+// Attention of many query rows per key head (prompts, large drafted trees), 16-bit keys and values,
+// dense or paged, on the tensor cores.  The formula is in pk_attend.cuh.
+//
+// What bounds it: 4 D operations per visible pair against one exponential, so the tensor pipe and
+// the exponential unit about equally (a 128 x 128 tile at D = 128 takes 1024 cycles of each).
+//
+// One CTA per SM works on 256 query rows of one key head (two 128-row tiles; row = token * group +
+// query head of the group, so that a tile's rows stand close together and share their window) over
+// 128-key tiles:
+//   - two softmax warpgroups, one per row tile, a thread per row: scores from tensor memory, running
+//     maximum and sum in registers, probabilities back to tensor memory over the scores;
+//   - an MMA warp: S = Q K^T from shared memory, O += P V with P from tensor memory; the two row
+//     tiles take turns, so that one's softmax runs beside the other's products;
+//   - a copy warp: K and V tiles by TMA through one ring.
+// Tensor memory: two score buffers of 128 columns, two accumulators of D columns.  A score buffer's
+// next product is issued behind the product that reads the probabilities in it; products run in the
+// order of issue.  An accumulator is rescaled by its softmax warpgroup, and only when a row's maximum
+// has grown by more than 2^8 since its last reference.
+// V is read as it lies in memory (keys in rows): the B operand is taken transposed.
+#pragma once
+
+#include "pk_attend.cuh"
+
+namespace pk {
+namespace {
+
+constexpr int kWideTile = 128;
+constexpr int kWideRows = 256;
+constexpr int kWideThreads = 3 * 128;  // two softmax warpgroups, one with the MMA and the copy warp
+// Registers of a thread after the split; setmaxnreg only moves what the CTA was launched with.
+constexpr int kWideLaunchRegs = 168, kSoftmaxRegs = 216, kHelperRegs = 64;
+static_assert((2 * kSoftmaxRegs + kHelperRegs) * 128 <= kWideThreads * kWideLaunchRegs, "register split exceeds the CTA's registers");
+constexpr float kWideRaise = 8.f;
+constexpr int kWideWorkers = 148;
+constexpr int64_t kWideShareBelow = 4 * kWideWorkers;
+constexpr int kThere = 8;  // a copy is issued at most six key tiles ahead of a tile whose V is still in use
+
+#define WIDE_ALL(x) __all_sync(0xffffffffu, (x))
+
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+template <int D>
+struct Wide {
+  static constexpr int HALF = kWideTile * 128;                 // 128 rows of 64 features
+  static constexpr int TILE_BYTES = HALF * (D / 64);           // a K, V or Q tile
+  static constexpr int STAGES = D == 128 ? 5 : 10;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_RING = 2 * TILE_BYTES;
+  static constexpr int OFF_TREE = OFF_RING + STAGES * TILE_BYTES;
+  static constexpr int OFF_BAR = OFF_TREE + 2 * static_cast<int>(sizeof(TreeMasks));
+  static constexpr int BARS = 2 * STAGES + 2 * 4;  // ring full / empty; q_full, s_full, p_full, o_done per row tile
+  static constexpr int OFF_RED = OFF_BAR + BARS * 8;
+  static constexpr int OFF_THERE = OFF_RED + 64;
+  static constexpr int OFF_MISC = OFF_THERE + kThere * 4;
+  static constexpr int SMEM = OFF_MISC + 16;
+  static constexpr uint32_t COL_S = 0, COL_O = 256;
+};
+
+// Both operands 16-bit, 32-bit accumulator.  B transposed: its rows lie along the contraction.
+template <typename T>
+__host__ __device__ constexpr uint32_t wide_idesc(int n, bool b_transposed) {
+  const uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_transposed ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Transposed operand: 64 contiguous features per 128-byte line, one key per line; groups of eight
+// keys 1024 bytes apart, the next 64 features HALF bytes further.
+__device__ __forceinline__ uint64_t v_desc(uint32_t addr, int half) {
+  return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(half >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+
+// What one CTA does next: tiles [tile, tile + count) of one unit.  Every role walks the same list.
+template <bool TREE>
+struct Segments {
+  Walk<TREE, kWideTile, kWideRows> walk;
+  int64_t left;
+  __device__ __forceinline__ int count() const { return static_cast<int>(min(static_cast<int64_t>(walk.s.n - walk.tile), left)); }
+  __device__ __forceinline__ void advance(const AttendParams& p) {
+    const int n = count();
+    left -= n;
+    walk.tile += n - 1;
+    walk.next(p);
+  }
+};
+
+// The keys that the rows of one 128-row tile see, for skipping key tiles that only the other needs.
+struct Reach {
+  int lo, hi;
+};
+template <bool TREE>
+__device__ __forceinline__ Reach reach_of(const AttendParams& p, const Span& s, int tile) {
+  const int r0 = s.rb * kWideRows + tile * 128, r1 = min(r0 + 128, p.rows) - 1;
+  Reach r{0, 0};
+  if (r0 >= p.rows) return r;
+  const int t0 = r0 / p.group, t1 = r1 / p.group;
+  if (s.off + t0 >= s.len) return r;
+  r.hi = max(0, TREE ? min(s.len, s.off + p.tokens) : min(s.len, s.off + t1 + 1));
+  r.lo = max(0, (TREE ? s.off : s.off + t0) - p.window + 1);
+  return r;
+}
+__device__ __forceinline__ bool needs(const Reach& r, int j0, int sinks) { return j0 < r.hi && (j0 + kWideTile > r.lo || j0 < sinks); }
+
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }  // bits [0, n)
+
+// Which of the keys [j, j + 32) a row sees.
+template <bool TREE>
+__device__ __forceinline__ uint32_t seen_bits(const RowView& v, int j, int off, int sinks) {
+  uint32_t bits = below(v.lim - j) & (~below(v.low + 1 - j) | below(sinks - j));
+  if (TREE) {
+    const int a = off - j;  // bit of the first drafted token
+    bits &= below(a);
+    if (a < 32 && a > -64) bits |= a >= 0 ? static_cast<uint32_t>(v.mask << a) : static_cast<uint32_t>(v.mask >> -a);
+  }
+  return bits;
+}
+
+template <typename T, int D, bool TREE>
+__global__ void __launch_bounds__(kWideThreads, 1)
+wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttendParams p) {
+  using C = Wide<D>;
+  constexpr int ST = C::STAGES;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_MISC + 4);
+  volatile uint32_t* there = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_THERE);
+  int64_t* red = reinterpret_cast<int64_t*>(smem + C::OFF_RED);
+  Found* found = reinterpret_cast<Found*>(smem + C::OFF_RED + 32);
+  const uint32_t bars = base + C::OFF_BAR;
+  auto full = [&](int i) { return bars + 8 * i; };
+  auto empty = [&](int i) { return bars + 8 * (ST + i); };
+  auto q_full = [&](int i) { return bars + 8 * (2 * ST + i); };
+  auto s_full = [&](int i) { return bars + 8 * (2 * ST + 2 + i); };
+  auto p_full = [&](int i) { return bars + 8 * (2 * ST + 4 + i); };
+  auto o_done = [&](int i) { return bars + 8 * (2 * ST + 6 + i); };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int MMA_WARP = 8, COPY_WARP = 9;
+
+  if (tid < C::BARS) {
+    const int kind = tid < 2 * ST ? 1 : (tid - 2 * ST) / 2;
+    mbar_init(bars + 8 * tid, tid >= 2 * ST && (kind == 0 || kind == 2) ? 128 : 1);  // q_full, p_full: a warpgroup
+    fence_barrier_init();
+  }
+  if (tid == 0) *abort_flag = 0;
+  if (warp == MMA_WARP) {
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  if (warp == COPY_WARP && lane == 0) { prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
+  cudaGridDependencySynchronize();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // This CTA's part: an equal share of all tiles, or (when there are many units) one unit.
+  Segments<TREE> seg;
+  if (p.workers) {
+    const int64_t total = sum_tiles<TREE, kWideTile, kWideRows>(p, p.batch * p.row_blocks, red);
+    const int64_t w0 = share_begin(total, gridDim.x, blockIdx.x), w1 = share_begin(total, gridDim.x, blockIdx.x + 1);
+    seg.left = w1 - w0;
+    if (seg.left > 0) {
+      const Found f = find_group<TREE, kWideTile, kWideRows>(p, w0, red, found);
+      seg.walk.start(p, f, w0);
+    }
+  } else {
+    seg.walk.g = blockIdx.x / p.kv_heads;
+    seg.walk.h = blockIdx.x % p.kv_heads;
+    seg.walk.tile = 0;
+    seg.walk.s = span_of<TREE, kWideTile, kWideRows>(p, seg.walk.g);
+    seg.left = seg.walk.s.n;
+  }
+
+  if (warp >= 8) setmaxnreg_dec<kHelperRegs>();
+  if (warp == COPY_WARP) {
+    // ---------------------------------------------------------------- copies
+    if (lane == 0) {
+      const int box = p.table ? min(p.page, kWideTile) : kWideTile;
+      int n = 0;  // tiles issued, K and V counted one after the other
+      bool ok = true;
+      for (; ok && seg.left > 0; seg.advance(p)) {
+        const int count = seg.count(), from = seg.walk.tile;
+        for (int u = 0; ok && u < count; ++u) {
+          const Span& s = seg.walk.s;
+          const int j0 = (from + u < s.ns ? from + u : s.first + from + u - s.ns) * kWideTile;
+          int pages[kWideTile / 16];
+          uint32_t mask = 1u;
+          if (p.table) {
+            mask = 0;
+#pragma unroll
+            for (int x = 0; x < kWideTile / 16; ++x) {
+              const int j = j0 + x * box;
+              pages[x] = (x * box < kWideTile && j < s.len) ? attend_page(p, s.b, j) : -1;
+              if (pages[x] >= 0) mask |= 1u << x;
+            }
+          }
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv, ++n) {
+            const int st = n % ST;
+            if (n >= ST && !mbar_wait_bounded(empty(st), ((n / ST) - 1) & 1, abort_flag, 71)) { ok = false; break; }
+            const uint32_t dst = base + C::OFF_RING + st * C::TILE_BYTES;
+            const CUtensorMap* tmap = kv ? &tm_v : &tm_k;
+            if (kv == 0) there[(n / 2) % kThere] = mask;
+            mbar_expect_tx(full(st), C::TILE_BYTES);
+            if (!p.table) {
+              const int64_t* str = kv ? p.v_stride : p.k_stride;
+              tma_load_5d(dst, tmap, full(st), 0, j0, 0, str[1] ? seg.walk.h : 0, str[0] ? s.b : 0);
+            } else {
+#pragma unroll
+              for (int x = 0; x < kWideTile / 16; ++x) {
+                if (x * box >= kWideTile) break;
+                const int row = (j0 + x * box) & (p.page - 1);
+                const int c4 = pages[x] >= 0 ? p.page_base + pages[x] : 0x7fffffff;
+#pragma unroll
+                for (int hf = 0; hf < D / 64; ++hf)
+                  tma_load_5d(dst + hf * C::HALF + x * box * 128, tmap, full(st), 0, row, hf, seg.walk.h, c4);
+              }
+            }
+          }
+        }
+      }
+      if (*abort_flag != 0) {  // let the copies that were issued land before the CTA returns
+        for (int i = max(0, n - ST); i < n; ++i) mbar_wait_quiet(full(i % ST), (i / ST) & 1, 100000);
+      }
+    }
+  } else if (warp == MMA_WARP) {
+    // ---------------------------------------------------------------- products
+    constexpr uint32_t id_s = wide_idesc<T>(kWideTile, false), id_o = wide_idesc<T>(D, true);
+    int n = 0;                     // tiles consumed, K and V counted one after the other
+    int np[2] = {0, 0}, nq = 0;    // probability tiles, segments
+    bool ok = true;
+    for (; ok && seg.left > 0; seg.advance(p), ++nq) {
+      const Span& s = seg.walk.s;
+      const int count = seg.count(), from = seg.walk.tile;
+      const Reach reach[2] = {reach_of<TREE>(p, s, 0), reach_of<TREE>(p, s, 1)};
+      bool begun[2] = {false, false};
+      auto key = [&](int u) { return (from + u < s.ns ? from + u : s.first + from + u - s.ns) * kWideTile; };
+      for (int i = 0; ok && i < 2; ++i) ok = WIDE_ALL(mbar_wait_bounded(q_full(i), nq & 1, abort_flag, 75));
+      tc_fence_after();
+      for (int u = -1; ok && u < count; ++u) {
+        // V of tile u sits at ring position n + 2u + 1, K of tile u + 1 at n + 2u + 2
+        const int vn = n + 2 * u + 1, kn = n + 2 * u + 2;
+        if (u >= 0) ok = WIDE_ALL(mbar_wait_bounded(full(vn % ST), (vn / ST) & 1, abort_flag, 72));
+        if (ok && u + 1 < count) ok = WIDE_ALL(mbar_wait_bounded(full(kn % ST), (kn / ST) & 1, abort_flag, 73));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (ok && u >= 0 && needs(reach[i], key(u), p.sinks)) {
+            ok = WIDE_ALL(mbar_wait_bounded(p_full(i), np[i] & 1, abort_flag, 74));
+            if (!ok) break;
+            ++np[i];
+            tc_fence_after();
+            const uint64_t vd = v_desc(base + C::OFF_RING + (vn % ST) * C::TILE_BYTES, C::HALF);
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < kWideTile / 16; ++k)
+                umma_f16_ts(tmem + C::COL_O + i * 128, tmem + C::COL_S + i * 128 + k * 8, vd + k * (2048 >> 4), id_o, begun[i] || k > 0);
+              tc_commit(o_done(i));
+            }
+            begun[i] = true;
+          }
+          if (ok && u + 1 < count && needs(reach[i], key(u + 1), p.sinks)) {
+            const uint32_t qa = base + C::OFF_Q + i * C::TILE_BYTES, ka = base + C::OFF_RING + (kn % ST) * C::TILE_BYTES;
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k)
+                umma_f16_ss(tmem + C::COL_S + i * 128, umma_smem_desc(qa + (k >> 2) * C::HALF, 128) + 2 * (k & 3),
+                            umma_smem_desc(ka + (k >> 2) * C::HALF, 128) + 2 * (k & 3), id_s, k > 0);
+              tc_commit(s_full(i));
+            }
+          }
+        }
+        if (!ok) break;
+        if (elect_one()) {  // completes with everything issued so far
+          if (u >= 0) tc_commit(empty(vn % ST));
+          if (u + 1 < count) tc_commit(empty(kn % ST));
+        }
+      }
+      n += 2 * count;
+    }
+  } else if (warp < 8) {
+    setmaxnreg_inc<kSoftmaxRegs>();
+    // ---------------------------------------------------------------- softmax, one warpgroup per row tile
+    const int i = warp >> 2, row = tid & 127, w4 = warp & 3;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(w4 * 32) << 16);
+    const uint32_t s_addr = lanes + C::COL_S + i * 128, o_addr = lanes + C::COL_O + i * 128;
+    uint8_t* q_tile = smem + C::OFF_Q + i * C::TILE_BYTES;
+    TreeMasks* tm = reinterpret_cast<TreeMasks*>(smem + C::OFF_TREE) + i;
+    int ns = 0, n = 0, tree_b = -1;
+    bool ok = true;
+    const int64_t share_from = seg.left;
+    for (; ok && seg.left > 0; seg.advance(p)) {
+      const Span& s = seg.walk.s;
+      const int count = seg.count(), from = seg.walk.tile, h = seg.walk.h;
+      const Reach reach = reach_of<TREE>(p, s, i);
+      if (TREE && s.b != tree_b) {
+        if (w4 == 0) build_tree(p, s.b, s.off, lane, tm);
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+        tree_b = s.b;
+      }
+      // ---- the tile's query rows into shared memory; a warp takes whole rows of its own 32
+      constexpr int PIECES = D / 8, PER = 32 / PIECES;  // 16-byte pieces per row, rows per access
+      {
+        const int piece = lane % PIECES;
+        uint4 v[32 / PER];
+#pragma unroll
+        for (int a = 0; a < 32 / PER; ++a) {
+          const int rl = w4 * 32 + a * PER + lane / PIECES, r = s.rb * kWideRows + i * 128 + rl;
+          v[a] = make_uint4(0, 0, 0, 0);
+          if (r < p.rows) {
+            const T* src = static_cast<const T*>(p.q) + s.b * p.q_stride[0] + (h * p.group + r % p.group) * p.q_stride[1] + (r / p.group) * p.q_stride[2] + piece * 8;
+            if (p.q_vec) {
+              v[a] = *reinterpret_cast<const uint4*>(src);
+            } else {
+              uint32_t e[8];
+#pragma unroll
+              for (int y = 0; y < 8; ++y) e[y] = *reinterpret_cast<const uint16_t*>(src + y);
+              v[a] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+            }
+          }
+        }
+#pragma unroll
+        for (int a = 0; a < 32 / PER; ++a) {
+          const int rl = w4 * 32 + a * PER + lane / PIECES;
+          *reinterpret_cast<uint4*>(q_tile + (piece >> 3) * C::HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4)) = v[a];
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(q_full(i));
+
+      const int r = s.rb * kWideRows + i * 128 + row, t = r / p.group;
+      const RowView view = r < p.rows ? row_view(p, s.off, s.len, t, TREE ? tm : nullptr) : RowView{0, 0, 0};
+      float m = -INFINITY, l = 0.f;
+      bool begun = false;
+      for (int u = 0; u < count; ++u, n += 2) {
+        const int j0 = (from + u < s.ns ? from + u : s.first + from + u - s.ns) * kWideTile;
+        if (!needs(reach, j0, p.sinks)) continue;
+        ok = WIDE_ALL(mbar_wait_bounded(s_full(i), ns & 1, abort_flag, 76));
+        if (!ok) break;
+        ++ns;
+        tc_fence_after();
+        const uint32_t held = there[(n / 2) % kThere];
+        const int box = p.table ? min(p.page, kWideTile) : kWideTile;
+        const uint32_t all = (1u << (kWideTile / box)) - 1;
+        const bool clear = held == all && ((j0 >= s.full_lo && j0 + kWideTile <= s.full_hi) || j0 + kWideTile <= min(p.sinks, s.full_hi));
+        uint32_t sr[128];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_ld32(s_addr + c, sr + c);
+        tmem_wait_ld();
+        float* sc = reinterpret_cast<float*>(sr);
+        if (!clear) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t bits = seen_bits<TREE>(view, j0 + 32 * c, s.off, p.sinks) & below(s.len - (j0 + 32 * c));
+            if (held != all) {
+              uint32_t good = 0;
+              for (int x = 0; x < 32; x += 16)
+                if ((held >> ((32 * c + x) / box)) & 1) good |= 0xffffu << x;
+              bits &= good;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((bits >> e) & 1)) sc[32 * c + e] = -INFINITY;
+          }
+          // V rows behind the sequence may hold anything (0 * NaN is a NaN): they become zeros before
+          // this thread's arrival, for which the product waits.  Both warpgroups write the same zeros.
+          if (j0 + kWideTile > s.len) {
+            const int vs = (n + 1) % ST;
+            ok = WIDE_ALL(mbar_wait_bounded(full(vs), ((n + 1) / ST) & 1, abort_flag, 77));
+            if (!ok) break;
+            uint8_t* vt = smem + C::OFF_RING + vs * C::TILE_BYTES;
+            if (j0 + row >= s.len) {
+#pragma unroll
+              for (int x = 0; x < D / 8; ++x) *reinterpret_cast<uint4*>(vt + (x >> 3) * C::HALF + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+        }
+        float t0 = max3f(sc[0], sc[1], sc[2]), t1 = max3f(sc[3], sc[4], sc[5]);
+#pragma unroll
+        for (int c = 6; c < 126; c += 4) {
+          t0 = max3f(t0, sc[c], sc[c + 1]);
+          t1 = max3f(t1, sc[c + 2], sc[c + 3]);
+        }
+        const float top = max3f(fmaxf(t0, t1), sc[126], sc[127]) * p.scale_log2;
+        const bool raise = top > m + kWideRaise;
+        if (__any_sync(0xffffffffu, raise)) {
+          const float mn = raise ? top : m;
+          const float keep = m == mn ? 1.f : ex2_approx(m - mn);
+          m = mn;
+          l *= keep;
+          if (begun) {
+            // the products of the tiles before this one are complete: they were issued before its scores
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(o_addr + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+              tmem_st16(o_addr + c, o);
+            }
+          }
+        }
+        begun = true;
+        const float ref = m == -INFINITY ? 0.f : m;
+        const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), ref2 = make_float2(-ref, -ref);
+        float2 l0 = make_float2(0.f, 0.f), l1 = l0;
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const float2 a = __ffma2_rn(make_float2(sc[c + 2 * e], sc[c + 2 * e + 1]), mul2, ref2);
+            const float2 b = __ffma2_rn(make_float2(sc[c + 2 * e + 2], sc[c + 2 * e + 3]), mul2, ref2);
+            const float2 ea = make_float2(ex2_approx(a.x), ex2_approx(a.y)), eb = make_float2(ex2_approx(b.x), ex2_approx(b.y));
+            l0 = __fadd2_rn(l0, ea);
+            l1 = __fadd2_rn(l1, eb);
+            pk[e] = pack2<T>(ea.x, ea.y);
+            pk[e + 1] = pack2<T>(eb.x, eb.y);
+          }
+          tmem_st16(s_addr + c / 2, pk);
+        }
+        l += (l0.x + l0.y) + (l1.x + l1.y);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(p_full(i));
+      }
+      // ---- rows out.  The warps of a row tile leave together when a wait was abandoned.
+      ok = vote_barrier(1 + i, ok && *abort_flag == 0);
+      if (!ok) break;
+      const bool whole = from == 0 && count == s.n;
+      if (begun) {
+        if (!WIDE_ALL(mbar_wait_bounded(o_done(i), (ns - 1) & 1, abort_flag, 78))) l = __int_as_float(0x7fc00000);
+        tc_fence_after();
+      }
+      const int idx = s.off + t;
+      const bool valid = r < p.rows && idx >= 0 && idx < s.len;
+      if (!whole) {
+        const int slot = blockIdx.x * 2 + (seg.left != share_from ? 1 : 0);
+        float* dst = p.partial + (static_cast<int64_t>(slot) * kWideRows + i * 128 + row) * (D + 2);
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          if (begun) {
+            tmem_ld32(o_addr + c, o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+          }
+          if (r < p.rows) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) *reinterpret_cast<float2*>(dst + c + e) = make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+          }
+        }
+        if (r < p.rows) *reinterpret_cast<float2*>(dst + D) = make_float2(m, l);
+        tc_fence_before();
+        continue;
+      }
+      // The query tile has been read by every product: its place takes the output rows, from where
+      // they leave as whole rows (a thread's own row would be written 16 bytes at a time).
+      const float inv = valid && l != 0.f ? 1.f / l : 0.f;
+      bool bad = false;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (begun) {
+          tmem_ld32(o_addr + c, o);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          float x[8];
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            x[y] = begun && inv != 0.f ? __uint_as_float(o[e + y]) * inv : 0.f;
+            bad |= !(fabsf(x[y]) <= 3.0e38f);
+          }
+          const int piece = (c + e) / 8;
+          *reinterpret_cast<uint4*>(q_tile + (piece >> 3) * C::HALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) =
+              make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+#pragma unroll 4
+      for (int a = 0; a < 32 / PER; ++a) {
+        const int piece = lane % PIECES, rl = w4 * 32 + a * PER + lane / PIECES, rr = s.rb * kWideRows + i * 128 + rl;
+        if (rr < p.rows) {
+          T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + rr % p.group) * p.tokens + rr / p.group) * D + piece * 8;
+          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(q_tile + (piece >> 3) * C::HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4));
+        }
+      }
+      uint32_t vote = __ballot_sync(0xffffffffu, bad);
+      __syncwarp();
+      while (vote) {  // rows with a value that is not finite, evaluated again from their own keys
+        const int src = __ffs(vote) - 1, rr = s.rb * kWideRows + i * 128 + w4 * 32 + src;
+        vote &= vote - 1;
+        plain_row<T, false, D>(p, s.b, h, rr, s.off, s.len, row_view(p, s.off, s.len, rr / p.group, TREE ? tm : nullptr), TREE);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (tid == 0 && *abort_flag != 0 && p.host_status != nullptr) atomicCAS_system(p.host_status, 0, *abort_flag);
+}
+
+template <typename T, int D, bool TREE>
+int launch_wide(AttendParams p, int device, cudaStream_t st) {
+  using C = Wide<D>;
+  static_assert(C::SMEM <= 227 * 1024, "shared memory of one CTA");
+  p.row_blocks = (p.rows + kWideRows - 1) / kWideRows;
+  CUtensorMap tk, tv;
+  int rc;
+  const int box = p.table ? (p.page < kWideTile ? p.page : kWideTile) : kWideTile, lines = p.table ? 1 : D / 64;
+  if ((rc = attend_map(&tk, p, p.k, p.k_stride, 128, D / 64, 2, box, lines))) return rc;
+  if ((rc = attend_map(&tv, p, p.v, p.v_stride, 128, D / 64, 2, box, lines))) return rc;
+  if ((rc = allow_smem<wide_rows_kernel<T, D, TREE>>(C::SMEM, device))) return rc;
+  const int64_t units = static_cast<int64_t>(p.batch) * p.row_blocks * p.kv_heads;
+  const bool share = units < kWideShareBelow;
+  p.workers = share ? kWideWorkers : 0;
+  cudaError_t e = launch_chained(wide_rows_kernel<T, D, TREE>, dim3(share ? kWideWorkers : static_cast<unsigned>(units)), dim3(kWideThreads), C::SMEM, st, tk, tv, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(PK_ERR_CUDA, "attention kernel launch failed: %s", cuda_err(e));
+  if (!share) return PK_OK;
+  e = launch_chained(join_kernel<T, false, D, TREE, kWideTile, kWideRows>, dim3(static_cast<unsigned>(units)), dim3(kCounters), 0, st, p, p.workers);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(PK_ERR_CUDA, "join kernel launch failed: %s", cuda_err(e));
+  return PK_OK;
+}
+
+template <typename T>
+int wide_by_dim(const AttendParams& p, int head_dim, int device, cudaStream_t st) {
+  if (head_dim == 128) return p.tree ? launch_wide<T, 128, true>(p, device, st) : launch_wide<T, 128, false>(p, device, st);
+  return p.tree ? launch_wide<T, 64, true>(p, device, st) : launch_wide<T, 64, false>(p, device, st);
+}
+
+}  // namespace
+}  // namespace pk

@@ -1,0 +1,16 @@
+// Wide-row attention (wide_rows.cuh) for float16.
+#include "wide_rows.cuh"
+
+namespace pk {
+
+uint64_t wide_rows_workspace(int batch, int kv_heads, int rows, int head_dim) {
+  const int64_t units = static_cast<int64_t>(batch) * kv_heads * ((rows + kWideRows - 1) / kWideRows);
+  if (units >= kWideShareBelow) return 0;
+  return static_cast<uint64_t>(kWideWorkers) * 2 * kWideRows * (head_dim + 2) * sizeof(float);
+}
+
+int launch_wide_rows_f16(const AttendParams& p, int head_dim, int device, cudaStream_t st) {
+  return wide_by_dim<__half>(p, head_dim, device, st);
+}
+
+}  // namespace pk
