@@ -517,7 +517,7 @@ int launch(AttendParams p, int device, cudaStream_t st) {
   cudaError_t e = launch_chained(few_rows_kernel<T, I8, D, WM, TREE>, dim3(p.workers), dim3(kThreads), C::SMEM, st, tk, tv, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "attention kernel launch failed: %s", cuda_err(e));
-  e = launch_chained(join_kernel<T, I8, D, TREE, kTile, C::ROWS>, dim3(p.batch * p.row_blocks * p.kv_heads), dim3(kConsumers), 0, st, p, p.workers);
+  e = launch_chained(join_kernel<T, I8, D, TREE, kTile, C::ROWS>, dim3(p.batch * p.row_blocks * p.kv_heads * (C::ROWS / kJoinRows)), dim3(kCounters), 0, st, p, p.workers);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "join kernel launch failed: %s", cuda_err(e));
   return PK_OK;

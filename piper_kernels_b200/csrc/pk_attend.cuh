@@ -366,13 +366,18 @@ struct Walk {  // position in the list of tiles
   __device__ __forceinline__ int key() const { return (tile < s.ns ? tile : s.first + tile - s.ns) * TILE; }
 };
 
-// Joins the pieces of every unit that more than one CTA worked on.  One CTA per unit (batch element,
-// row block, key head); units that one CTA finished are left alone.
+// Joins the pieces of every unit that more than one CTA worked on.  kJoinRows rows of a unit (batch
+// element, row block, key head) per CTA, one or two per warp: a row's pieces are a chain of loads, and
+// rows are what there is to run side by side.  Units that one CTA finished are left alone.
+constexpr int kJoinRows = 8;
+
 template <typename T, bool I8, int D, bool TREE, int TILE, int ROWS>
 __global__ void __launch_bounds__(kCounters) join_kernel(const __grid_constant__ AttendParams p, int workers) {
   __shared__ int64_t red[4];
   __shared__ TreeMasks tm;
-  const int unit = blockIdx.x, g = unit / p.kv_heads, h = unit % p.kv_heads, groups = p.batch * p.row_blocks;
+  const int unit = blockIdx.x / (ROWS / kJoinRows), g = unit / p.kv_heads, h = unit % p.kv_heads, groups = p.batch * p.row_blocks;
+  const int r0 = blockIdx.x % (ROWS / kJoinRows) * kJoinRows;
+  if (g % p.row_blocks * ROWS + r0 >= p.rows) return;
   cudaGridDependencySynchronize();
   const int64_t total = sum_tiles<TREE, TILE, ROWS>(p, groups, red);
   int64_t u0 = sum_tiles<TREE, TILE, ROWS>(p, g, red);
@@ -387,8 +392,8 @@ __global__ void __launch_bounds__(kCounters) join_kernel(const __grid_constant__
   }
   const bool first_second = u0 > share_begin(total, workers, c0);  // its first CTA began with another unit
   constexpr int E = D / 32;
-  const int r1 = min(p.rows - s.rb * ROWS, ROWS);
-  for (int r = warp; r < r1; r += kCounters / 32) {
+  const int r1 = min(p.rows - s.rb * ROWS, r0 + kJoinRows);
+  for (int r = r0 + warp; r < r1; r += kCounters / 32) {
     float mx = -INFINITY, sum = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;

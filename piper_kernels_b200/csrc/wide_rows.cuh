@@ -543,7 +543,7 @@ int launch_wide(AttendParams p, int device, cudaStream_t st) {
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "attention kernel launch failed: %s", cuda_err(e));
   if (!share) return PK_OK;
-  e = launch_chained(join_kernel<T, false, D, TREE, kWideTile, kWideRows>, dim3(static_cast<unsigned>(units)), dim3(kCounters), 0, st, p, p.workers);
+  e = launch_chained(join_kernel<T, false, D, TREE, kWideTile, kWideRows>, dim3(static_cast<unsigned>(units) * (kWideRows / kJoinRows)), dim3(kCounters), 0, st, p, p.workers);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "join kernel launch failed: %s", cuda_err(e));
   return PK_OK;
