@@ -228,6 +228,7 @@ PK_API int pk_window_attention_fwd(const pk_window_problem* pp) {
   a.out = p.out;
   a.batch = p.batch, a.heads = p.heads, a.kv_heads = p.kv_heads, a.group = p.heads / p.kv_heads, a.tokens = p.q_len;
   a.rows = a.group * a.tokens;
+  a.group_inv = ~0ull / a.group + 1;  // not used for groups of one
   a.lengths = p.lengths;
   a.kv_len = p.kv_len, a.offset = p.kv_len - p.q_len;
   a.k = p.k, a.v = p.v;
@@ -287,6 +288,7 @@ PK_API int pk_cache_attention_fwd(const pk_cache* c, const pk_cache_query* q) {
   a.out = q->out;
   a.batch = c->batch, a.heads = q->heads, a.kv_heads = c->kv_heads, a.group = q->heads / c->kv_heads, a.tokens = q->tokens;
   a.rows = a.group * a.tokens;
+  a.group_inv = ~0ull / a.group + 1;  // not used for groups of one
   a.lengths = c->lengths, a.starts = c->starts;
   a.table = c->table, a.width = c->width, a.page = c->page_size, a.pages = c->pages, a.page_base = q->layer * c->pages;
   a.page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));

@@ -214,10 +214,10 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     const T* qrow[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const int r = s.rb * C::ROWS + wm * 16 + g8 + 8 * x, t = r / p.group;
+      const int r = s.rb * C::ROWS + wm * 16 + g8 + 8 * x, t = token_of(p, r);
       view[x] = r < p.rows ? row_view(p, s.off, s.len, t, TREE ? tm : nullptr) : RowView{0, 0, 0};
       const bool there = r < p.rows;
-      qrow[x] = there ? static_cast<const T*>(p.q) + s.b * p.q_stride[0] + (h * p.group + r % p.group) * p.q_stride[1] + t * p.q_stride[2] : nullptr;
+      qrow[x] = there ? static_cast<const T*>(p.q) + s.b * p.q_stride[0] + (h * p.group + r - t * p.group) * p.q_stride[1] + t * p.q_stride[2] : nullptr;
       m[x] = -INFINITY;
       l[x] = 0.f;
     }
@@ -255,7 +255,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       const int st = i % kStages;
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * st, (i / kStages) & 1, abort_flag, 62));
       if (!ok) break;
-      const int j0 = (unit_from + u < s.ns ? unit_from + u : s.first + unit_from + u - s.ns) * kTile;
+      const int j0 = key_of_tile<kTile>(s, unit_from + u);
       // Keys on pages that are not there are masked like those that no row may see.
       const uint32_t held = there[st], all = (1u << (kTile / box)) - 1;
       const bool full = held == all && ((j0 >= s.full_lo && j0 + kTile <= s.full_hi) || (j0 + kTile <= min(p.sinks, s.full_hi)));
@@ -463,7 +463,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             *reinterpret_cast<float2*>(dst + pass * kJoinCols + col + 2) = make_float2(acc[2], acc[3]);
             if (pass == 0 && (tid & 7) == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mx, sum);
           } else {
-            const int t = row / p.group, idx = s.off + t;
+            const int t = token_of(p, row), idx = s.off + t;
             const bool valid = idx >= 0 && idx < s.len;
             const float r = valid && sum != 0.f ? 1.f / sum : 0.f;
             float v[4];
@@ -472,7 +472,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
               v[y] = r == 0.f ? 0.f : acc[y] * r;
               bad[it] |= !(fabsf(v[y]) <= 3.0e38f);
             }
-            T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + row % p.group) * p.tokens + t) * D + pass * kJoinCols + col;
+            T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + row - t * p.group) * p.tokens + t) * D + pass * kJoinCols + col;
             *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
           }
         }
@@ -488,7 +488,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       for (int r = 0; vote && r < 4; ++r) {
         if (!(vote & (0xffu << (8 * r)))) continue;
         const int row = s.rb * C::ROWS + it * 16 + warp * 4 + r;
-        plain_row<T, I8, D>(p, s.b, h, row, s.off, s.len, row_view(p, s.off, s.len, row / p.group, TREE ? tm : nullptr), TREE);
+        plain_row<T, I8, D>(p, s.b, h, row, s.off, s.len, row_view(p, s.off, s.len, token_of(p, row), TREE ? tm : nullptr), TREE);
       }
     }
     // the next unit
@@ -506,13 +506,14 @@ int launch(AttendParams p, int device, cudaStream_t st) {
   using C = Few<T, I8, D, WM>;
   static_assert(C::SMEM <= 113 * 1024, "two CTAs share an SM");
   p.row_blocks = (p.rows + C::ROWS - 1) / C::ROWS;
+  p.key_align = p.table ? (p.page < kTile ? p.page : kTile) : 8;
   CUtensorMap tk, tv;
   int rc;
   if ((rc = attend_map(&tk, p, p.k, p.k_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < kTile ? p.page : kTile) : kTile, C::HALVES))) return rc;
   if ((rc = attend_map(&tv, p, p.v, p.v_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < kTile ? p.page : kTile) : kTile, C::HALVES))) return rc;
   if ((rc = allow_smem<few_rows_kernel<T, I8, D, WM, TREE>>(C::SMEM, device))) return rc;
   // No more CTAs than there can be tiles.
-  const int64_t most = static_cast<int64_t>(p.batch) * p.row_blocks * p.kv_heads * (((p.table ? p.width * p.page : p.kv_len) + kTile - 1) / kTile + 1);
+  const int64_t most = static_cast<int64_t>(p.batch) * p.row_blocks * p.kv_heads * (((p.table ? p.width * p.page : p.kv_len) + kTile - 1) / kTile + 2);
   p.workers = static_cast<int>(most < kMaxWorkers ? most : kMaxWorkers);
   cudaError_t e = launch_chained(few_rows_kernel<T, I8, D, WM, TREE>, dim3(p.workers), dim3(kThreads), C::SMEM, st, tk, tv, p);
   if (e == cudaSuccess) e = cudaGetLastError();

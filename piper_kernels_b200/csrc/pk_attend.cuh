@@ -31,6 +31,7 @@ struct AttendParams {
   int q_vec;            // rows start on 16-byte boundaries
   void* out;            // [batch, heads, tokens, D]
   int batch, heads, kv_heads, group, tokens, rows, row_blocks;
+  uint64_t group_inv;  // ceil(2^64 / group): row / group is the high half of row * group_inv (group > 1)
   const int32_t* lengths;  // may be null (dense): every batch element holds kv_len keys
   const int32_t* starts;   // null (dense): off(b) = offset
   int kv_len, offset;
@@ -44,12 +45,17 @@ struct AttendParams {
   const int32_t* tree;  // [batch, tokens] parents, or null
   int64_t tree_stride;
   int window, sinks;
+  int key_align;     // tiles begin on multiples of this: 8, or what keeps a tile's copies within pages
   float scale_log2;  // softmax scale * log2(e)
   float* partial;    // pieces of rows whose keys are shared by several CTAs
   int workers;
   int32_t* host_status;  // pinned word that takes the site of an abandoned wait
 };
 
+// Token of a row (its query head within the group is the remainder).
+__device__ __forceinline__ int token_of(const AttendParams& p, int row) {
+  return p.group == 1 ? row : static_cast<int>(__umul64hi(static_cast<uint64_t>(row), p.group_inv));
+}
 __device__ __forceinline__ int attend_len(const AttendParams& p, int b) {
   const int most = p.table ? p.width * p.page : p.kv_len;
   if (!p.lengths) return most;
@@ -189,7 +195,7 @@ __device__ __forceinline__ __nv_bfloat16 from_f32(float a) { return __float2bflo
 template <typename T, bool I8, int D>
 __device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, int row, int off, int len, RowView view, bool tree) {
   constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31, t = row / p.group, head = kvh * p.group + row % p.group;
+  const int lane = threadIdx.x & 31, t = token_of(p, row), head = kvh * p.group + row - t * p.group;
   const T* q = static_cast<const T*>(p.q) + b * p.q_stride[0] + head * p.q_stride[1] + t * p.q_stride[2] + lane * E;
   float qf[E], acc[E], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -245,9 +251,9 @@ __device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, in
 // tiles, of which every CTA takes an equal, contiguous part.
 // ---------------------------------------------------------------------------------------
 // One group of query rows (batch element, row block; the same for every key head) and the key tiles
-// that any of its rows sees: `ns` tiles of sinks, then the tiles from `first` on.
+// that any of its rows sees: `ns` tiles of sinks, then those from key `begin` on.
 struct Span {
-  int b, rb, off, len, ns, first, n;
+  int b, rb, off, len, ns, begin, n;
   int full_lo, full_hi;  // keys that every row sees
 };
 
@@ -259,7 +265,7 @@ __device__ __forceinline__ Span span_of(const AttendParams& p, int g) {
   s.len = attend_len(p, s.b);
   s.off = attend_off(p, s.b, s.len);
   const int r0 = s.rb * ROWS, r1 = min(r0 + ROWS, p.rows) - 1;
-  const int t0 = r0 / p.group, t1 = r1 / p.group;
+  const int t0 = token_of(p, r0), t1 = token_of(p, r1);
   int hi, lo;
   if (TREE) {
     hi = min(s.len, s.off + p.tokens);
@@ -276,10 +282,16 @@ __device__ __forceinline__ Span span_of(const AttendParams& p, int g) {
   hi = max(hi, 0);
   lo = min(max(lo, 0), hi);
   s.ns = (min(p.sinks, lo) + TILE - 1) / TILE;
-  s.first = max(lo / TILE, s.ns);
-  s.n = s.ns + max(0, (hi + TILE - 1) / TILE - s.first);
-  if (s.n == 0) s.n = 1, s.ns = 0, s.first = 0;  // rows that see nothing still have to be written
+  s.begin = max(lo & -p.key_align, s.ns * TILE);
+  s.n = s.ns + max(0, (hi - s.begin + TILE - 1) / TILE);
+  if (s.n == 0) s.n = 1, s.ns = 0, s.begin = 0;  // rows that see nothing still have to be written
   return s;
+}
+
+// First key of tile i.
+template <int TILE>
+__device__ __forceinline__ int key_of_tile(const Span& s, int i) {
+  return i < s.ns ? i * TILE : s.begin + (i - s.ns) * TILE;
 }
 
 // First tile of worker w, when `total` tiles are shared out.
@@ -363,7 +375,7 @@ struct Walk {  // position in the list of tiles
     h = 0;
     if (++g < p.batch * p.row_blocks) s = span_of<TREE, TILE, ROWS>(p, g);
   }
-  __device__ __forceinline__ int key() const { return (tile < s.ns ? tile : s.first + tile - s.ns) * TILE; }
+  __device__ __forceinline__ int key() const { return key_of_tile<TILE>(s, tile); }
 };
 
 // Joins the pieces of every unit that more than one CTA worked on.  kJoinRows rows of a unit (batch
@@ -414,9 +426,9 @@ __global__ void __launch_bounds__(kCounters) join_kernel(const __grid_constant__
         acc[e + 1] = fmaf(v.y, wgt, acc[e + 1]);
       }
     }
-    const int row = s.rb * ROWS + r, t = row / p.group, idx = s.off + t;
+    const int row = s.rb * ROWS + r, t = token_of(p, row), idx = s.off + t;
     const float inv = idx >= 0 && idx < s.len && sum != 0.f ? 1.f / sum : 0.f;
-    T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + row % p.group) * p.tokens + t) * D + lane * E;
+    T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + row - t * p.group) * p.tokens + t) * D + lane * E;
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < E; e += 2) {

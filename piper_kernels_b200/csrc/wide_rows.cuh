@@ -52,7 +52,7 @@ struct Wide {
   static constexpr int OFF_RING = 2 * TILE_BYTES;
   static constexpr int OFF_TREE = OFF_RING + STAGES * TILE_BYTES;
   static constexpr int OFF_BAR = OFF_TREE + 2 * static_cast<int>(sizeof(TreeMasks));
-  static constexpr int BARS = 2 * STAGES + 2 * 4;  // ring full / empty; q_full, s_full, p_full, o_done per row tile
+  static constexpr int BARS = 2 * STAGES + 2 * 5;  // ring full / empty; q_full, s_full, p_half, p_full, o_done per row tile
   static constexpr int OFF_RED = OFF_BAR + BARS * 8;
   static constexpr int OFF_THERE = OFF_RED + 64;
   static constexpr int OFF_MISC = OFF_THERE + kThere * 4;
@@ -62,7 +62,7 @@ struct Wide {
 
 // Both operands 16-bit, 32-bit accumulator.  B transposed: its rows lie along the contraction.
 template <typename T>
-__host__ __device__ constexpr uint32_t wide_idesc(int n, bool b_transposed) {
+__host__ __device__ constexpr uint32_t wide_idesc(int n, bool b_transposed) {  // M = 128
   const uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_transposed ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
@@ -83,6 +83,33 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, 
 __device__ __forceinline__ uint64_t v_desc(uint32_t addr, int half) {
   return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(half >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) |
          (2ull << 61);
+}
+
+// 2^x for two values on the FMA pipe (the exponential unit alone would set the pace): x = n + r with
+// n the nearest integer and |r| <= 1/2; 2^r by a polynomial of degree 4, fitted here for the least
+// largest relative error with value 1 at 0 (2.9e-6, measured over r in 32-bit arithmetic); n goes into
+// the exponent.  Below -127 the result is 0 (r = 0 there).  A NaN or infinity may come out as any huge
+// number: the row is then not finite and is evaluated again.
+constexpr int kPolyEvery = 4;
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  float a, b;
+  asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(a) : "f"(x.x));  // -127
+  asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(b) : "f"(x.y));
+  const float2 magic = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f), neg = make_float2(-1.f, -1.f);
+  x = make_float2(a, b);
+  const float2 u = __fadd2_rn(x, magic);             // 1.5 * 2^23 + n: n in the low bits
+  const float2 r = __ffma2_rn(__fadd2_rn(u, minus), neg, x);
+  float2 y = make_float2(0x1.3a007ap-7f, 0x1.3a007ap-7f);
+  y = __ffma2_rn(y, r, make_float2(0x1.c9fd1ep-5f, 0x1.c9fd1ep-5f));
+  y = __ffma2_rn(y, r, make_float2(0x1.ec0382p-3f, 0x1.ec0382p-3f));
+  y = __ffma2_rn(y, r, make_float2(0x1.62e12ap-1f, 0x1.62e12ap-1f));
+  y = __ffma2_rn(y, r, make_float2(1.f, 1.f));
+  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(u.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(u.y) << 23)));
+}
+
+// Sixteen bytes from global to shared memory, asynchronously; `bytes` 0: zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 // What one CTA does next: tiles [tile, tile + count) of one unit.  Every role walks the same list.
@@ -108,13 +135,19 @@ __device__ __forceinline__ Reach reach_of(const AttendParams& p, const Span& s, 
   const int r0 = s.rb * kWideRows + tile * 128, r1 = min(r0 + 128, p.rows) - 1;
   Reach r{0, 0};
   if (r0 >= p.rows) return r;
-  const int t0 = r0 / p.group, t1 = r1 / p.group;
+  const int t0 = token_of(p, r0), t1 = token_of(p, r1);
   if (s.off + t0 >= s.len) return r;
   r.hi = max(0, TREE ? min(s.len, s.off + p.tokens) : min(s.len, s.off + t1 + 1));
   r.lo = max(0, (TREE ? s.off : s.off + t0) - p.window + 1);
   return r;
 }
 __device__ __forceinline__ bool needs(const Reach& r, int j0, int sinks) { return j0 < r.hi && (j0 + kWideTile > r.lo || j0 < sinks); }
+
+// How many of a tile's keys, from its first on, a row tile has to look at (a multiple of 32).
+__device__ __forceinline__ int width_of(const Reach& r, int j0, int sinks) {
+  const int end = j0 + kWideTile > r.lo ? r.hi : min(sinks, r.hi);
+  return min((end - j0 + 31) & ~31, kWideTile);
+}
 
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }  // bits [0, n)
 
@@ -147,14 +180,15 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   auto empty = [&](int i) { return bars + 8 * (ST + i); };
   auto q_full = [&](int i) { return bars + 8 * (2 * ST + i); };
   auto s_full = [&](int i) { return bars + 8 * (2 * ST + 2 + i); };
-  auto p_full = [&](int i) { return bars + 8 * (2 * ST + 4 + i); };
-  auto o_done = [&](int i) { return bars + 8 * (2 * ST + 6 + i); };
+  auto p_half = [&](int i) { return bars + 8 * (2 * ST + 4 + i); };
+  auto p_full = [&](int i) { return bars + 8 * (2 * ST + 6 + i); };
+  auto o_done = [&](int i) { return bars + 8 * (2 * ST + 8 + i); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int MMA_WARP = 8, COPY_WARP = 9;
 
   if (tid < C::BARS) {
     const int kind = tid < 2 * ST ? 1 : (tid - 2 * ST) / 2;
-    mbar_init(bars + 8 * tid, tid >= 2 * ST && (kind == 0 || kind == 2) ? 128 : 1);  // q_full, p_full: a warpgroup
+    mbar_init(bars + 8 * tid, kind == 1 || kind == 4 ? 1 : 128);  // q_full, p_half, p_full: a warpgroup
     fence_barrier_init();
   }
   if (tid == 0) *abort_flag = 0;
@@ -198,7 +232,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const int count = seg.count(), from = seg.walk.tile;
         for (int u = 0; ok && u < count; ++u) {
           const Span& s = seg.walk.s;
-          const int j0 = (from + u < s.ns ? from + u : s.first + from + u - s.ns) * kWideTile;
+          const int j0 = key_of_tile<kWideTile>(s, from + u);
           int pages[kWideTile / 16];
           uint32_t mask = 1u;
           if (p.table) {
@@ -241,7 +275,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     }
   } else if (warp == MMA_WARP) {
     // ---------------------------------------------------------------- products
-    constexpr uint32_t id_s = wide_idesc<T>(kWideTile, false), id_o = wide_idesc<T>(D, true);
+    constexpr uint32_t id_o = wide_idesc<T>(D, true);
     int n = 0;                     // tiles consumed, K and V counted one after the other
     int np[2] = {0, 0}, nq = 0;    // probability tiles, segments
     bool ok = true;
@@ -250,7 +284,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       const int count = seg.count(), from = seg.walk.tile;
       const Reach reach[2] = {reach_of<TREE>(p, s, 0), reach_of<TREE>(p, s, 1)};
       bool begun[2] = {false, false};
-      auto key = [&](int u) { return (from + u < s.ns ? from + u : s.first + from + u - s.ns) * kWideTile; };
+      auto key = [&](int u) { return key_of_tile<kWideTile>(s, from + u); };
       for (int i = 0; ok && i < 2; ++i) ok = WIDE_ALL(mbar_wait_bounded(q_full(i), nq & 1, abort_flag, 75));
       tc_fence_after();
       for (int u = -1; ok && u < count; ++u) {
@@ -261,21 +295,33 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (ok && u >= 0 && needs(reach[i], key(u), p.sinks)) {
-            ok = WIDE_ALL(mbar_wait_bounded(p_full(i), np[i] & 1, abort_flag, 74));
+            // the first 64 keys' probabilities come first: their product runs while the others are evaluated
+            const int steps = width_of(reach[i], key(u), p.sinks) / 16;
+            const uint64_t vd = v_desc(base + C::OFF_RING + (vn % ST) * C::TILE_BYTES, C::HALF);
+            const uint32_t o = tmem + C::COL_O + i * 128, pr = tmem + C::COL_S + i * 128;
+            ok = WIDE_ALL(mbar_wait_bounded(p_half(i), np[i] & 1, abort_flag, 74));
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < steps) umma_f16_ts(o, pr + k * 8, vd + k * (2048 >> 4), id_o, begun[i] || k > 0);
+            }
+            ok = WIDE_ALL(mbar_wait_bounded(p_full(i), np[i] & 1, abort_flag, 79));
             if (!ok) break;
             ++np[i];
             tc_fence_after();
-            const uint64_t vd = v_desc(base + C::OFF_RING + (vn % ST) * C::TILE_BYTES, C::HALF);
             if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < kWideTile / 16; ++k)
-                umma_f16_ts(tmem + C::COL_O + i * 128, tmem + C::COL_S + i * 128 + k * 8, vd + k * (2048 >> 4), id_o, begun[i] || k > 0);
+              for (int k = 4; k < 8; ++k)
+                if (k < steps) umma_f16_ts(o, pr + k * 8, vd + k * (2048 >> 4), id_o, 1);
               tc_commit(o_done(i));
             }
             begun[i] = true;
           }
           if (ok && u + 1 < count && needs(reach[i], key(u + 1), p.sinks)) {
             const uint32_t qa = base + C::OFF_Q + i * C::TILE_BYTES, ka = base + C::OFF_RING + (kn % ST) * C::TILE_BYTES;
+            const uint32_t id_s = wide_idesc<T>(0, false) | (static_cast<uint32_t>(width_of(reach[i], key(u + 1), p.sinks) >> 3) << 17);
             if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < D / 16; ++k)
@@ -304,6 +350,8 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     int ns = 0, n = 0, tree_b = -1;
     bool ok = true;
     const int64_t share_from = seg.left;
+    const int box = p.table ? min(p.page, kWideTile) : kWideTile;
+    const uint32_t all = (1u << (kWideTile / box)) - 1;
     for (; ok && seg.left > 0; seg.advance(p)) {
       const Span& s = seg.walk.s;
       const int count = seg.count(), from = seg.walk.tile, h = seg.walk.h;
@@ -316,94 +364,111 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       // ---- the tile's query rows into shared memory; a warp takes whole rows of its own 32
       constexpr int PIECES = D / 8, PER = 32 / PIECES;  // 16-byte pieces per row, rows per access
       {
-        const int piece = lane % PIECES;
-        uint4 v[32 / PER];
+        const int piece = lane % PIECES, rl0 = w4 * 32 + lane / PIECES;
+        const T* q0 = static_cast<const T*>(p.q) + s.b * p.q_stride[0] + static_cast<int64_t>(h) * p.group * p.q_stride[1] + piece * 8;
 #pragma unroll
         for (int a = 0; a < 32 / PER; ++a) {
-          const int rl = w4 * 32 + a * PER + lane / PIECES, r = s.rb * kWideRows + i * 128 + rl;
-          v[a] = make_uint4(0, 0, 0, 0);
-          if (r < p.rows) {
-            const T* src = static_cast<const T*>(p.q) + s.b * p.q_stride[0] + (h * p.group + r % p.group) * p.q_stride[1] + (r / p.group) * p.q_stride[2] + piece * 8;
-            if (p.q_vec) {
-              v[a] = *reinterpret_cast<const uint4*>(src);
-            } else {
-              uint32_t e[8];
+          const int rl = rl0 + a * PER, r = s.rb * kWideRows + i * 128 + rl, tq = token_of(p, r);
+          const T* src = q0 + (r - tq * p.group) * p.q_stride[1] + tq * p.q_stride[2];
+          uint8_t* dst = q_tile + (piece >> 3) * C::HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4);
+          if (p.q_vec) {
+            copy16(smem_u32(dst), r < p.rows ? src : q0, r < p.rows ? 16 : 0);
+          } else {
+            uint32_t e[8];
 #pragma unroll
-              for (int y = 0; y < 8; ++y) e[y] = *reinterpret_cast<const uint16_t*>(src + y);
-              v[a] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-            }
+            for (int y = 0; y < 8; ++y) e[y] = r < p.rows ? *reinterpret_cast<const uint16_t*>(src + y) : 0;
+            *reinterpret_cast<uint4*>(dst) = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
           }
         }
-#pragma unroll
-        for (int a = 0; a < 32 / PER; ++a) {
-          const int rl = w4 * 32 + a * PER + lane / PIECES;
-          *reinterpret_cast<uint4*>(q_tile + (piece >> 3) * C::HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4)) = v[a];
-        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
       }
       fence_proxy_async_smem();
       mbar_arrive(q_full(i));
 
-      const int r = s.rb * kWideRows + i * 128 + row, t = r / p.group;
+      const int r = s.rb * kWideRows + i * 128 + row, t = token_of(p, r);
       const RowView view = r < p.rows ? row_view(p, s.off, s.len, t, TREE ? tm : nullptr) : RowView{0, 0, 0};
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY;
+      float2 l0 = make_float2(0.f, 0.f), l1 = l0;
       bool begun = false;
+      // keys that every row of this row tile sees
+      const int t_first = token_of(p, min(s.rb * kWideRows + i * 128, p.rows - 1)), t_last = token_of(p, min(s.rb * kWideRows + i * 128 + 127, p.rows - 1));
+      const int full_hi = TREE ? s.full_hi : min(s.len, s.off + t_first + 1), full_lo = TREE ? s.full_lo : s.off + t_last - p.window + 1;
       for (int u = 0; u < count; ++u, n += 2) {
-        const int j0 = (from + u < s.ns ? from + u : s.first + from + u - s.ns) * kWideTile;
+        const int j0 = key_of_tile<kWideTile>(s, from + u);
         if (!needs(reach, j0, p.sinks)) continue;
         ok = WIDE_ALL(mbar_wait_bounded(s_full(i), ns & 1, abort_flag, 76));
         if (!ok) break;
         ++ns;
         tc_fence_after();
+        const int width = width_of(reach, j0, p.sinks);  // the same for the whole warpgroup
         const uint32_t held = there[(n / 2) % kThere];
-        const int box = p.table ? min(p.page, kWideTile) : kWideTile;
-        const uint32_t all = (1u << (kWideTile / box)) - 1;
-        const bool clear = held == all && ((j0 >= s.full_lo && j0 + kWideTile <= s.full_hi) || j0 + kWideTile <= min(p.sinks, s.full_hi));
+        const bool clear = held == all && ((j0 >= full_lo && j0 + width <= full_hi) || j0 + width <= min(p.sinks, full_hi));
         uint32_t sr[128];
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) tmem_ld32(s_addr + c, sr + c);
-        tmem_wait_ld();
         float* sc = reinterpret_cast<float*>(sr);
+        float top = -INFINITY;
+        // Keys that this row does not see get -inf, 32 at a time where any row of the warp needs it.
+        auto mask32 = [&](int c) {
+          uint32_t bits = seen_bits<TREE>(view, j0 + 32 * c, s.off, p.sinks);
+          if (held != all) {
+            if (!((held >> (32 * c / box)) & 1)) bits &= 0xffff0000u;
+            if (!((held >> ((32 * c + 16) / box)) & 1)) bits &= 0x0000ffffu;
+          }
+          if (__all_sync(0xffffffffu, bits == 0xffffffffu)) return;
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((bits >> e) & 1)) sc[32 * c + e] = -INFINITY;
+        };
+        auto top32 = [&](int c) {
+          float t[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) t[x] = max3f(sc[32 * c + x], sc[32 * c + 4 + x], sc[32 * c + 8 + x]);
+#pragma unroll
+          for (int y = 12; y < 28; y += 8)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) t[x] = max3f(t[x], sc[32 * c + y + x], sc[32 * c + y + 4 + x]);
+          top = fmaxf(top, fmaxf(max3f(t[0], t[1], sc[32 * c + 28]), max3f(t[2], t[3], sc[32 * c + 29])));
+          top = max3f(top, sc[32 * c + 30], sc[32 * c + 31]);
+        };
+        tmem_ld32(s_addr, sr);
+        if (width > 32) tmem_ld32(s_addr + 32, sr + 32);
+        tmem_wait_ld();
+        if (width > 64) tmem_ld32(s_addr + 64, sr + 64);  // on their way while the first are looked at
+        if (width > 96) tmem_ld32(s_addr + 96, sr + 96);
         if (!clear) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t bits = seen_bits<TREE>(view, j0 + 32 * c, s.off, p.sinks) & below(s.len - (j0 + 32 * c));
-            if (held != all) {
-              uint32_t good = 0;
-              for (int x = 0; x < 32; x += 16)
-                if ((held >> ((32 * c + x) / box)) & 1) good |= 0xffffu << x;
-              bits &= good;
-            }
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((bits >> e) & 1)) sc[32 * c + e] = -INFINITY;
-          }
-          // V rows behind the sequence may hold anything (0 * NaN is a NaN): they become zeros before
-          // this thread's arrival, for which the product waits.  Both warpgroups write the same zeros.
-          if (j0 + kWideTile > s.len) {
-            const int vs = (n + 1) % ST;
-            ok = WIDE_ALL(mbar_wait_bounded(full(vs), ((n + 1) / ST) & 1, abort_flag, 77));
-            if (!ok) break;
-            uint8_t* vt = smem + C::OFF_RING + vs * C::TILE_BYTES;
-            if (j0 + row >= s.len) {
-#pragma unroll
-              for (int x = 0; x < D / 8; ++x) *reinterpret_cast<uint4*>(vt + (x >> 3) * C::HALF + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-          }
+          mask32(0);
+          if (width > 32) mask32(1);
         }
-        float t0 = max3f(sc[0], sc[1], sc[2]), t1 = max3f(sc[3], sc[4], sc[5]);
-#pragma unroll
-        for (int c = 6; c < 126; c += 4) {
-          t0 = max3f(t0, sc[c], sc[c + 1]);
-          t1 = max3f(t1, sc[c + 2], sc[c + 3]);
+        top32(0);
+        if (width > 32) top32(1);
+        tmem_wait_ld();
+        if (width > 64) {
+          if (!clear) mask32(2);
+          top32(2);
         }
-        const float top = max3f(fmaxf(t0, t1), sc[126], sc[127]) * p.scale_log2;
+        if (width > 96) {
+          if (!clear) mask32(3);
+          top32(3);
+        }
+        // V rows behind the sequence may hold anything (0 * NaN is a NaN): they become zeros before this
+        // thread's arrival, for which the product waits.  Both warpgroups write the same zeros.
+        if (j0 + width > s.len) {
+          const int vs = (n + 1) % ST;
+          ok = WIDE_ALL(mbar_wait_bounded(full(vs), ((n + 1) / ST) & 1, abort_flag, 77));
+          if (!ok) break;
+          uint8_t* vt = smem + C::OFF_RING + vs * C::TILE_BYTES;
+          if (j0 + row >= s.len) {
+#pragma unroll
+            for (int x = 0; x < D / 8; ++x) *reinterpret_cast<uint4*>(vt + (x >> 3) * C::HALF + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        top *= p.scale_log2;
         const bool raise = top > m + kWideRaise;
         if (__any_sync(0xffffffffu, raise)) {
           const float mn = raise ? top : m;
           const float keep = m == mn ? 1.f : ex2_approx(m - mn);
           m = mn;
-          l *= keep;
+          l0.x *= keep, l0.y *= keep, l1.x *= keep, l1.y *= keep;
           if (begun) {
             // the products of the tiles before this one are complete: they were issued before its scores
 #pragma unroll
@@ -420,27 +485,29 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         begun = true;
         const float ref = m == -INFINITY ? 0.f : m;
         const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), ref2 = make_float2(-ref, -ref);
-        float2 l0 = make_float2(0.f, 0.f), l1 = l0;
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) {
+        auto exp32 = [&](int c) {
           uint32_t pk[16];
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const float2 a = __ffma2_rn(make_float2(sc[c + 2 * e], sc[c + 2 * e + 1]), mul2, ref2);
-            const float2 b = __ffma2_rn(make_float2(sc[c + 2 * e + 2], sc[c + 2 * e + 3]), mul2, ref2);
-            const float2 ea = make_float2(ex2_approx(a.x), ex2_approx(a.y)), eb = make_float2(ex2_approx(b.x), ex2_approx(b.y));
-            l0 = __fadd2_rn(l0, ea);
-            l1 = __fadd2_rn(l1, eb);
-            pk[e] = pack2<T>(ea.x, ea.y);
-            pk[e + 1] = pack2<T>(eb.x, eb.y);
+          for (int e = 0; e < 16; ++e) {
+            const float2 x = __ffma2_rn(make_float2(sc[32 * c + 2 * e], sc[32 * c + 2 * e + 1]), mul2, ref2);
+            const float2 y = e % kPolyEvery == kPolyEvery - 1 ? exp2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            if (e & 1) l1 = __fadd2_rn(l1, y); else l0 = __fadd2_rn(l0, y);
+            pk[e] = pack2<T>(y.x, y.y);
           }
-          tmem_st16(s_addr + c / 2, pk);
-        }
-        l += (l0.x + l0.y) + (l1.x + l1.y);
+          tmem_st16(s_addr + 16 * c, pk);
+        };
+        exp32(0);
+        if (width > 32) exp32(1);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(p_half(i));
+        if (width > 64) exp32(2);
+        if (width > 96) exp32(3);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_full(i));
       }
+      float l = (l0.x + l0.y) + (l1.x + l1.y);
       // ---- rows out.  The warps of a row tile leave together when a wait was abandoned.
       ok = vote_barrier(1 + i, ok && *abort_flag == 0);
       if (!ok) break;
@@ -499,12 +566,14 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       }
       tc_fence_before();
       __syncwarp();
-#pragma unroll 4
-      for (int a = 0; a < 32 / PER; ++a) {
-        const int piece = lane % PIECES, rl = w4 * 32 + a * PER + lane / PIECES, rr = s.rb * kWideRows + i * 128 + rl;
-        if (rr < p.rows) {
-          T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + rr % p.group) * p.tokens + rr / p.group) * D + piece * 8;
-          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(q_tile + (piece >> 3) * C::HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4));
+      {
+        const int piece = lane % PIECES, rl0 = w4 * 32 + lane / PIECES;
+        T* out0 = static_cast<T*>(p.out) + (static_cast<int64_t>(s.b) * p.heads + static_cast<int64_t>(h) * p.group) * p.tokens * D + piece * 8;
+#pragma unroll 8
+        for (int a = 0; a < 32 / PER; ++a) {
+          const int rl = rl0 + a * PER, rr = s.rb * kWideRows + i * 128 + rl, tq = token_of(p, rr);
+          const uint4 x = *reinterpret_cast<const uint4*>(q_tile + (piece >> 3) * C::HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4));
+          if (rr < p.rows) *reinterpret_cast<uint4*>(out0 + (static_cast<int64_t>(rr - tq * p.group) * p.tokens + tq) * D) = x;
         }
       }
       uint32_t vote = __ballot_sync(0xffffffffu, bad);
@@ -512,7 +581,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       while (vote) {  // rows with a value that is not finite, evaluated again from their own keys
         const int src = __ffs(vote) - 1, rr = s.rb * kWideRows + i * 128 + w4 * 32 + src;
         vote &= vote - 1;
-        plain_row<T, false, D>(p, s.b, h, rr, s.off, s.len, row_view(p, s.off, s.len, rr / p.group, TREE ? tm : nullptr), TREE);
+        plain_row<T, false, D>(p, s.b, h, rr, s.off, s.len, row_view(p, s.off, s.len, token_of(p, rr), TREE ? tm : nullptr), TREE);
       }
     }
   }
@@ -530,6 +599,7 @@ int launch_wide(AttendParams p, int device, cudaStream_t st) {
   using C = Wide<D>;
   static_assert(C::SMEM <= 227 * 1024, "shared memory of one CTA");
   p.row_blocks = (p.rows + kWideRows - 1) / kWideRows;
+  p.key_align = p.table ? (p.page < kWideTile ? p.page : kWideTile) : 8;
   CUtensorMap tk, tv;
   int rc;
   const int box = p.table ? (p.page < kWideTile ? p.page : kWideTile) : kWideTile, lines = p.table ? 1 : D / 64;
