@@ -6,16 +6,19 @@
 //
 // One CTA per SM works on 256 query rows of one key head (two 128-row tiles; row = token * group +
 // query head of the group, so that a tile's rows stand close together and share their window) over
-// 128-key tiles:
+// 64-key tiles:
 //   - two softmax warpgroups, one per row tile, a thread per row: scores from tensor memory, running
 //     maximum and sum in registers, probabilities back to tensor memory over the scores;
-//   - an MMA warp: S = Q K^T from shared memory, O += P V with P from tensor memory; the two row
-//     tiles take turns, so that one's softmax runs beside the other's products;
+//   - an MMA warp: S = Q K^T from shared memory, O += P V with P from tensor memory;
 //   - a copy warp: K and V tiles by TMA through one ring.
-// Tensor memory: two score buffers of 128 columns, two accumulators of D columns.  A score buffer's
-// next product is issued behind the product that reads the probabilities in it; products run in the
-// order of issue.  An accumulator is rescaled by its softmax warpgroup, and only when a row's maximum
-// has grown by more than 2^8 since its last reference.
+// Tensor memory: per row tile two score buffers of 64 columns and an accumulator of D columns.  The
+// scores of tile u + 1 are issued before the products with the probabilities of tile u, so that the
+// softmax warpgroups need not wait for them; probabilities lie over their own scores, and a buffer's
+// next scores are issued behind the product that reads them (products run in the order of issue).
+// With 128-key tiles there is room for one buffer only, and each warpgroup waited for 1300 of 4050
+// cycles per 128 keys (prompts of 8192 tokens, window 1024, 4 x 32 heads: 815 us).
+// An accumulator is rescaled by its softmax warpgroup, and only when a row's maximum has grown by
+// more than 2^8 since its last reference.
 // V is read as it lies in memory (keys in rows): the B operand is taken transposed.
 #pragma once
 
@@ -24,16 +27,15 @@
 namespace pk {
 namespace {
 
-constexpr int kWideTile = 128;
+constexpr int kWideTile = 64;
 constexpr int kWideRows = 256;
 constexpr int kWideThreads = 3 * 128;  // two softmax warpgroups, one with the MMA and the copy warp
 // Registers of a thread after the split; setmaxnreg only moves what the CTA was launched with.
-constexpr int kWideLaunchRegs = 168, kSoftmaxRegs = 216, kHelperRegs = 64;
+constexpr int kWideLaunchRegs = 168, kSoftmaxRegs = 168, kHelperRegs = 168;
 static_assert((2 * kSoftmaxRegs + kHelperRegs) * 128 <= kWideThreads * kWideLaunchRegs, "register split exceeds the CTA's registers");
 constexpr float kWideRaise = 8.f;
 constexpr int kWideWorkers = 148;
 constexpr int64_t kWideShareBelow = 4 * kWideWorkers;
-constexpr int kThere = 8;  // a copy is issued at most six key tiles ahead of a tile whose V is still in use
 
 #define WIDE_ALL(x) __all_sync(0xffffffffu, (x))
 
@@ -45,17 +47,18 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
 
 template <int D>
 struct Wide {
-  static constexpr int HALF = kWideTile * 128;                 // 128 rows of 64 features
-  static constexpr int TILE_BYTES = HALF * (D / 64);           // a K, V or Q tile
-  static constexpr int STAGES = D == 128 ? 5 : 10;
+  static constexpr int HALF = kWideTile * 128;  // 64 features of a K or V tile
+  static constexpr int TILE_BYTES = HALF * (D / 64);
+  static constexpr int Q_HALF = 128 * 128, Q_BYTES = Q_HALF * (D / 64);  // a row tile
+  static constexpr int STAGES = D == 128 ? 5 : 8;  // a stage holds a K tile and its V tile
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_RING = 2 * TILE_BYTES;
-  static constexpr int OFF_TREE = OFF_RING + STAGES * TILE_BYTES;
+  static constexpr int OFF_RING = 2 * Q_BYTES;
+  static constexpr int OFF_TREE = OFF_RING + STAGES * 2 * TILE_BYTES;
   static constexpr int OFF_BAR = OFF_TREE + 2 * static_cast<int>(sizeof(TreeMasks));
-  static constexpr int BARS = 2 * STAGES + 2 * 5;  // ring full / empty; q_full, s_full, p_half, p_full, o_done per row tile
+  static constexpr int BARS = 2 * STAGES + 9;  // ring full / empty; s_full (2), p_full (2 per row tile), q_full per row tile, o_done
   static constexpr int OFF_RED = OFF_BAR + BARS * 8;
   static constexpr int OFF_THERE = OFF_RED + 64;
-  static constexpr int OFF_MISC = OFF_THERE + kThere * 4;
+  static constexpr int OFF_MISC = OFF_THERE + STAGES * 4;
   static constexpr int SMEM = OFF_MISC + 16;
   static constexpr uint32_t COL_S = 0, COL_O = 256;
 };
@@ -90,7 +93,7 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t addr, int half) {
 // largest relative error with value 1 at 0 (2.9e-6, measured over r in 32-bit arithmetic); n goes into
 // the exponent.  Below -127 the result is 0 (r = 0 there).  A NaN or infinity may come out as any huge
 // number: the row is then not finite and is evaluated again.
-constexpr int kPolyEvery = 4;
+constexpr int kPolyEvery = 8;
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
   float a, b;
   asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(a) : "f"(x.x));  // -127
@@ -110,6 +113,18 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
 // Sixteen bytes from global to shared memory, asynchronously; `bytes` 0: zeros.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// A bounded wait with little code (the roles' loops should stay in the instruction caches): gives up
+// after some 2^24 probes, or when another wait has been given up.
+__device__ __forceinline__ bool wide_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int where) {
+  for (int n = 0; !mbar_try_wait(bar, parity); ++n) {
+    if ((n & 63) == 63 && (*abort_flag != 0 || n > (1 << 24))) {
+      *abort_flag = where;
+      return false;
+    }
+  }
+  return true;
 }
 
 // What one CTA does next: tiles [tile, tile + count) of one unit.  Every role walks the same list.
@@ -141,12 +156,10 @@ __device__ __forceinline__ Reach reach_of(const AttendParams& p, const Span& s, 
   r.lo = max(0, (TREE ? s.off : s.off + t0) - p.window + 1);
   return r;
 }
-__device__ __forceinline__ bool needs(const Reach& r, int j0, int sinks) { return j0 < r.hi && (j0 + kWideTile > r.lo || j0 < sinks); }
-
-// How many of a tile's keys, from its first on, a row tile has to look at (a multiple of 32).
+// How many of a tile's keys, from its first on, a row tile has to look at (a multiple of 32; 0: none).
 __device__ __forceinline__ int width_of(const Reach& r, int j0, int sinks) {
   const int end = j0 + kWideTile > r.lo ? r.hi : min(sinks, r.hi);
-  return min((end - j0 + 31) & ~31, kWideTile);
+  return max(0, min((end - j0 + 31) & ~31, kWideTile));
 }
 
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }  // bits [0, n)
@@ -178,17 +191,16 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   const uint32_t bars = base + C::OFF_BAR;
   auto full = [&](int i) { return bars + 8 * i; };
   auto empty = [&](int i) { return bars + 8 * (ST + i); };
-  auto q_full = [&](int i) { return bars + 8 * (2 * ST + i); };
-  auto s_full = [&](int i) { return bars + 8 * (2 * ST + 2 + i); };
-  auto p_half = [&](int i) { return bars + 8 * (2 * ST + 4 + i); };
-  auto p_full = [&](int i) { return bars + 8 * (2 * ST + 6 + i); };
-  auto o_done = [&](int i) { return bars + 8 * (2 * ST + 8 + i); };
+  auto s_full = [&](uint32_t n) { return bars + 8 * (2 * ST + (n & 1)); };                  // scores of the n-th key tile, both row tiles
+  auto p_full = [&](int i, uint32_t n) { return bars + 8 * (2 * ST + 2 + 2 * i + (n & 1)); };  // probabilities of row tile i's n-th
+  auto q_full = [&](int i) { return bars + 8 * (2 * ST + 6 + i); };
+  const uint32_t o_done = bars + 8 * (2 * ST + 8);  // the products of a segment
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int MMA_WARP = 8, COPY_WARP = 9;
 
   if (tid < C::BARS) {
-    const int kind = tid < 2 * ST ? 1 : (tid - 2 * ST) / 2;
-    mbar_init(bars + 8 * tid, kind == 1 || kind == 4 ? 1 : 128);  // q_full, p_half, p_full: a warpgroup
+    const int at = tid - 2 * ST;
+    mbar_init(bars + 8 * tid, at >= 2 && at < 8 ? 128 : 1);  // p_full, q_full: a warpgroup
     fence_barrier_init();
   }
   if (tid == 0) *abort_flag = 0;
@@ -226,47 +238,45 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     // ---------------------------------------------------------------- copies
     if (lane == 0) {
       const int box = p.table ? min(p.page, kWideTile) : kWideTile;
-      int n = 0;  // tiles issued, K and V counted one after the other
+      uint32_t st = 0, ph = 1;
+      int n = 0;  // tiles issued
       bool ok = true;
       for (; ok && seg.left > 0; seg.advance(p)) {
+        const Span& s = seg.walk.s;
         const int count = seg.count(), from = seg.walk.tile;
-        for (int u = 0; ok && u < count; ++u) {
-          const Span& s = seg.walk.s;
+        for (int u = 0; u < count; ++u, ++n) {
           const int j0 = key_of_tile<kWideTile>(s, from + u);
-          int pages[kWideTile / 16];
-          uint32_t mask = 1u;
-          if (p.table) {
-            mask = 0;
+          if (n >= ST && !(ok = wide_wait(empty(st), ph, abort_flag, 71))) break;
+          const uint32_t dst = base + C::OFF_RING + st * 2 * C::TILE_BYTES;
+          if (!p.table) {
+            there[st] = 1u;
+            mbar_expect_tx(full(st), 2 * C::TILE_BYTES);
+            tma_load_5d(dst, &tm_k, full(st), 0, j0, 0, p.k_stride[1] ? seg.walk.h : 0, p.k_stride[0] ? s.b : 0);
+            tma_load_5d(dst + C::TILE_BYTES, &tm_v, full(st), 0, j0, 0, p.v_stride[1] ? seg.walk.h : 0, p.v_stride[0] ? s.b : 0);
+          } else {
+            int pages[kWideTile / 16];
+            uint32_t mask = 0;
 #pragma unroll
             for (int x = 0; x < kWideTile / 16; ++x) {
               const int j = j0 + x * box;
               pages[x] = (x * box < kWideTile && j < s.len) ? attend_page(p, s.b, j) : -1;
               if (pages[x] >= 0) mask |= 1u << x;
             }
-          }
-#pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv, ++n) {
-            const int st = n % ST;
-            if (n >= ST && !mbar_wait_bounded(empty(st), ((n / ST) - 1) & 1, abort_flag, 71)) { ok = false; break; }
-            const uint32_t dst = base + C::OFF_RING + st * C::TILE_BYTES;
-            const CUtensorMap* tmap = kv ? &tm_v : &tm_k;
-            if (kv == 0) there[(n / 2) % kThere] = mask;
-            mbar_expect_tx(full(st), C::TILE_BYTES);
-            if (!p.table) {
-              const int64_t* str = kv ? p.v_stride : p.k_stride;
-              tma_load_5d(dst, tmap, full(st), 0, j0, 0, str[1] ? seg.walk.h : 0, str[0] ? s.b : 0);
-            } else {
+            there[st] = mask;
+            mbar_expect_tx(full(st), 2 * C::TILE_BYTES);
 #pragma unroll
-              for (int x = 0; x < kWideTile / 16; ++x) {
-                if (x * box >= kWideTile) break;
-                const int row = (j0 + x * box) & (p.page - 1);
-                const int c4 = pages[x] >= 0 ? p.page_base + pages[x] : 0x7fffffff;
+            for (int x = 0; x < kWideTile / 16; ++x) {
+              if (x * box >= kWideTile) break;
+              const int row = (j0 + x * box) & (p.page - 1);
+              const int c4 = pages[x] >= 0 ? p.page_base + pages[x] : 0x7fffffff;
 #pragma unroll
-                for (int hf = 0; hf < D / 64; ++hf)
-                  tma_load_5d(dst + hf * C::HALF + x * box * 128, tmap, full(st), 0, row, hf, seg.walk.h, c4);
+              for (int hf = 0; hf < D / 64; ++hf) {
+                tma_load_5d(dst + hf * C::HALF + x * box * 128, &tm_k, full(st), 0, row, hf, seg.walk.h, c4);
+                tma_load_5d(dst + C::TILE_BYTES + hf * C::HALF + x * box * 128, &tm_v, full(st), 0, row, hf, seg.walk.h, c4);
               }
             }
           }
+          if (++st == ST) st = 0, ph ^= 1;
         }
       }
       if (*abort_flag != 0) {  // let the copies that were issued land before the CTA returns
@@ -275,79 +285,94 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     }
   } else if (warp == MMA_WARP) {
     // ---------------------------------------------------------------- products
-    constexpr uint32_t id_o = wide_idesc<T>(D, true);
-    int n = 0;                     // tiles consumed, K and V counted one after the other
-    int np[2] = {0, 0}, nq = 0;    // probability tiles, segments
+    // On everybody's critical path: scalars only, descriptors built once, two commits per key tile (one
+    // costs more than a hundred cycles of this warp: with six of them 743 instead of MEASURED us, 8192
+    // tokens, 32 heads, no window).
+    constexpr uint32_t id_o = wide_idesc<T>(D, true), id_s0 = wide_idesc<T>(0, false);
+    const uint64_t q_desc = umma_smem_desc(base + C::OFF_Q, 128), k_desc = umma_smem_desc(base + C::OFF_RING, 128);
+    const uint64_t v_desc0 = v_desc(base + C::OFF_RING + C::TILE_BYTES, C::HALF);
+    uint32_t st = 0, ph = 0, v_st = 0;                // stage of tile u + 1, of tile u
+    uint32_t nt = 0, np0 = 0, np1 = 0, nq = 0;  // key tiles, probability tiles, segments so far
+    auto scores = [&](int i, int width, uint64_t kd) {
+      const uint32_t d = tmem + C::COL_S + i * 128 + (nt & 1) * 64, id = id_s0 | (static_cast<uint32_t>(width >> 3) << 17);
+      const uint64_t qd = q_desc + i * (C::Q_BYTES >> 4);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+        umma_f16_ss(d, qd + ((k >> 2) * (C::Q_HALF >> 4) + 2 * (k & 3)), kd + ((k >> 2) * (C::HALF >> 4) + 2 * (k & 3)), id, k > 0);
+    };
+    auto values = [&](int i, uint32_t tile, int width, uint64_t vd, bool more) {
+      const uint32_t d = tmem + C::COL_O + i * 128, a = tmem + C::COL_S + i * 128 + (tile & 1) * 64;
+#pragma unroll
+      for (int k = 0; k < kWideTile / 16; k += 2) {
+        if (16 * k < width) {
+          umma_f16_ts(d, a + k * 8, vd + k * (2048 >> 4), id_o, more || k > 0);
+          umma_f16_ts(d, a + k * 8 + 8, vd + (k + 1) * (2048 >> 4), id_o, 1);
+        }
+      }
+    };
     bool ok = true;
     for (; ok && seg.left > 0; seg.advance(p), ++nq) {
       const Span& s = seg.walk.s;
       const int count = seg.count(), from = seg.walk.tile;
-      const Reach reach[2] = {reach_of<TREE>(p, s, 0), reach_of<TREE>(p, s, 1)};
-      bool begun[2] = {false, false};
-      auto key = [&](int u) { return key_of_tile<kWideTile>(s, from + u); };
-      for (int i = 0; ok && i < 2; ++i) ok = WIDE_ALL(mbar_wait_bounded(q_full(i), nq & 1, abort_flag, 75));
+      const Reach r0 = reach_of<TREE>(p, s, 0), r1 = reach_of<TREE>(p, s, 1);
+      bool more0 = false, more1 = false;
+      int w0 = 0, w1 = 0;  // widths of tile u for the two row tiles, 0: not needed
+      ok = WIDE_ALL(wide_wait(q_full(0), nq & 1, abort_flag, 75)) && WIDE_ALL(wide_wait(q_full(1), nq & 1, abort_flag, 75));
       tc_fence_after();
       for (int u = -1; ok && u < count; ++u) {
-        // V of tile u sits at ring position n + 2u + 1, K of tile u + 1 at n + 2u + 2
-        const int vn = n + 2 * u + 1, kn = n + 2 * u + 2;
-        if (u >= 0) ok = WIDE_ALL(mbar_wait_bounded(full(vn % ST), (vn / ST) & 1, abort_flag, 72));
-        if (ok && u + 1 < count) ok = WIDE_ALL(mbar_wait_bounded(full(kn % ST), (kn / ST) & 1, abort_flag, 73));
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (ok && u >= 0 && needs(reach[i], key(u), p.sinks)) {
-            // the first 64 keys' probabilities come first: their product runs while the others are evaluated
-            const int steps = width_of(reach[i], key(u), p.sinks) / 16;
-            const uint64_t vd = v_desc(base + C::OFF_RING + (vn % ST) * C::TILE_BYTES, C::HALF);
-            const uint32_t o = tmem + C::COL_O + i * 128, pr = tmem + C::COL_S + i * 128;
-            ok = WIDE_ALL(mbar_wait_bounded(p_half(i), np[i] & 1, abort_flag, 74));
+        int x0 = 0, x1 = 0;
+        if (u + 1 < count) {
+          const int j0 = key_of_tile<kWideTile>(s, from + u + 1);
+          x0 = width_of(r0, j0, p.sinks), x1 = width_of(r1, j0, p.sinks);
+          ok = WIDE_ALL(wide_wait(full(st), ph, abort_flag, 73));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t kd = k_desc + st * (2 * C::TILE_BYTES >> 4);
+          if (elect_one()) {
+            if (x0) scores(0, x0, kd);
+            if (x1) scores(1, x1, kd);
+            tc_commit(s_full(nt));
+          }
+          ++nt;
+        }
+        if (u >= 0) {
+          const uint64_t vd = v_desc0 + v_st * (2 * C::TILE_BYTES >> 4);
+          const uint32_t tile = nt - (u + 1 < count ? 2 : 1);
+          if (w0) {
+            ok = WIDE_ALL(wide_wait(p_full(0, np0), (np0 >> 1) & 1, abort_flag, 74));
             if (!ok) break;
             tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (k < steps) umma_f16_ts(o, pr + k * 8, vd + k * (2048 >> 4), id_o, begun[i] || k > 0);
-            }
-            ok = WIDE_ALL(mbar_wait_bounded(p_full(i), np[i] & 1, abort_flag, 79));
+            if (elect_one()) values(0, tile, w0, vd, more0);
+            ++np0, more0 = true;
+          }
+          if (w1) {
+            ok = WIDE_ALL(wide_wait(p_full(1, np1), (np1 >> 1) & 1, abort_flag, 79));
             if (!ok) break;
-            ++np[i];
             tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int k = 4; k < 8; ++k)
-                if (k < steps) umma_f16_ts(o, pr + k * 8, vd + k * (2048 >> 4), id_o, 1);
-              tc_commit(o_done(i));
-            }
-            begun[i] = true;
+            if (elect_one()) values(1, tile, w1, vd, more1);
+            ++np1, more1 = true;
           }
-          if (ok && u + 1 < count && needs(reach[i], key(u + 1), p.sinks)) {
-            const uint32_t qa = base + C::OFF_Q + i * C::TILE_BYTES, ka = base + C::OFF_RING + (kn % ST) * C::TILE_BYTES;
-            const uint32_t id_s = wide_idesc<T>(0, false) | (static_cast<uint32_t>(width_of(reach[i], key(u + 1), p.sinks) >> 3) << 17);
-            if (elect_one()) {
-#pragma unroll
-              for (int k = 0; k < D / 16; ++k)
-                umma_f16_ss(tmem + C::COL_S + i * 128, umma_smem_desc(qa + (k >> 2) * C::HALF, 128) + 2 * (k & 3),
-                            umma_smem_desc(ka + (k >> 2) * C::HALF, 128) + 2 * (k & 3), id_s, k > 0);
-              tc_commit(s_full(i));
-            }
+          if (elect_one()) {  // complete with everything issued so far
+            tc_commit(empty(v_st));
+            if (u + 1 == count) tc_commit(o_done);
           }
         }
-        if (!ok) break;
-        if (elect_one()) {  // completes with everything issued so far
-          if (u >= 0) tc_commit(empty(vn % ST));
-          if (u + 1 < count) tc_commit(empty(kn % ST));
-        }
+        v_st = st;
+        if (u + 1 < count && ++st == ST) st = 0, ph ^= 1;
+        w0 = x0, w1 = x1;
       }
-      n += 2 * count;
     }
   } else if (warp < 8) {
     setmaxnreg_inc<kSoftmaxRegs>();
     // ---------------------------------------------------------------- softmax, one warpgroup per row tile
     const int i = warp >> 2, row = tid & 127, w4 = warp & 3;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(w4 * 32) << 16);
-    const uint32_t s_addr = lanes + C::COL_S + i * 128, o_addr = lanes + C::COL_O + i * 128;
-    uint8_t* q_tile = smem + C::OFF_Q + i * C::TILE_BYTES;
+    const uint32_t o_addr = lanes + C::COL_O + i * 128;
+    uint8_t* q_tile = smem + C::OFF_Q + i * C::Q_BYTES;
     TreeMasks* tm = reinterpret_cast<TreeMasks*>(smem + C::OFF_TREE) + i;
-    int ns = 0, n = 0, tree_b = -1;
+    uint32_t nt = 0, np = 0, nq = 0;  // key tiles, probability tiles of this row tile, segments so far
+    uint32_t st = 0;
+    int tree_b = -1;
     bool ok = true;
     const int64_t share_from = seg.left;
     const int box = p.table ? min(p.page, kWideTile) : kWideTile;
@@ -370,7 +395,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         for (int a = 0; a < 32 / PER; ++a) {
           const int rl = rl0 + a * PER, r = s.rb * kWideRows + i * 128 + rl, tq = token_of(p, r);
           const T* src = q0 + (r - tq * p.group) * p.q_stride[1] + tq * p.q_stride[2];
-          uint8_t* dst = q_tile + (piece >> 3) * C::HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4);
+          uint8_t* dst = q_tile + (piece >> 3) * C::Q_HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4);
           if (p.q_vec) {
             copy16(smem_u32(dst), r < p.rows ? src : q0, r < p.rows ? 16 : 0);
           } else {
@@ -390,20 +415,21 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       float m = -INFINITY;
       float2 l0 = make_float2(0.f, 0.f), l1 = l0;
       bool begun = false;
+      uint32_t last_st = 0, last_ph = 0;
       // keys that every row of this row tile sees
       const int t_first = token_of(p, min(s.rb * kWideRows + i * 128, p.rows - 1)), t_last = token_of(p, min(s.rb * kWideRows + i * 128 + 127, p.rows - 1));
       const int full_hi = TREE ? s.full_hi : min(s.len, s.off + t_first + 1), full_lo = TREE ? s.full_lo : s.off + t_last - p.window + 1;
-      for (int u = 0; u < count; ++u, n += 2) {
+      for (int u = 0; u < count; ++u, ++nt, st = st + 1 == ST ? 0 : st + 1) {
         const int j0 = key_of_tile<kWideTile>(s, from + u);
-        if (!needs(reach, j0, p.sinks)) continue;
-        ok = WIDE_ALL(mbar_wait_bounded(s_full(i), ns & 1, abort_flag, 76));
-        if (!ok) break;
-        ++ns;
-        tc_fence_after();
         const int width = width_of(reach, j0, p.sinks);  // the same for the whole warpgroup
-        const uint32_t held = there[(n / 2) % kThere];
+        ok = WIDE_ALL(wide_wait(s_full(nt), (nt >> 1) & 1, abort_flag, 76));
+        if (!ok) break;
+        if (width == 0) continue;
+        const uint32_t s_addr = lanes + C::COL_S + i * 128 + (nt & 1) * 64;
+        tc_fence_after();
+        const uint32_t held = there[st];
         const bool clear = held == all && ((j0 >= full_lo && j0 + width <= full_hi) || j0 + width <= min(p.sinks, full_hi));
-        uint32_t sr[128];
+        uint32_t sr[64];
         float* sc = reinterpret_cast<float*>(sr);
         float top = -INFINITY;
         // Keys that this row does not see get -inf, 32 at a time where any row of the warp needs it.
@@ -432,31 +458,19 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         tmem_ld32(s_addr, sr);
         if (width > 32) tmem_ld32(s_addr + 32, sr + 32);
         tmem_wait_ld();
-        if (width > 64) tmem_ld32(s_addr + 64, sr + 64);  // on their way while the first are looked at
-        if (width > 96) tmem_ld32(s_addr + 96, sr + 96);
-        if (!clear) {
-          mask32(0);
-          if (width > 32) mask32(1);
-        }
+        if (!clear) mask32(0);
         top32(0);
-        if (width > 32) top32(1);
-        tmem_wait_ld();
-        if (width > 64) {
-          if (!clear) mask32(2);
-          top32(2);
-        }
-        if (width > 96) {
-          if (!clear) mask32(3);
-          top32(3);
+        if (width > 32) {
+          if (!clear) mask32(1);
+          top32(1);
         }
         // V rows behind the sequence may hold anything (0 * NaN is a NaN): they become zeros before this
         // thread's arrival, for which the product waits.  Both warpgroups write the same zeros.
         if (j0 + width > s.len) {
-          const int vs = (n + 1) % ST;
-          ok = WIDE_ALL(mbar_wait_bounded(full(vs), ((n + 1) / ST) & 1, abort_flag, 77));
+          ok = WIDE_ALL(wide_wait(full(st), (nt / ST) & 1, abort_flag, 77));
           if (!ok) break;
-          uint8_t* vt = smem + C::OFF_RING + vs * C::TILE_BYTES;
-          if (j0 + row >= s.len) {
+          uint8_t* vt = smem + C::OFF_RING + st * 2 * C::TILE_BYTES + C::TILE_BYTES;
+          if (row < kWideTile && j0 + row >= s.len) {
 #pragma unroll
             for (int x = 0; x < D / 8; ++x) *reinterpret_cast<uint4*>(vt + (x >> 3) * C::HALF + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
@@ -470,7 +484,10 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           m = mn;
           l0.x *= keep, l0.y *= keep, l1.x *= keep, l1.y *= keep;
           if (begun) {
-            // the products of the tiles before this one are complete: they were issued before its scores
+            // the product of this row tile's latest key tile has to be complete; the next waits for this thread
+            ok = WIDE_ALL(wide_wait(empty(last_st), last_ph, abort_flag, 80));
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D; c += 16) {
               uint32_t o[16];
@@ -500,22 +517,18 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         if (width > 32) exp32(1);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(p_half(i));
-        if (width > 64) exp32(2);
-        if (width > 96) exp32(3);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(p_full(i));
+        mbar_arrive(p_full(i, np));
+        ++np;
+        last_st = st, last_ph = (nt / ST) & 1;
       }
       float l = (l0.x + l0.y) + (l1.x + l1.y);
       // ---- rows out.  The warps of a row tile leave together when a wait was abandoned.
       ok = vote_barrier(1 + i, ok && *abort_flag == 0);
       if (!ok) break;
       const bool whole = from == 0 && count == s.n;
-      if (begun) {
-        if (!WIDE_ALL(mbar_wait_bounded(o_done(i), (ns - 1) & 1, abort_flag, 78))) l = __int_as_float(0x7fc00000);
-        tc_fence_after();
-      }
+      if (!WIDE_ALL(wide_wait(o_done, nq & 1, abort_flag, 78))) l = __int_as_float(0x7fc00000);
+      ++nq;
+      tc_fence_after();
       const int idx = s.off + t;
       const bool valid = r < p.rows && idx >= 0 && idx < s.len;
       if (!whole) {
@@ -560,7 +573,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             bad |= !(fabsf(x[y]) <= 3.0e38f);
           }
           const int piece = (c + e) / 8;
-          *reinterpret_cast<uint4*>(q_tile + (piece >> 3) * C::HALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(q_tile + (piece >> 3) * C::Q_HALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) =
               make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
         }
       }
@@ -572,7 +585,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 #pragma unroll 8
         for (int a = 0; a < 32 / PER; ++a) {
           const int rl = rl0 + a * PER, rr = s.rb * kWideRows + i * 128 + rl, tq = token_of(p, rr);
-          const uint4 x = *reinterpret_cast<const uint4*>(q_tile + (piece >> 3) * C::HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4));
+          const uint4 x = *reinterpret_cast<const uint4*>(q_tile + (piece >> 3) * C::Q_HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4));
           if (rr < p.rows) *reinterpret_cast<uint4*>(out0 + (static_cast<int64_t>(rr - tq * p.group) * p.tokens + tq) * D) = x;
         }
       }
