@@ -415,7 +415,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       if (!ok) l[x] = __int_as_float(0x7FC00000);
       if (c4 == 0) ml[warp * 16 + g8 + 8 * x] = make_float2(m[x], l[x]);
     }
-    ok = vote_barrier(1, ok && *abort_flag == 0);  // the same answer in every warp: they leave together
+    ok = vote_barrier(1, kConsumers, ok && *abort_flag == 0);  // the same answer in every warp: they leave together
     const int slot = blockIdx.x * 2 + (unit_from == 0 && w - unit_tiles != w0 ? 1 : 0);
     float* piece = p.partial + static_cast<int64_t>(slot) * C::ROWS * (D + 2);
     // thread -> (row, four consecutive columns) of the CTA's rows; a row's columns belong to 8 neighbouring threads

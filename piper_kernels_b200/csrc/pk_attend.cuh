@@ -121,14 +121,14 @@ __device__ __forceinline__ void build_tree(const AttendParams& p, int b, int off
   __syncwarp();
 }
 
-// Barrier `id` of 128 threads; true when `good` holds in all of them.
-__device__ __forceinline__ bool vote_barrier(int id, bool good) {
+// Barrier `id` of `threads` threads; true when `good` holds in all of them.
+__device__ __forceinline__ bool vote_barrier(int id, int threads, bool good) {
   uint32_t all;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\t"
-      "barrier.cta.red.and.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(all)
-      : "r"(id), "r"(static_cast<uint32_t>(good))
+      : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(good))
       : "memory");
   return all != 0;
 }
@@ -191,9 +191,10 @@ __device__ __forceinline__ __nv_bfloat16 from_f32(float a) { return __float2bflo
 // One output row from its visible keys alone, one key after the other, by one warp; lane i holds
 // features [i * D/32, (i+1) * D/32).  The tiled kernels multiply whole tiles, so that an infinity
 // or NaN in a V row that this query row must not see would still reach it (0 * NaN); a row that
-// comes out of them with a value that is not finite is evaluated again here.  Rare, and slow.
+// comes out of them with a value that is not finite is evaluated again here (its features
+// [first, last) are written).  Rare, and slow.
 template <typename T, bool I8, int D>
-__device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, int row, int off, int len, RowView view, bool tree) {
+__device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, int row, int off, int len, RowView view, bool tree, int first = 0, int last = D) {
   constexpr int E = D / 32;
   const int lane = threadIdx.x & 31, t = token_of(p, row), head = kvh * p.group + row - t * p.group;
   const T* q = static_cast<const T*>(p.q) + b * p.q_stride[0] + head * p.q_stride[1] + t * p.q_stride[2] + lane * E;
@@ -243,7 +244,8 @@ __device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, in
   }
   T* out = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.heads + head) * p.tokens + t) * D + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = from_f32<T>(l == 0.f ? 0.f : acc[e] / l);
+  for (int e = 0; e < E; ++e)
+    if (lane * E + e >= first && lane * E + e < last) out[e] = from_f32<T>(l == 0.f ? 0.f : acc[e] / l);
 }
 
 // ---------------------------------------------------------------------------------------

@@ -6,19 +6,23 @@
 //
 // One CTA per SM works on 256 query rows of one key head (two 128-row tiles; row = token * group +
 // query head of the group, so that a tile's rows stand close together and share their window) over
-// 64-key tiles:
-//   - two softmax warpgroups, one per row tile, a thread per row: scores from tensor memory, running
-//     maximum and sum in registers, probabilities back to tensor memory over the scores;
-//   - an MMA warp: S = Q K^T from shared memory, O += P V with P from tensor memory;
+// 128-key tiles:
+//   - four softmax warpgroups, two per row tile on 64 keys each, a thread per row: scores from tensor
+//     memory, maximum, sum, probabilities back to tensor memory over the scores;
+//   - an MMA warp: S = Q K^T from shared memory, O += P V with P from tensor memory; the row tiles take
+//     turns, so that one's softmax runs beside the other's products;
 //   - a copy warp: K and V tiles by TMA through one ring.
-// Tensor memory: per row tile two score buffers of 64 columns and an accumulator of D columns.  The
-// scores of tile u + 1 are issued before the products with the probabilities of tile u, so that the
-// softmax warpgroups need not wait for them; probabilities lie over their own scores, and a buffer's
-// next scores are issued behind the product that reads them (products run in the order of issue).
-// With 128-key tiles there is room for one buffer only, and each warpgroup waited for 1300 of 4050
-// cycles per 128 keys (prompts of 8192 tokens, window 1024, 4 x 32 heads: 815 us).
-// An accumulator is rescaled by its softmax warpgroup, and only when a row's maximum has grown by
-// more than 2^8 since its last reference.
+// Tensor memory holds one score tile of 128 columns and one accumulator per row tile, no more: a row
+// tile's scores, softmax and products follow one another, and the time of this chain is the kernel's.
+// So the softmax keeps it short:
+//   - Probabilities are relative to a reference exponent that follows the running maximum only when that
+//     has grown by more than 2^8.  The exponentials start with the reference of the tile before, without
+//     waiting for this tile's maximum; only when a row has to raise it (the first tile, and rarely later)
+//     they are evaluated again, and the accumulator is rescaled.
+//   - A part of the exponentials is evaluated on the FMA pipe beside the exponential unit.
+// Tried and slower (prompt of 8192, 32 heads, no window): one warpgroup per row tile MEASURED1; 64-key tiles
+// with two score buffers per row tile, with one or two warpgroups per row tile and one or two issuing
+// warps, 660 to 870 us: the smaller tiles halve what is in flight per buffer and every hand-over costs the same.
 // V is read as it lies in memory (keys in rows): the B operand is taken transposed.
 #pragma once
 
@@ -27,13 +31,14 @@
 namespace pk {
 namespace {
 
-constexpr int kWideTile = 64;
+constexpr int kWideTile = 128;
 constexpr int kWideRows = 256;
-constexpr int kWideThreads = 3 * 128;  // two softmax warpgroups, one with the MMA and the copy warp
+constexpr int kWideThreads = 5 * 128;  // four softmax warpgroups, one with the MMA and the copy warp
 // Registers of a thread after the split; setmaxnreg only moves what the CTA was launched with.
-constexpr int kWideLaunchRegs = 168, kSoftmaxRegs = 168, kHelperRegs = 168;
-static_assert((2 * kSoftmaxRegs + kHelperRegs) * 128 <= kWideThreads * kWideLaunchRegs, "register split exceeds the CTA's registers");
+constexpr int kWideLaunchRegs = 96, kSoftmaxRegs = 104, kHelperRegs = 64;
+static_assert((4 * kSoftmaxRegs + kHelperRegs) * 128 <= kWideThreads * kWideLaunchRegs, "register split exceeds the CTA's registers");
 constexpr float kWideRaise = 8.f;
+constexpr int kThere = 8;  // a copy is issued at most STAGES / 2 + 1 key tiles ahead of a tile whose V is still in use
 constexpr int kWideWorkers = 148;
 constexpr int64_t kWideShareBelow = 4 * kWideWorkers;
 
@@ -45,21 +50,22 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
   return r;
 }
 
-template <int D>
+template <int D, bool TREE>
 struct Wide {
-  static constexpr int HALF = kWideTile * 128;  // 64 features of a K or V tile
-  static constexpr int TILE_BYTES = HALF * (D / 64);
-  static constexpr int Q_HALF = 128 * 128, Q_BYTES = Q_HALF * (D / 64);  // a row tile
-  static constexpr int STAGES = D == 128 ? 5 : 8;  // a stage holds a K tile and its V tile
+  static constexpr int HALF = 128 * 128;                // 128 rows of 64 features
+  static constexpr int TILE_BYTES = HALF * (D / 64);    // a K, V or Q tile
+  static constexpr int STAGES = D == 128 ? (TREE ? 4 : 5) : 10;
+  static_assert(STAGES / 2 + 1 < kThere, "entries of `there` outlive their tiles");
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_RING = 2 * Q_BYTES;
-  static constexpr int OFF_TREE = OFF_RING + STAGES * 2 * TILE_BYTES;
-  static constexpr int OFF_BAR = OFF_TREE + 2 * static_cast<int>(sizeof(TreeMasks));
-  static constexpr int BARS = 2 * STAGES + 9;  // ring full / empty; s_full (2), p_full (2 per row tile), q_full per row tile, o_done
-  static constexpr int OFF_RED = OFF_BAR + BARS * 8;
+  static constexpr int OFF_RING = 2 * TILE_BYTES;
+  static constexpr int OFF_TOP = OFF_RING + STAGES * TILE_BYTES;  // [row tile][half][128]: maxima, then sums
+  static constexpr int OFF_BAR = OFF_TOP + 2 * 2 * 128 * 4;
+  static constexpr int BARS = 2 * STAGES + 7;  // ring full / empty; q_full, s_full, p_full per row tile, o_done
+  static constexpr int OFF_RED = OFF_BAR + (BARS + 1) / 2 * 16;
   static constexpr int OFF_THERE = OFF_RED + 64;
-  static constexpr int OFF_MISC = OFF_THERE + STAGES * 4;
-  static constexpr int SMEM = OFF_MISC + 16;
+  static constexpr int OFF_MISC = OFF_THERE + kThere * 4;
+  static constexpr int OFF_TREE = (OFF_MISC + 8 + 7) / 8 * 8;
+  static constexpr int SMEM = OFF_TREE + (TREE ? 2 * static_cast<int>(sizeof(TreeMasks)) : 0);
   static constexpr uint32_t COL_S = 0, COL_O = 256;
 };
 
@@ -179,7 +185,7 @@ __device__ __forceinline__ uint32_t seen_bits(const RowView& v, int j, int off, 
 template <typename T, int D, bool TREE>
 __global__ void __launch_bounds__(kWideThreads, 1)
 wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttendParams p) {
-  using C = Wide<D>;
+  using C = Wide<D, TREE>;
   constexpr int ST = C::STAGES;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
@@ -191,16 +197,16 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   const uint32_t bars = base + C::OFF_BAR;
   auto full = [&](int i) { return bars + 8 * i; };
   auto empty = [&](int i) { return bars + 8 * (ST + i); };
-  auto s_full = [&](uint32_t n) { return bars + 8 * (2 * ST + (n & 1)); };                  // scores of the n-th key tile, both row tiles
-  auto p_full = [&](int i, uint32_t n) { return bars + 8 * (2 * ST + 2 + 2 * i + (n & 1)); };  // probabilities of row tile i's n-th
-  auto q_full = [&](int i) { return bars + 8 * (2 * ST + 6 + i); };
-  const uint32_t o_done = bars + 8 * (2 * ST + 8);  // the products of a segment
+  auto q_full = [&](int i) { return bars + 8 * (2 * ST + i); };
+  auto s_full = [&](int i) { return bars + 8 * (2 * ST + 2 + i); };
+  auto p_full = [&](int i) { return bars + 8 * (2 * ST + 4 + i); };
+  const uint32_t o_done = bars + 8 * (2 * ST + 6);  // the products of a segment
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int MMA_WARP = 8, COPY_WARP = 9;
+  constexpr int MMA_WARP = 16, COPY_WARP = 17;
 
   if (tid < C::BARS) {
     const int at = tid - 2 * ST;
-    mbar_init(bars + 8 * tid, at >= 2 && at < 8 ? 128 : 1);  // p_full, q_full: a warpgroup
+    mbar_init(bars + 8 * tid, at < 0 || at == 2 || at == 3 || at == 6 ? 1 : 256);  // q_full, p_full: two warpgroups
     fence_barrier_init();
   }
   if (tid == 0) *abort_flag = 0;
@@ -233,50 +239,52 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     seg.left = seg.walk.s.n;
   }
 
-  if (warp >= 8) setmaxnreg_dec<kHelperRegs>();
+  if (warp >= 16) setmaxnreg_dec<kHelperRegs>();
   if (warp == COPY_WARP) {
     // ---------------------------------------------------------------- copies
     if (lane == 0) {
       const int box = p.table ? min(p.page, kWideTile) : kWideTile;
       uint32_t st = 0, ph = 1;
-      int n = 0;  // tiles issued
+      int n = 0;  // K and V tiles issued
       bool ok = true;
       for (; ok && seg.left > 0; seg.advance(p)) {
         const Span& s = seg.walk.s;
         const int count = seg.count(), from = seg.walk.tile;
-        for (int u = 0; u < count; ++u, ++n) {
+        for (int u = 0; ok && u < count; ++u) {
           const int j0 = key_of_tile<kWideTile>(s, from + u);
-          if (n >= ST && !(ok = wide_wait(empty(st), ph, abort_flag, 71))) break;
-          const uint32_t dst = base + C::OFF_RING + st * 2 * C::TILE_BYTES;
-          if (!p.table) {
-            there[st] = 1u;
-            mbar_expect_tx(full(st), 2 * C::TILE_BYTES);
-            tma_load_5d(dst, &tm_k, full(st), 0, j0, 0, p.k_stride[1] ? seg.walk.h : 0, p.k_stride[0] ? s.b : 0);
-            tma_load_5d(dst + C::TILE_BYTES, &tm_v, full(st), 0, j0, 0, p.v_stride[1] ? seg.walk.h : 0, p.v_stride[0] ? s.b : 0);
-          } else {
-            int pages[kWideTile / 16];
-            uint32_t mask = 0;
+          int pages[kWideTile / 16];
+          uint32_t mask = 1u;
+          if (p.table) {
+            mask = 0;
 #pragma unroll
             for (int x = 0; x < kWideTile / 16; ++x) {
               const int j = j0 + x * box;
               pages[x] = (x * box < kWideTile && j < s.len) ? attend_page(p, s.b, j) : -1;
               if (pages[x] >= 0) mask |= 1u << x;
             }
-            there[st] = mask;
-            mbar_expect_tx(full(st), 2 * C::TILE_BYTES);
+          }
+          there[(n / 2) % kThere] = mask;
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv, ++n) {
+            if (n >= ST && !(ok = wide_wait(empty(st), ph, abort_flag, 71))) break;
+            const uint32_t dst = base + C::OFF_RING + st * C::TILE_BYTES;
+            const CUtensorMap* tmap = kv ? &tm_v : &tm_k;
+            mbar_expect_tx(full(st), C::TILE_BYTES);
+            if (!p.table) {
+              const int64_t sh = kv ? p.v_stride[1] : p.k_stride[1], sb = kv ? p.v_stride[0] : p.k_stride[0];
+              tma_load_5d(dst, tmap, full(st), 0, j0, 0, sh ? seg.walk.h : 0, sb ? s.b : 0);
+            } else {
 #pragma unroll
-            for (int x = 0; x < kWideTile / 16; ++x) {
-              if (x * box >= kWideTile) break;
-              const int row = (j0 + x * box) & (p.page - 1);
-              const int c4 = pages[x] >= 0 ? p.page_base + pages[x] : 0x7fffffff;
+              for (int x = 0; x < kWideTile / 16; ++x) {
+                if (x * box >= kWideTile) break;
+                const int row = (j0 + x * box) & (p.page - 1);
+                const int c4 = pages[x] >= 0 ? p.page_base + pages[x] : 0x7fffffff;
 #pragma unroll
-              for (int hf = 0; hf < D / 64; ++hf) {
-                tma_load_5d(dst + hf * C::HALF + x * box * 128, &tm_k, full(st), 0, row, hf, seg.walk.h, c4);
-                tma_load_5d(dst + C::TILE_BYTES + hf * C::HALF + x * box * 128, &tm_v, full(st), 0, row, hf, seg.walk.h, c4);
+                for (int hf = 0; hf < D / 64; ++hf) tma_load_5d(dst + hf * C::HALF + x * box * 128, tmap, full(st), 0, row, hf, seg.walk.h, c4);
               }
             }
+            if (++st == ST) st = 0, ph ^= 1;
           }
-          if (++st == ST) st = 0, ph ^= 1;
         }
       }
       if (*abort_flag != 0) {  // let the copies that were issued land before the CTA returns
@@ -285,30 +293,37 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     }
   } else if (warp == MMA_WARP) {
     // ---------------------------------------------------------------- products
-    // On everybody's critical path: scalars only, descriptors built once, two commits per key tile (one
-    // costs more than a hundred cycles of this warp: with six of them 743 instead of MEASURED us, 8192
-    // tokens, 32 heads, no window).
+    // Scalars only, descriptors built once: this warp is in everybody's chain.
     constexpr uint32_t id_o = wide_idesc<T>(D, true), id_s0 = wide_idesc<T>(0, false);
     const uint64_t q_desc = umma_smem_desc(base + C::OFF_Q, 128), k_desc = umma_smem_desc(base + C::OFF_RING, 128);
-    const uint64_t v_desc0 = v_desc(base + C::OFF_RING + C::TILE_BYTES, C::HALF);
-    uint32_t st = 0, ph = 0, v_st = 0;                // stage of tile u + 1, of tile u
-    uint32_t nt = 0, np0 = 0, np1 = 0, nq = 0;  // key tiles, probability tiles, segments so far
+    const uint64_t v_desc0 = v_desc(base + C::OFF_RING, C::HALF);
+    uint32_t k_st = 0, k_ph = 0, v_st = 1, v_ph = 0;  // stages of K of tile u + 1 and of V of tile u
+    uint32_t ph0 = 0, ph1 = 0, nq = 0;                // phases of the p_full barriers, segments so far
     auto scores = [&](int i, int width, uint64_t kd) {
-      const uint32_t d = tmem + C::COL_S + i * 128 + (nt & 1) * 64, id = id_s0 | (static_cast<uint32_t>(width >> 3) << 17);
-      const uint64_t qd = q_desc + i * (C::Q_BYTES >> 4);
+      const uint32_t d = tmem + C::COL_S + i * 128, id = id_s0 | (static_cast<uint32_t>(width >> 3) << 17);
+      const uint64_t qd = q_desc + i * (C::TILE_BYTES >> 4);
+      if (elect_one()) {
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k)
-        umma_f16_ss(d, qd + ((k >> 2) * (C::Q_HALF >> 4) + 2 * (k & 3)), kd + ((k >> 2) * (C::HALF >> 4) + 2 * (k & 3)), id, k > 0);
+        for (int k = 0; k < D / 16; ++k)
+          umma_f16_ss(d, qd + ((k >> 2) * (C::HALF >> 4) + 2 * (k & 3)), kd + ((k >> 2) * (C::HALF >> 4) + 2 * (k & 3)), id, k > 0);
+        tc_commit(s_full(i));
+      }
     };
-    auto values = [&](int i, uint32_t tile, int width, uint64_t vd, bool more) {
-      const uint32_t d = tmem + C::COL_O + i * 128, a = tmem + C::COL_S + i * 128 + (tile & 1) * 64;
+    auto values = [&](int i, int width, uint64_t vd, bool more) {
+      const uint32_t d = tmem + C::COL_O + i * 128, a = tmem + C::COL_S + i * 128;
+      if (elect_one()) {
 #pragma unroll
-      for (int k = 0; k < kWideTile / 16; k += 2) {
-        if (16 * k < width) {
-          umma_f16_ts(d, a + k * 8, vd + k * (2048 >> 4), id_o, more || k > 0);
-          umma_f16_ts(d, a + k * 8 + 8, vd + (k + 1) * (2048 >> 4), id_o, 1);
+        for (int k = 0; k < kWideTile / 16; k += 2) {
+          if (16 * k < width) {  // the second 64 keys' probabilities lie over their own scores
+            umma_f16_ts(d, a + (k >> 2) * 64 + (k & 3) * 8, vd + k * (2048 >> 4), id_o, more || k > 0);
+            umma_f16_ts(d, a + (k >> 2) * 64 + (k & 3) * 8 + 8, vd + (k + 1) * (2048 >> 4), id_o, 1);
+          }
         }
       }
+    };
+    auto turn = [&](uint32_t& stage, uint32_t& phase) {
+      stage += 2;
+      if (stage >= ST) stage -= ST, phase ^= 1;
     };
     bool ok = true;
     for (; ok && seg.left > 0; seg.advance(p), ++nq) {
@@ -317,85 +332,90 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       const Reach r0 = reach_of<TREE>(p, s, 0), r1 = reach_of<TREE>(p, s, 1);
       bool more0 = false, more1 = false;
       int w0 = 0, w1 = 0;  // widths of tile u for the two row tiles, 0: not needed
-      ok = WIDE_ALL(wide_wait(q_full(0), nq & 1, abort_flag, 75)) && WIDE_ALL(wide_wait(q_full(1), nq & 1, abort_flag, 75));
-      tc_fence_after();
       for (int u = -1; ok && u < count; ++u) {
         int x0 = 0, x1 = 0;
         if (u + 1 < count) {
           const int j0 = key_of_tile<kWideTile>(s, from + u + 1);
           x0 = width_of(r0, j0, p.sinks), x1 = width_of(r1, j0, p.sinks);
-          ok = WIDE_ALL(wide_wait(full(st), ph, abort_flag, 73));
+          ok = WIDE_ALL(wide_wait(full(k_st), k_ph, abort_flag, 73));
+        }
+        if (ok && u >= 0) ok = WIDE_ALL(wide_wait(full(v_st), v_ph, abort_flag, 72));
+        if (!ok) break;
+        const uint64_t kd = k_desc + k_st * (C::TILE_BYTES >> 4), vd = v_desc0 + v_st * (C::TILE_BYTES >> 4);
+        if (w0) {
+          ok = WIDE_ALL(wide_wait(p_full(0), ph0, abort_flag, 74));
           if (!ok) break;
+          ph0 ^= 1;
           tc_fence_after();
-          const uint64_t kd = k_desc + st * (2 * C::TILE_BYTES >> 4);
-          if (elect_one()) {
-            if (x0) scores(0, x0, kd);
-            if (x1) scores(1, x1, kd);
-            tc_commit(s_full(nt));
-          }
-          ++nt;
+          values(0, w0, vd, more0);
+          more0 = true;
         }
-        if (u >= 0) {
-          const uint64_t vd = v_desc0 + v_st * (2 * C::TILE_BYTES >> 4);
-          const uint32_t tile = nt - (u + 1 < count ? 2 : 1);
-          if (w0) {
-            ok = WIDE_ALL(wide_wait(p_full(0, np0), (np0 >> 1) & 1, abort_flag, 74));
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) values(0, tile, w0, vd, more0);
-            ++np0, more0 = true;
-          }
-          if (w1) {
-            ok = WIDE_ALL(wide_wait(p_full(1, np1), (np1 >> 1) & 1, abort_flag, 79));
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) values(1, tile, w1, vd, more1);
-            ++np1, more1 = true;
-          }
-          if (elect_one()) {  // complete with everything issued so far
-            tc_commit(empty(v_st));
-            if (u + 1 == count) tc_commit(o_done);
-          }
+        if (u < 0 && !(ok = WIDE_ALL(wide_wait(q_full(0), nq & 1, abort_flag, 75)))) break;
+        tc_fence_after();
+        if (x0) scores(0, x0, kd);
+        if (w1) {
+          ok = WIDE_ALL(wide_wait(p_full(1), ph1, abort_flag, 79));
+          if (!ok) break;
+          ph1 ^= 1;
+          tc_fence_after();
+          values(1, w1, vd, more1);
+          more1 = true;
         }
-        v_st = st;
-        if (u + 1 < count && ++st == ST) st = 0, ph ^= 1;
+        if (u < 0 && !(ok = WIDE_ALL(wide_wait(q_full(1), nq & 1, abort_flag, 75)))) break;
+        tc_fence_after();
+        if (x1) scores(1, x1, kd);
+        if (elect_one()) {  // complete with everything issued so far
+          if (u >= 0) tc_commit(empty(v_st));
+          if (u + 1 < count) tc_commit(empty(k_st));
+          else tc_commit(o_done);
+        }
+        if (u >= 0) turn(v_st, v_ph);
+        if (u + 1 < count) turn(k_st, k_ph);
         w0 = x0, w1 = x1;
       }
     }
-  } else if (warp < 8) {
+  } else if (warp < 16) {
     setmaxnreg_inc<kSoftmaxRegs>();
-    // ---------------------------------------------------------------- softmax, one warpgroup per row tile
-    const int i = warp >> 2, row = tid & 127, w4 = warp & 3;
+    // ---------------------------------------------------------------- softmax
+    // Row tile i; of each key tile the 64 keys of half `half`, of its features (query rows in, output
+    // rows out) likewise.
+    const int i = (warp >> 2) & 1, half = warp >> 3, row = tid & 127, w4 = warp & 3;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(w4 * 32) << 16);
-    const uint32_t o_addr = lanes + C::COL_O + i * 128;
-    uint8_t* q_tile = smem + C::OFF_Q + i * C::Q_BYTES;
+    const uint32_t o_addr = lanes + C::COL_O + i * 128 + half * (D / 2), s_addr = lanes + C::COL_S + i * 128 + half * 64;
+    constexpr int FEATURES = D / 2, PIECES = FEATURES / 8, PER = 32 / PIECES;  // 16-byte pieces of a row's half, rows per access
+    uint8_t* q_tile = smem + C::OFF_Q + i * C::TILE_BYTES;
+    auto q_piece = [&](int r, int piece) {  // of this half
+      const int at = half * PIECES + piece;
+      return q_tile + (at >> 3) * C::HALF + r * 128 + (((at & 7) ^ (r & 7)) << 4);
+    };
+    float* tops = reinterpret_cast<float*>(smem + C::OFF_TOP) + i * 256 + row;
     TreeMasks* tm = reinterpret_cast<TreeMasks*>(smem + C::OFF_TREE) + i;
-    uint32_t nt = 0, np = 0, nq = 0;  // key tiles, probability tiles of this row tile, segments so far
-    uint32_t st = 0;
-    int tree_b = -1;
-    bool ok = true;
-    const int64_t share_from = seg.left;
     const int box = p.table ? min(p.page, kWideTile) : kWideTile;
     const uint32_t all = (1u << (kWideTile / box)) - 1;
+    const int64_t share_from = seg.left;
+    uint32_t nt = 0, ns = 0, nq = 0;  // key tiles, those that this row tile needed, and segments so far
+    int tree_b = -1;
+    bool ok = true;
     for (; ok && seg.left > 0; seg.advance(p)) {
       const Span& s = seg.walk.s;
       const int count = seg.count(), from = seg.walk.tile, h = seg.walk.h;
       const Reach reach = reach_of<TREE>(p, s, i);
+      const int row0 = s.rb * kWideRows + i * 128;
       if (TREE && s.b != tree_b) {
-        if (w4 == 0) build_tree(p, s.b, s.off, lane, tm);
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+        asm volatile("bar.sync %0, 256;" ::"r"(1 + i) : "memory");  // the previous masks have been used
+        if (w4 == 0 && half == 0) build_tree(p, s.b, s.off, lane, tm);
+        asm volatile("bar.sync %0, 256;" ::"r"(1 + i) : "memory");
         tree_b = s.b;
       }
-      // ---- the tile's query rows into shared memory; a warp takes whole rows of its own 32
-      constexpr int PIECES = D / 8, PER = 32 / PIECES;  // 16-byte pieces per row, rows per access
+      // ---- the query rows into shared memory
       {
         const int piece = lane % PIECES, rl0 = w4 * 32 + lane / PIECES;
-        const T* q0 = static_cast<const T*>(p.q) + s.b * p.q_stride[0] + static_cast<int64_t>(h) * p.group * p.q_stride[1] + piece * 8;
+        const T* q0 = static_cast<const T*>(p.q) + s.b * p.q_stride[0] + static_cast<int64_t>(h) * p.group * p.q_stride[1] + half * FEATURES + piece * 8;
 #pragma unroll
         for (int a = 0; a < 32 / PER; ++a) {
-          const int rl = rl0 + a * PER, r = s.rb * kWideRows + i * 128 + rl, tq = token_of(p, r);
+          const int rl = rl0 + a * PER, r = row0 + rl, tq = token_of(p, r);
           const T* src = q0 + (r - tq * p.group) * p.q_stride[1] + tq * p.q_stride[2];
-          uint8_t* dst = q_tile + (piece >> 3) * C::Q_HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4);
+          uint8_t* dst = q_piece(rl, piece);
           if (p.q_vec) {
             copy16(smem_u32(dst), r < p.rows ? src : q0, r < p.rows ? 16 : 0);
           } else {
@@ -410,86 +430,87 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       fence_proxy_async_smem();
       mbar_arrive(q_full(i));
 
-      const int r = s.rb * kWideRows + i * 128 + row, t = token_of(p, r);
+      const int r = row0 + row, t = token_of(p, r);
       const RowView view = r < p.rows ? row_view(p, s.off, s.len, t, TREE ? tm : nullptr) : RowView{0, 0, 0};
-      float m = -INFINITY;
-      float2 l0 = make_float2(0.f, 0.f), l1 = l0;
-      bool begun = false;
-      uint32_t last_st = 0, last_ph = 0;
       // keys that every row of this row tile sees
-      const int t_first = token_of(p, min(s.rb * kWideRows + i * 128, p.rows - 1)), t_last = token_of(p, min(s.rb * kWideRows + i * 128 + 127, p.rows - 1));
+      const int t_first = token_of(p, min(row0, p.rows - 1)), t_last = token_of(p, min(row0 + 127, p.rows - 1));
       const int full_hi = TREE ? s.full_hi : min(s.len, s.off + t_first + 1), full_lo = TREE ? s.full_lo : s.off + t_last - p.window + 1;
-      for (int u = 0; u < count; ++u, ++nt, st = st + 1 == ST ? 0 : st + 1) {
+      float ref = -INFINITY, l = 0.f;  // reference exponent of the probabilities, sum of this half's
+      bool begun = false;
+      for (int u = 0; u < count; ++u, ++nt) {
         const int j0 = key_of_tile<kWideTile>(s, from + u);
-        const int width = width_of(reach, j0, p.sinks);  // the same for the whole warpgroup
-        ok = WIDE_ALL(wide_wait(s_full(nt), (nt >> 1) & 1, abort_flag, 76));
-        if (!ok) break;
+        const int width = width_of(reach, j0, p.sinks), mine = width - 64 * half;  // the same for the whole warpgroup
         if (width == 0) continue;
-        const uint32_t s_addr = lanes + C::COL_S + i * 128 + (nt & 1) * 64;
+        ok = WIDE_ALL(wide_wait(s_full(i), ns & 1, abort_flag, 76));
+        ++ns;
         tc_fence_after();
-        const uint32_t held = there[st];
+        const uint32_t held = there[nt % kThere];
         const bool clear = held == all && ((j0 >= full_lo && j0 + width <= full_hi) || j0 + width <= min(p.sinks, full_hi));
-        uint32_t sr[64];
+        uint32_t sr[32], pk[32];
         float* sc = reinterpret_cast<float*>(sr);
-        float top = -INFINITY;
-        // Keys that this row does not see get -inf, 32 at a time where any row of the warp needs it.
+        float top, shift;
+        float2 l0, l1;
+        const float2 mul2 = make_float2(p.scale_log2, p.scale_log2);
+        // 32 keys in sr: those that this row does not see get -inf, where any row of the warp needs it
         auto mask32 = [&](int c) {
-          uint32_t bits = seen_bits<TREE>(view, j0 + 32 * c, s.off, p.sinks);
+          const int at = 64 * half + 32 * c;
+          uint32_t bits = seen_bits<TREE>(view, j0 + at, s.off, p.sinks);
           if (held != all) {
-            if (!((held >> (32 * c / box)) & 1)) bits &= 0xffff0000u;
-            if (!((held >> ((32 * c + 16) / box)) & 1)) bits &= 0x0000ffffu;
+            if (!((held >> (at / box)) & 1)) bits &= 0xffff0000u;
+            if (!((held >> ((at + 16) / box)) & 1)) bits &= 0x0000ffffu;
           }
           if (__all_sync(0xffffffffu, bits == 0xffffffffu)) return;
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (!((bits >> e) & 1)) sc[32 * c + e] = -INFINITY;
+            if (!((bits >> e) & 1)) sc[e] = -INFINITY;
         };
-        auto top32 = [&](int c) {
-          float t[4];
+        auto pass = [&](int c) {  // exponentials relative to the reference, and the maximum beside them
+          tmem_ld32(s_addr + 32 * c, sr);
+          tmem_wait_ld();
+          if (!clear) mask32(c);
+          const float2 shift2 = make_float2(shift, shift);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) t[x] = max3f(sc[32 * c + x], sc[32 * c + 4 + x], sc[32 * c + 8 + x]);
-#pragma unroll
-          for (int y = 12; y < 28; y += 8)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) t[x] = max3f(t[x], sc[32 * c + y + x], sc[32 * c + y + 4 + x]);
-          top = fmaxf(top, fmaxf(max3f(t[0], t[1], sc[32 * c + 28]), max3f(t[2], t[3], sc[32 * c + 29])));
-          top = max3f(top, sc[32 * c + 30], sc[32 * c + 31]);
+          for (int e = 0; e < 16; ++e) {
+            top = max3f(top, sc[2 * e], sc[2 * e + 1]);
+            const float2 x = __ffma2_rn(make_float2(sc[2 * e], sc[2 * e + 1]), mul2, shift2);
+            const float2 y = e % kPolyEvery == kPolyEvery - 1 ? exp2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            if (e & 1) l1 = __fadd2_rn(l1, y); else l0 = __fadd2_rn(l0, y);
+            pk[16 * c + e] = pack2<T>(y.x, y.y);
+          }
         };
-        tmem_ld32(s_addr, sr);
-        if (width > 32) tmem_ld32(s_addr + 32, sr + 32);
-        tmem_wait_ld();
-        if (!clear) mask32(0);
-        top32(0);
-        if (width > 32) {
-          if (!clear) mask32(1);
-          top32(1);
-        }
+        auto passes = [&]() {
+          top = -INFINITY, shift = ref == -INFINITY ? 0.f : -ref;
+          l0 = l1 = make_float2(0.f, 0.f);
+          if (mine > 0) pass(0);
+          if (mine > 32) pass(1);
+        };
+        passes();
         // V rows behind the sequence may hold anything (0 * NaN is a NaN): they become zeros before this
-        // thread's arrival, for which the product waits.  Both warpgroups write the same zeros.
+        // thread's arrival, for which the product waits.  All warpgroups write the same zeros.
         if (j0 + width > s.len) {
-          ok = WIDE_ALL(wide_wait(full(st), (nt / ST) & 1, abort_flag, 77));
-          if (!ok) break;
-          uint8_t* vt = smem + C::OFF_RING + st * 2 * C::TILE_BYTES + C::TILE_BYTES;
-          if (row < kWideTile && j0 + row >= s.len) {
+          const uint32_t vn = 2 * nt + 1;
+          ok = ok && WIDE_ALL(wide_wait(full(vn % ST), (vn / ST) & 1, abort_flag, 80));
+          uint8_t* vt = smem + C::OFF_RING + vn % ST * C::TILE_BYTES;
+          if (ok && j0 + row >= s.len) {
 #pragma unroll
             for (int x = 0; x < D / 8; ++x) *reinterpret_cast<uint4*>(vt + (x >> 3) * C::HALF + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
         }
         top *= p.scale_log2;
-        const bool raise = top > m + kWideRaise;
-        if (__any_sync(0xffffffffu, raise)) {
-          const float mn = raise ? top : m;
-          const float keep = m == mn ? 1.f : ex2_approx(m - mn);
-          m = mn;
-          l0.x *= keep, l0.y *= keep, l1.x *= keep, l1.y *= keep;
+        // Does a row of the row tile have to raise its reference?  (At the first tile every row that sees a key.)
+        if (!vote_barrier(1 + i, 256, ok && !(top > ref + kWideRaise))) {
+          tops[half * 128] = top;
+          ok = vote_barrier(1 + i, 256, ok && *abort_flag == 0);
+          if (!ok) break;  // the row tile's warps leave together when a wait was abandoned
+          const float most = fmaxf(tops[0], tops[128]);
+          const float now = most > ref + kWideRaise ? most : ref, keep = now == ref ? 1.f : ex2_approx(ref - now);
+          ref = now;
+          l *= keep;
           if (begun) {
-            // the product of this row tile's latest key tile has to be complete; the next waits for this thread
-            ok = WIDE_ALL(wide_wait(empty(last_st), last_ph, abort_flag, 80));
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < D; c += 16) {
+            // the products of the tiles before this one are complete: they were issued before its scores
+#pragma unroll 1
+            for (int c = 0; c < FEATURES; c += 16) {
               uint32_t o[16];
               tmem_ld16(o_addr + c, o);
               tmem_wait_ld();
@@ -498,103 +519,84 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
               tmem_st16(o_addr + c, o);
             }
           }
+          passes();
         }
         begun = true;
-        const float ref = m == -INFINITY ? 0.f : m;
-        const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), ref2 = make_float2(-ref, -ref);
-        auto exp32 = [&](int c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 x = __ffma2_rn(make_float2(sc[32 * c + 2 * e], sc[32 * c + 2 * e + 1]), mul2, ref2);
-            const float2 y = e % kPolyEvery == kPolyEvery - 1 ? exp2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
-            if (e & 1) l1 = __fadd2_rn(l1, y); else l0 = __fadd2_rn(l0, y);
-            pk[e] = pack2<T>(y.x, y.y);
-          }
-          tmem_st16(s_addr + 16 * c, pk);
-        };
-        exp32(0);
-        if (width > 32) exp32(1);
+        l += (l0.x + l0.y) + (l1.x + l1.y);
+        if (mine > 0) tmem_st16(s_addr, pk);
+        if (mine > 32) tmem_st16(s_addr + 16, pk + 16);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(p_full(i, np));
-        ++np;
-        last_st = st, last_ph = (nt / ST) & 1;
+        mbar_arrive(p_full(i));
       }
-      float l = (l0.x + l0.y) + (l1.x + l1.y);
-      // ---- rows out.  The warps of a row tile leave together when a wait was abandoned.
-      ok = vote_barrier(1 + i, ok && *abort_flag == 0);
+      // ---- rows out; the two halves add their sums
+      ok = vote_barrier(1 + i, 256, ok && *abort_flag == 0);  // and the maxima have been read
       if (!ok) break;
-      const bool whole = from == 0 && count == s.n;
+      tops[half * 128] = l;
+      asm volatile("bar.sync %0, 256;" ::"r"(1 + i) : "memory");
+      const float m = ref;
+      l = tops[0] + tops[128];
       if (!WIDE_ALL(wide_wait(o_done, nq & 1, abort_flag, 78))) l = __int_as_float(0x7fc00000);
       ++nq;
       tc_fence_after();
       const int idx = s.off + t;
       const bool valid = r < p.rows && idx >= 0 && idx < s.len;
-      if (!whole) {
+      if (from != 0 || count != s.n) {
         const int slot = blockIdx.x * 2 + (seg.left != share_from ? 1 : 0);
         float* dst = p.partial + (static_cast<int64_t>(slot) * kWideRows + i * 128 + row) * (D + 2);
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
+        for (int c = 0; c < FEATURES; c += 32) {
           uint32_t o[32];
-          if (begun) {
-            tmem_ld32(o_addr + c, o);
-            tmem_wait_ld();
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0;
-          }
+          tmem_ld32(o_addr + c, o);
+          tmem_wait_ld();
           if (r < p.rows) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) *reinterpret_cast<float2*>(dst + c + e) = make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+            for (int e = 0; e < 32; e += 2)
+              *reinterpret_cast<float2*>(dst + half * FEATURES + c + e) = begun ? make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])) : make_float2(0.f, 0.f);
           }
         }
-        if (r < p.rows) *reinterpret_cast<float2*>(dst + D) = make_float2(m, l);
+        if (r < p.rows && half == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m, l);
         tc_fence_before();
         continue;
       }
       // The query tile has been read by every product: its place takes the output rows, from where
-      // they leave as whole rows (a thread's own row would be written 16 bytes at a time).
-      const float inv = valid && l != 0.f ? 1.f / l : 0.f;
+      // they leave as whole lines (a thread's own row would be written 16 bytes at a time).
+      const float inv = valid && begun && l != 0.f ? 1.f / l : 0.f;
       bool bad = false;
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
+      for (int c = 0; c < FEATURES; c += 32) {
         uint32_t o[32];
-        if (begun) {
-          tmem_ld32(o_addr + c, o);
-          tmem_wait_ld();
-        }
+        tmem_ld32(o_addr + c, o);
+        tmem_wait_ld();
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
           float x[8];
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
-            x[y] = begun && inv != 0.f ? __uint_as_float(o[e + y]) * inv : 0.f;
+            x[y] = inv != 0.f ? __uint_as_float(o[e + y]) * inv : 0.f;
             bad |= !(fabsf(x[y]) <= 3.0e38f);
           }
-          const int piece = (c + e) / 8;
-          *reinterpret_cast<uint4*>(q_tile + (piece >> 3) * C::Q_HALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) =
-              make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+          *reinterpret_cast<uint4*>(q_piece(row, (c + e) / 8)) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
         }
       }
       tc_fence_before();
       __syncwarp();
       {
         const int piece = lane % PIECES, rl0 = w4 * 32 + lane / PIECES;
-        T* out0 = static_cast<T*>(p.out) + (static_cast<int64_t>(s.b) * p.heads + static_cast<int64_t>(h) * p.group) * p.tokens * D + piece * 8;
-#pragma unroll 8
+        T* out0 = static_cast<T*>(p.out) + (static_cast<int64_t>(s.b) * p.heads + static_cast<int64_t>(h) * p.group) * p.tokens * D + half * FEATURES + piece * 8;
+#pragma unroll
         for (int a = 0; a < 32 / PER; ++a) {
-          const int rl = rl0 + a * PER, rr = s.rb * kWideRows + i * 128 + rl, tq = token_of(p, rr);
-          const uint4 x = *reinterpret_cast<const uint4*>(q_tile + (piece >> 3) * C::Q_HALF + rl * 128 + (((piece & 7) ^ (rl & 7)) << 4));
+          const int rl = rl0 + a * PER, rr = row0 + rl, tq = token_of(p, rr);
+          const uint4 x = *reinterpret_cast<const uint4*>(q_piece(rl, piece));
           if (rr < p.rows) *reinterpret_cast<uint4*>(out0 + (static_cast<int64_t>(rr - tq * p.group) * p.tokens + tq) * D) = x;
         }
       }
       uint32_t vote = __ballot_sync(0xffffffffu, bad);
       __syncwarp();
       while (vote) {  // rows with a value that is not finite, evaluated again from their own keys
-        const int src = __ffs(vote) - 1, rr = s.rb * kWideRows + i * 128 + w4 * 32 + src;
+        const int src = __ffs(vote) - 1, rr = row0 + w4 * 32 + src;
         vote &= vote - 1;
-        plain_row<T, false, D>(p, s.b, h, rr, s.off, s.len, row_view(p, s.off, s.len, token_of(p, rr), TREE ? tm : nullptr), TREE);
+        plain_row<T, false, D>(p, s.b, h, rr, s.off, s.len, row_view(p, s.off, s.len, token_of(p, rr), TREE ? tm : nullptr), TREE, half * FEATURES, half * FEATURES + FEATURES);
       }
     }
   }
@@ -609,7 +611,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 
 template <typename T, int D, bool TREE>
 int launch_wide(AttendParams p, int device, cudaStream_t st) {
-  using C = Wide<D>;
+  using C = Wide<D, TREE>;
   static_assert(C::SMEM <= 227 * 1024, "shared memory of one CTA");
   p.row_blocks = (p.rows + kWideRows - 1) / kWideRows;
   p.key_align = p.table ? (p.page < kWideTile ? p.page : kWideTile) : 8;
