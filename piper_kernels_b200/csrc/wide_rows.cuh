@@ -60,7 +60,7 @@ struct Wide {
   static constexpr int OFF_RING = 2 * TILE_BYTES;
   static constexpr int OFF_TOP = OFF_RING + STAGES * TILE_BYTES;  // [row tile][half][128]: maxima, then sums
   static constexpr int OFF_BAR = OFF_TOP + 2 * 2 * 128 * 4;
-  static constexpr int BARS = 2 * STAGES + 7;  // ring full / empty; q_full, s_full, p_full per row tile, o_done
+  static constexpr int BARS = 2 * STAGES + 8;  // ring full / empty; q_full, s_full, p_full, o_done per row tile
   static constexpr int OFF_RED = OFF_BAR + (BARS + 1) / 2 * 16;
   static constexpr int OFF_THERE = OFF_RED + 64;
   static constexpr int OFF_MISC = OFF_THERE + kThere * 4;
@@ -133,17 +133,34 @@ __device__ __forceinline__ bool wide_wait(uint32_t bar, uint32_t parity, volatil
   return true;
 }
 
-// What one CTA does next: tiles [tile, tile + count) of one unit.  Every role walks the same list.
+// What one CTA does next: tiles [tile, tile + count) of one unit.  Every role walks the same list: an
+// equal, contiguous share of all tiles, or (when there are many units) every gridDim.x-th unit from the
+// back, where causal rows see the most keys.
 template <bool TREE>
 struct Segments {
   Walk<TREE, kWideTile, kWideRows> walk;
-  int64_t left;
-  __device__ __forceinline__ int count() const { return static_cast<int>(min(static_cast<int64_t>(walk.s.n - walk.tile), left)); }
+  int64_t left;  // shares: tiles; else units
+  int unit;
+  __device__ __forceinline__ void take(const AttendParams& p) {
+    const int at = p.batch * p.row_blocks * p.kv_heads - 1 - unit;
+    walk.g = at / p.kv_heads;
+    walk.h = at - walk.g * p.kv_heads;
+    walk.tile = 0;
+    walk.s = span_of<TREE, kWideTile, kWideRows>(p, walk.g);
+  }
+  __device__ __forceinline__ int count(const AttendParams& p) const {
+    return p.workers ? static_cast<int>(min(static_cast<int64_t>(walk.s.n - walk.tile), left)) : walk.s.n;
+  }
   __device__ __forceinline__ void advance(const AttendParams& p) {
-    const int n = count();
-    left -= n;
-    walk.tile += n - 1;
-    walk.next(p);
+    if (p.workers) {
+      const int n = count(p);
+      left -= n;
+      walk.tile += n - 1;
+      walk.next(p);
+    } else if (--left > 0) {
+      unit += gridDim.x;
+      take(p);
+    }
   }
 };
 
@@ -200,13 +217,13 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   auto q_full = [&](int i) { return bars + 8 * (2 * ST + i); };
   auto s_full = [&](int i) { return bars + 8 * (2 * ST + 2 + i); };
   auto p_full = [&](int i) { return bars + 8 * (2 * ST + 4 + i); };
-  const uint32_t o_done = bars + 8 * (2 * ST + 6);  // the products of a segment
+  auto o_done = [&](int i) { return bars + 8 * (2 * ST + 6 + i); };  // the products of a segment
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int MMA_WARP = 16, COPY_WARP = 17;
 
   if (tid < C::BARS) {
     const int at = tid - 2 * ST;
-    mbar_init(bars + 8 * tid, at < 0 || at == 2 || at == 3 || at == 6 ? 1 : 256);  // q_full, p_full: two warpgroups
+    mbar_init(bars + 8 * tid, at < 0 || at == 2 || at == 3 || at >= 6 ? 1 : 256);  // q_full, p_full: two warpgroups
     fence_barrier_init();
   }
   if (tid == 0) *abort_flag = 0;
@@ -232,11 +249,10 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       seg.walk.start(p, f, w0);
     }
   } else {
-    seg.walk.g = blockIdx.x / p.kv_heads;
-    seg.walk.h = blockIdx.x % p.kv_heads;
-    seg.walk.tile = 0;
-    seg.walk.s = span_of<TREE, kWideTile, kWideRows>(p, seg.walk.g);
-    seg.left = seg.walk.s.n;
+    const int units = p.batch * p.row_blocks * p.kv_heads;
+    seg.unit = blockIdx.x;
+    seg.left = (units - 1 - seg.unit) / static_cast<int>(gridDim.x) + 1;  // no more CTAs than units
+    seg.take(p);
   }
 
   if (warp >= 16) setmaxnreg_dec<kHelperRegs>();
@@ -249,7 +265,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       bool ok = true;
       for (; ok && seg.left > 0; seg.advance(p)) {
         const Span& s = seg.walk.s;
-        const int count = seg.count(), from = seg.walk.tile;
+        const int count = seg.count(p), from = seg.walk.tile;
         for (int u = 0; ok && u < count; ++u) {
           const int j0 = key_of_tile<kWideTile>(s, from + u);
           int pages[kWideTile / 16];
@@ -328,7 +344,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     bool ok = true;
     for (; ok && seg.left > 0; seg.advance(p), ++nq) {
       const Span& s = seg.walk.s;
-      const int count = seg.count(), from = seg.walk.tile;
+      const int count = seg.count(p), from = seg.walk.tile;
       const Reach r0 = reach_of<TREE>(p, s, 0), r1 = reach_of<TREE>(p, s, 1);
       bool more0 = false, more1 = false;
       int w0 = 0, w1 = 0;  // widths of tile u for the two row tiles, 0: not needed
@@ -350,6 +366,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           values(0, w0, vd, more0);
           more0 = true;
         }
+        if (u + 1 == count && elect_one()) tc_commit(o_done(0));
         if (u < 0 && !(ok = WIDE_ALL(wide_wait(q_full(0), nq & 1, abort_flag, 75)))) break;
         tc_fence_after();
         if (x0) scores(0, x0, kd);
@@ -367,7 +384,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         if (elect_one()) {  // complete with everything issued so far
           if (u >= 0) tc_commit(empty(v_st));
           if (u + 1 < count) tc_commit(empty(k_st));
-          else tc_commit(o_done);
+          else tc_commit(o_done(1));
         }
         if (u >= 0) turn(v_st, v_ph);
         if (u + 1 < count) turn(k_st, k_ph);
@@ -398,7 +415,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     bool ok = true;
     for (; ok && seg.left > 0; seg.advance(p)) {
       const Span& s = seg.walk.s;
-      const int count = seg.count(), from = seg.walk.tile, h = seg.walk.h;
+      const int count = seg.count(p), from = seg.walk.tile, h = seg.walk.h;
       const Reach reach = reach_of<TREE>(p, s, i);
       const int row0 = s.rb * kWideRows + i * 128;
       if (TREE && s.b != tree_b) {
@@ -536,12 +553,12 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       asm volatile("bar.sync %0, 256;" ::"r"(1 + i) : "memory");
       const float m = ref;
       l = tops[0] + tops[128];
-      if (!WIDE_ALL(wide_wait(o_done, nq & 1, abort_flag, 78))) l = __int_as_float(0x7fc00000);
+      if (!WIDE_ALL(wide_wait(o_done(i), nq & 1, abort_flag, 78))) l = __int_as_float(0x7fc00000);
       ++nq;
       tc_fence_after();
       const int idx = s.off + t;
       const bool valid = r < p.rows && idx >= 0 && idx < s.len;
-      if (from != 0 || count != s.n) {
+      if (p.workers && (from != 0 || count != s.n)) {
         const int slot = blockIdx.x * 2 + (seg.left != share_from ? 1 : 0);
         float* dst = p.partial + (static_cast<int64_t>(slot) * kWideRows + i * 128 + row) * (D + 2);
 #pragma unroll
@@ -624,7 +641,7 @@ int launch_wide(AttendParams p, int device, cudaStream_t st) {
   const int64_t units = static_cast<int64_t>(p.batch) * p.row_blocks * p.kv_heads;
   const bool share = units < kWideShareBelow;
   p.workers = share ? kWideWorkers : 0;
-  cudaError_t e = launch_chained(wide_rows_kernel<T, D, TREE>, dim3(share ? kWideWorkers : static_cast<unsigned>(units)), dim3(kWideThreads), C::SMEM, st, tk, tv, p);
+  cudaError_t e = launch_chained(wide_rows_kernel<T, D, TREE>, dim3(share || units > kWideWorkers ? kWideWorkers : static_cast<unsigned>(units)), dim3(kWideThreads), C::SMEM, st, tk, tv, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "attention kernel launch failed: %s", cuda_err(e));
   if (!share) return PK_OK;
