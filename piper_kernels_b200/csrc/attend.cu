@@ -89,7 +89,7 @@ size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 bool wide(int rows, bool i8) { return !i8 && rows > 64; }
 
 uint64_t attend_workspace(int batch, int kv_heads, int rows, int head_dim, bool i8) {
-  const uint64_t n = wide(rows, i8) ? wide_rows_workspace(batch, kv_heads, rows, head_dim) : few_rows_workspace(rows, head_dim);
+  const uint64_t n = wide(rows, i8) ? wide_rows_workspace(batch, kv_heads, rows, head_dim) : few_rows_workspace(batch, kv_heads, rows, head_dim);
   return n ? n : 256;
 }
 

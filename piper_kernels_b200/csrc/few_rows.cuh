@@ -30,7 +30,6 @@
 namespace pk {
 namespace {
 
-constexpr int kTile = 64;  // keys per stage
 constexpr int kStages = 3;
 constexpr int kConsumers = 128;
 constexpr int kThreads = kConsumers + 32;
@@ -44,12 +43,13 @@ struct Few {
   static constexpr int ROWS = 16 * WM;
   static constexpr int ESZ = I8 ? 1 : 2;
   static constexpr int ROW_BYTES = D * ESZ;
+  static constexpr int TILE = ROW_BYTES > 128 ? 64 : 128;  // keys per stage: 16 to 32 KB of K and V
   static constexpr int LINE = ROW_BYTES > 128 ? 128 : ROW_BYTES;  // swizzled line
   static constexpr int HALVES = ROW_BYTES / LINE;
-  static constexpr int KV_BYTES = kTile * ROW_BYTES;
-  static constexpr int SCALE_BYTES = I8 ? 2 * kTile * 4 : 0;
+  static constexpr int KV_BYTES = TILE * ROW_BYTES;
+  static constexpr int SCALE_BYTES = I8 ? 2 * TILE * 4 : 0;
   static constexpr int STAGE = 2 * KV_BYTES;
-  static constexpr int KEYS = kTile / WN;  // keys of a tile per warp
+  static constexpr int KEYS = TILE / WN;  // keys of a tile per warp
   // In a 16-byte shared-memory access eight threads (two key columns x four pieces) are served at
   // once.  128-byte lines: neighbouring columns are mapped to keys four apart, whose pieces the
   // swizzle puts into the other half of the banks.  64-byte lines: neighbours are two halves of 128 bytes.
@@ -66,12 +66,12 @@ struct Few {
 };
 
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1, __half) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1, __nv_bfloat16) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -91,15 +91,14 @@ __device__ __forceinline__ uint32_t two_bytes(uint32_t w, bool high, __nv_bfloat
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
+// Plain loads (not inline assembly), so that the compiler may move them within what the waits allow.
+__device__ __forceinline__ uint4 lds128(const uint8_t* smem, uint32_t at) { return *reinterpret_cast<const uint4*>(smem + at); }
+__device__ __forceinline__ uint2 lds64(const uint8_t* smem, uint32_t at) { return *reinterpret_cast<const uint2*>(smem + at); }
+
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 template <typename T, bool I8, int D, int WM, bool TREE>
@@ -108,7 +107,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   using C = Few<T, I8, D, WM>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
-  int64_t* red = reinterpret_cast<int64_t*>(smem + C::OFF_RED);
+  uint32_t* red = reinterpret_cast<uint32_t*>(smem + C::OFF_RED);
   Found* found = reinterpret_cast<Found*>(smem + C::OFF_RED + 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC);
   volatile uint32_t* there = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_THERE);
@@ -125,20 +124,20 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   __syncthreads();
 
   const int groups = p.batch * p.row_blocks;
-  const int64_t total = sum_tiles<TREE, kTile, C::ROWS>(p, groups, red);
-  const int64_t w0 = share_begin(total, gridDim.x, blockIdx.x), w1 = share_begin(total, gridDim.x, blockIdx.x + 1);
+  const uint32_t total = sum_tiles<TREE, C::TILE, C::ROWS>(p, 0, groups, red);
+  const uint32_t w0 = share_begin(total, gridDim.x, blockIdx.x), w1 = share_begin(total, gridDim.x, blockIdx.x + 1);
   if (w0 >= w1) return;
-  const Found f = find_group<TREE, kTile, C::ROWS>(p, w0, red, found);
-  Walk<TREE, kTile, C::ROWS> walk;
+  const Found f = find_group<TREE, C::TILE, C::ROWS>(p, 0, w0, red, found);
+  Walk<TREE, C::TILE, C::ROWS> walk;
   walk.start(p, f, w0);
 
   if (warp == kConsumers / 32) {
     // ---------------------------------------------------------------- producer
     if (lane == 0) {
-      const int box = p.table ? min(p.page, kTile) : kTile;
+      const int box = p.table ? min(p.page, C::TILE) : C::TILE;
       int last = -1;
       bool ok = true;
-      for (int64_t w = w0; w < w1; ++w, walk.next(p)) {
+      for (uint32_t w = w0; w < w1; ++w, walk.next(p)) {
         const int i = static_cast<int>(w - w0), st = i % kStages;
         if (i >= kStages && !mbar_wait_bounded(bars + 8 * (kStages + st), ((i / kStages) - 1) & 1, abort_flag, 61)) { ok = false; break; }
         const uint32_t full = bars + 8 * st, dst = base + st * C::STAGE;
@@ -150,21 +149,21 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           tma_load_5d(dst, &tm_k, full, 0, j0, 0, p.k_stride[1] ? walk.h : 0, p.k_stride[0] ? walk.s.b : 0);
           tma_load_5d(dst + C::KV_BYTES, &tm_v, full, 0, j0, 0, p.v_stride[1] ? walk.h : 0, p.v_stride[0] ? walk.s.b : 0);
         } else {
-          int pages[kTile / 16];
+          int pages[C::TILE / 16];
           uint32_t mask = 0;
 #pragma unroll
-          for (int x = 0; x < kTile / 16; ++x) {
+          for (int x = 0; x < C::TILE / 16; ++x) {
             const int j = j0 + x * box;
             // a page that is not there, or lies behind the sequence, reads as zeros (outside the map)
-            pages[x] = (x * box < kTile && j < walk.s.len) ? attend_page(p, walk.s.b, j) : -1;
+            pages[x] = (x * box < C::TILE && j < walk.s.len) ? attend_page(p, walk.s.b, j) : -1;
             if (pages[x] >= 0) mask |= 1u << x;
             if (I8 && pages[x] >= 0) ++scale_boxes;
           }
           there[st] = mask;
           mbar_expect_tx(full, C::STAGE + scale_boxes * 2 * box * 4);
 #pragma unroll
-          for (int x = 0; x < kTile / 16; ++x) {
-            if (x * box >= kTile) break;
+          for (int x = 0; x < C::TILE / 16; ++x) {
+            if (x * box >= C::TILE) break;
             const int row = (j0 + x * box) & (p.page - 1);
             const int c4 = pages[x] >= 0 ? p.page_base + pages[x] : 0x7fffffff;
             tma_load_5d(dst + x * box * C::ROW_BYTES, &tm_k, full, 0, row, 0, walk.h, c4);
@@ -173,7 +172,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
               const int64_t at = (static_cast<int64_t>(pages[x]) * p.kv_heads + walk.h) * p.page + row;
               const uint32_t sdst = base + C::OFF_SCALE + st * C::SCALE_BYTES + x * box * 4;
               bulk_load(sdst, p.k_scale + at, box * 4, full);
-              bulk_load(sdst + kTile * 4, p.v_scale + at, box * 4, full);
+              bulk_load(sdst + C::TILE * 4, p.v_scale + at, box * 4, full);
             }
           }
         }
@@ -200,7 +199,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   int tree_b = -1;
   bool ok = true;
 
-  int64_t w = w0;
+  uint32_t w = w0;
   for (int i = 0; ok && w < w1;) {
     // -------- a new unit: rows [rb * ROWS, ...) of key head h of batch element b
     const Span s = walk.s;
@@ -249,47 +248,59 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 #pragma unroll
     for (int t = 0; t < OT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
 
-    const int unit_tiles = static_cast<int>(min(static_cast<int64_t>(s.n - walk.tile), w1 - w));
-    const int box = p.table ? min(p.page, kTile) : kTile;
+    const int unit_tiles = static_cast<int>(min(static_cast<uint32_t>(s.n - walk.tile), w1 - w));
+    const int box = p.table ? min(p.page, C::TILE) : C::TILE;
     for (int u = 0; u < unit_tiles; ++u, ++i, ++w) {
       const int st = i % kStages;
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * st, (i / kStages) & 1, abort_flag, 62));
       if (!ok) break;
-      const int j0 = key_of_tile<kTile>(s, unit_from + u);
+      const int j0 = key_of_tile<C::TILE>(s, unit_from + u);
       // Keys on pages that are not there are masked like those that no row may see.
-      const uint32_t held = there[st], all = (1u << (kTile / box)) - 1;
-      const bool full = held == all && ((j0 >= s.full_lo && j0 + kTile <= s.full_hi) || (j0 + kTile <= min(p.sinks, s.full_hi)));
-      const uint32_t kst = base + st * C::STAGE, vst = kst + C::KV_BYTES;
+      const uint32_t held = there[st], all = (1u << (C::TILE / box)) - 1;
+      const bool full = held == all && ((j0 >= s.full_lo && j0 + C::TILE <= s.full_hi) || (j0 + C::TILE <= min(p.sinks, s.full_hi)));
+      const uint32_t kst = st * C::STAGE, vst = kst + C::KV_BYTES;  // offsets in shared memory
       const float* sc = reinterpret_cast<const float*>(smem + C::OFF_SCALE + st * C::SCALE_BYTES);
-#pragma unroll 1
+#pragma unroll(I8 ? 2 : 1)
       for (int step = 0; step < C::KEYS / 16; ++step) {
         const int k0 = wn * C::KEYS + step * 16;  // within the tile
         if (j0 + k0 >= s.len && !full) continue;  // behind the sequence (the same for the whole warp)
         const uint32_t off0 = C::HALVES == 2 ? (k0 / box) * (box * C::ROW_BYTES) + (k0 % box) * 128 : k0 * C::LINE;
         const uint32_t half = box * 128;
-        // ---- scores of 16 keys
-        float sv[2][4];
+        // ---- scores of 16 keys: two 8-key columns of the fragment, each in two sums (a product that
+        // accumulates waits for its predecessor; four chains are interleaved)
+        float sv[2][4], sw[2][4];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          sv[nt][0] = sv[nt][1] = sv[nt][2] = sv[nt][3] = 0.f;
-          const int kk = nt * 8 + key_of(g8);
-          const uint32_t row = kst + off0 + kk * C::LINE;
-          const int sw = C::LINE == 128 ? (kk & 7) : ((kk >> 1) & 3);
+        for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-          for (int j = 0; j < C::ROW_BYTES / 64; ++j) {
-            const int chunk = j * 4 + c4;
-            const uint32_t a = row + (C::HALVES == 2 ? (chunk >> 3) * half : 0) + (((chunk & (C::LINE / 16 - 1)) ^ sw) << 4);
-            const uint4 v = lds128(a);
-            if (I8) {
-              const uint32_t wv[4] = {v.x, v.y, v.z, v.w};
+          for (int y = 0; y < 4; ++y) sv[nt][y] = sw[nt][y] = 0.f;
 #pragma unroll
-              for (int y = 0; y < 4; ++y) mma16816(sv[nt], qf[j * 4 + y], two_bytes(wv[y], false, T{}), two_bytes(wv[y], true, T{}), T{});
-            } else {
-              mma16816(sv[nt], qf[j * 2], v.x, v.y, T{});
-              mma16816(sv[nt], qf[j * 2 + 1], v.z, v.w, T{});
-            }
+        for (int j = 0; j < C::ROW_BYTES / 64; ++j) {
+          uint4 v[2];
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            const int kk = nt * 8 + key_of(g8), chunk = j * 4 + c4;
+            const int sw_ = C::LINE == 128 ? (kk & 7) : ((kk >> 1) & 3);
+            v[nt] = lds128(smem, kst + off0 + kk * C::LINE + (C::HALVES == 2 ? (chunk >> 3) * half : 0) + (((chunk & (C::LINE / 16 - 1)) ^ sw_) << 4));
+          }
+          if (I8) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+              for (int nt = 0; nt < 2; ++nt) {
+                const uint32_t w8 = y == 0 ? v[nt].x : y == 1 ? v[nt].y : y == 2 ? v[nt].z : v[nt].w;
+                mma16816(y & 1 ? sw[nt] : sv[nt], qf[j * 4 + y], two_bytes(w8, false, T{}), two_bytes(w8, true, T{}), T{});
+              }
+          } else {
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) mma16816(sv[nt], qf[j * 2], v[nt].x, v[nt].y, T{});
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) mma16816(sw[nt], qf[j * 2 + 1], v[nt].z, v[nt].w, T{});
           }
         }
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) sv[nt][y] += sw[nt][y];
         // ---- to base-2 exponents; column n of the fragment is key key_of(n)
         float inv[4];
 #pragma unroll
@@ -298,11 +309,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           float mul = p.scale_log2, add = 0.f;
           if (I8) {
             // A scale of zero makes a zero row, whose weight still counts: taken as 2^-60.
-            float vs = sc[kTile + k0 + kk];
+            float vs = sc[C::TILE + k0 + kk];
             vs = vs < 0x1p-60f ? 0x1p-60f : vs;
             mul *= sc[k0 + kk];
             add = __log2f(vs);
-            inv[y] = __frcp_rn(vs);
+            inv[y] = rcp_approx(vs);
           }
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
@@ -367,10 +378,10 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           for (int y = 0; y < 4; ++y) {
             const uint32_t row = vst + off0 + kk[y] * C::LINE;
             if (D == 128) {
-              const uint4 v = lds128(row + ((key_of(g8) ^ (kk[y] & 7)) << 4));
+              const uint4 v = lds128(smem, row + ((key_of(g8) ^ (kk[y] & 7)) << 4));
               vw[y][0] = v.x, vw[y][1] = v.y, vw[y][2] = v.z, vw[y][3] = v.w;
             } else {
-              const uint2 v = lds64(row + (((g8 >> 1) ^ ((kk[y] >> 1) & 3)) << 4) + (g8 & 1) * 8);
+              const uint2 v = lds64(smem, row + (((g8 >> 1) ^ ((kk[y] >> 1) & 3)) << 4) + (g8 & 1) * 8);
               vw[y][0] = v.x, vw[y][1] = v.y, vw[y][2] = vw[y][3] = 0;
             }
           }
@@ -390,7 +401,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             uint32_t vw[4][4];
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              const uint4 v = lds128(vst + off0 + hf * half + kk[y] * 128 + ((key_of(g8) ^ (kk[y] & 7)) << 4));
+              const uint4 v = lds128(smem, vst + off0 + hf * half + kk[y] * 128 + ((key_of(g8) ^ (kk[y] & 7)) << 4));
               vw[y][0] = v.x, vw[y][1] = v.y, vw[y][2] = v.z, vw[y][3] = v.w;
               if (ragged && j0 + k0 + kk[y] >= s.len) vw[y][0] = vw[y][1] = vw[y][2] = vw[y][3] = 0;
             }
@@ -408,6 +419,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 
     // -------- join the warps that shared the unit's keys; write rows, or a piece for the join kernel
     const bool whole = unit_from == 0 && unit_tiles == s.n;
+    if (unit_from == 0 && tid == 0) {
+      const uint32_t u0 = w - unit_tiles;  // (after an abandoned wait the pieces do not matter)
+      const int last = whole ? static_cast<int>(blockIdx.x) : static_cast<int>(owner_of(total, gridDim.x, u0 + s.n - 1));
+      p.pieces[walk.g * p.kv_heads + h] = Pieces{static_cast<int>(blockIdx.x), last, u0 != w0, 0};
+    }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
@@ -417,7 +433,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     }
     ok = vote_barrier(1, kConsumers, ok && *abort_flag == 0);  // the same answer in every warp: they leave together
     const int slot = blockIdx.x * 2 + (unit_from == 0 && w - unit_tiles != w0 ? 1 : 0);
-    float* piece = p.partial + static_cast<int64_t>(slot) * C::ROWS * (D + 2);
+    float* piece = p.partial + static_cast<int64_t>(slot) * C::ROWS * (D + 4);
     // thread -> (row, four consecutive columns) of the CTA's rows; a row's columns belong to 8 neighbouring threads
     bool bad[WM];
 #pragma unroll
@@ -458,9 +474,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         }
         if (row < p.rows) {
           if (!whole) {
-            float* dst = piece + (it * 16 + r16) * (D + 2);
-            *reinterpret_cast<float2*>(dst + pass * kJoinCols + col) = make_float2(acc[0], acc[1]);
-            *reinterpret_cast<float2*>(dst + pass * kJoinCols + col + 2) = make_float2(acc[2], acc[3]);
+            float* dst = piece + (it * 16 + r16) * (D + 4);
+            *reinterpret_cast<float4*>(dst + pass * kJoinCols + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
             if (pass == 0 && (tid & 7) == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mx, sum);
           } else {
             const int t = token_of(p, row), idx = s.off + t;
@@ -506,19 +521,24 @@ int launch(AttendParams p, int device, cudaStream_t st) {
   using C = Few<T, I8, D, WM>;
   static_assert(C::SMEM <= 113 * 1024, "two CTAs share an SM");
   p.row_blocks = (p.rows + C::ROWS - 1) / C::ROWS;
-  p.key_align = p.table ? (p.page < kTile ? p.page : kTile) : 8;
+  p.key_align = p.table ? (p.page < C::TILE ? p.page : C::TILE) : 8;
   CUtensorMap tk, tv;
   int rc;
-  if ((rc = attend_map(&tk, p, p.k, p.k_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < kTile ? p.page : kTile) : kTile, C::HALVES))) return rc;
-  if ((rc = attend_map(&tv, p, p.v, p.v_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < kTile ? p.page : kTile) : kTile, C::HALVES))) return rc;
+  if ((rc = attend_map(&tk, p, p.k, p.k_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < C::TILE ? p.page : C::TILE) : C::TILE, C::HALVES))) return rc;
+  if ((rc = attend_map(&tv, p, p.v, p.v_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < C::TILE ? p.page : C::TILE) : C::TILE, C::HALVES))) return rc;
   if ((rc = allow_smem<few_rows_kernel<T, I8, D, WM, TREE>>(C::SMEM, device))) return rc;
   // No more CTAs than there can be tiles.
-  const int64_t most = static_cast<int64_t>(p.batch) * p.row_blocks * p.kv_heads * (((p.table ? p.width * p.page : p.kv_len) + kTile - 1) / kTile + 2);
+  const int64_t units = static_cast<int64_t>(p.batch) * p.row_blocks * p.kv_heads;
+  const int64_t most = units * (((p.table ? p.width * p.page : p.kv_len) + C::TILE - 1) / C::TILE + 2);
+  if (most >= (1ll << 31)) return fail(PK_ERR_BAD_ARG, "attention: too many keys and rows for one call; split it over the batch");
   p.workers = static_cast<int>(most < kMaxWorkers ? most : kMaxWorkers);
+  p.first_unit = 0;
+  p.pieces = reinterpret_cast<Pieces*>(p.partial);
+  p.partial += (units * (sizeof(Pieces) / sizeof(float)) + 63) / 64 * 64;
   cudaError_t e = launch_chained(few_rows_kernel<T, I8, D, WM, TREE>, dim3(p.workers), dim3(kThreads), C::SMEM, st, tk, tv, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "attention kernel launch failed: %s", cuda_err(e));
-  e = launch_chained(join_kernel<T, I8, D, TREE, kTile, C::ROWS>, dim3(p.batch * p.row_blocks * p.kv_heads * (C::ROWS / kJoinRows)), dim3(kCounters), 0, st, p, p.workers);
+  e = launch_chained(join_kernel<T, I8, D, TREE, C::TILE, C::ROWS>, dim3(static_cast<unsigned>(units) * (C::ROWS / kJoinRows)), dim3(32 * kJoinRows), 0, st, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "join kernel launch failed: %s", cuda_err(e));
   return PK_OK;

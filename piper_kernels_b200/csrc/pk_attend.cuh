@@ -47,8 +47,11 @@ struct AttendParams {
   int window, sinks;
   int key_align;     // tiles begin on multiples of this: 8, or what keeps a tile's copies within pages
   float scale_log2;  // softmax scale * log2(e)
-  float* partial;    // pieces of rows whose keys are shared by several CTAs
-  int workers;
+  // Units (group, key head) from first_unit on are shared out by tiles over `workers` CTAs (0: none is);
+  // pieces of their rows: [2 * workers][rows of a unit][D + 4] (numerators, maximum, sum, -, -).
+  float* partial;
+  struct Pieces* pieces;  // per unit
+  int workers, first_unit;
   int32_t* host_status;  // pinned word that takes the site of an abandoned wait
 };
 
@@ -296,60 +299,59 @@ __device__ __forceinline__ int key_of_tile(const Span& s, int i) {
   return i < s.ns ? i * TILE : s.begin + (i - s.ns) * TILE;
 }
 
-// First tile of worker w, when `total` tiles are shared out.
-__device__ __forceinline__ int64_t share_begin(int64_t total, int workers, int w) {
-  return total / workers * w + min(static_cast<int64_t>(w), total % workers);
+// First tile of worker w, when `total` tiles are shared out (fewer than 2^31: checked on the host).
+__device__ __forceinline__ uint32_t share_begin(uint32_t total, uint32_t workers, uint32_t w) {
+  return total / workers * w + min(w, total % workers);
 }
-__device__ __forceinline__ int owner_of(int64_t total, int workers, int64_t tile) {
-  const int64_t base = total / workers, extra = total % workers, big = extra * (base + 1);
-  return static_cast<int>(tile < big ? tile / (base + 1) : extra + (tile - big) / base);
+__device__ __forceinline__ uint32_t owner_of(uint32_t total, uint32_t workers, uint32_t tile) {
+  const uint32_t base = total / workers, extra = total % workers, big = extra * (base + 1);
+  return tile < big ? tile / (base + 1) : extra + (tile - big) / base;
 }
 
 constexpr int kCounters = 128;  // threads that count tiles
 
 struct Found {  // a group and the tiles in front of it
-  int64_t before;
+  uint32_t before;
   int group;
 };
 
-// Tiles of the groups in front of `upto`, all key heads; by the whole CTA, threads [0, 128) count.
+// Tiles of the groups [from, upto), all key heads; by the whole CTA, threads [0, 128) count.
 template <bool TREE, int TILE, int ROWS>
-__device__ __forceinline__ int64_t sum_tiles(const AttendParams& p, int upto, int64_t* red) {
-  int64_t mine = 0;
+__device__ __forceinline__ uint32_t sum_tiles(const AttendParams& p, int from, int upto, uint32_t* red) {
+  uint32_t mine = 0;
   if (threadIdx.x < kCounters)
-    for (int g = threadIdx.x; g < upto; g += kCounters) mine += span_of<TREE, TILE, ROWS>(p, g).n;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    for (int g = from + threadIdx.x; g < upto; g += kCounters) mine += span_of<TREE, TILE, ROWS>(p, g).n;
+  mine = __reduce_add_sync(0xffffffffu, mine);
   if ((threadIdx.x & 31) == 0 && threadIdx.x < kCounters) red[threadIdx.x >> 5] = mine;
   __syncthreads();
-  const int64_t sum = red[0] + red[1] + red[2] + red[3];
+  const uint32_t sum = red[0] + red[1] + red[2] + red[3];
   __syncthreads();
   return sum * p.kv_heads;
 }
 
-// Finds the group that holds tile `at` (0 <= at < total), 128 groups at a time.
+// Finds the group that holds tile `at` of those from group `from` on, 128 groups at a time.
 template <bool TREE, int TILE, int ROWS>
-__device__ __forceinline__ Found find_group(const AttendParams& p, int64_t at, int64_t* red, Found* out) {
+__device__ __forceinline__ Found find_group(const AttendParams& p, int from, uint32_t at, uint32_t* red, Found* out) {
   const int groups = p.batch * p.row_blocks, lane = threadIdx.x & 31;
-  int64_t before = 0;
+  uint32_t before = 0;
   if (threadIdx.x == 0) out->group = -1;
   __syncthreads();
-  for (int g0 = 0; g0 < groups; g0 += kCounters) {
+  for (int g0 = from; g0 < groups; g0 += kCounters) {
     const int g = g0 + threadIdx.x;
-    int64_t n = 0;
-    if (threadIdx.x < kCounters && g < groups) n = static_cast<int64_t>(span_of<TREE, TILE, ROWS>(p, g).n) * p.kv_heads;
-    int64_t incl = n;
+    uint32_t n = 0;
+    if (threadIdx.x < kCounters && g < groups) n = span_of<TREE, TILE, ROWS>(p, g).n * p.kv_heads;
+    uint32_t incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += up;
     }
     if (lane == 31 && threadIdx.x < kCounters) red[threadIdx.x >> 5] = incl;
     __syncthreads();
     if (threadIdx.x < kCounters) {
-      int64_t base = before;
+      uint32_t base = before;
       for (int w = 0; w < (threadIdx.x >> 5); ++w) base += red[w];
-      const int64_t b0 = base + incl - n;
+      const uint32_t b0 = base + incl - n;
       if (n > 0 && at >= b0 && at < b0 + n) out->group = g, out->before = b0;
     }
     before += red[0] + red[1] + red[2] + red[3];
@@ -359,14 +361,21 @@ __device__ __forceinline__ Found find_group(const AttendParams& p, int64_t at, i
   return *out;
 }
 
+// Where the pieces of a unit (group, key head) are, written by the CTA that has its first tile: CTAs
+// c0 .. c1, each in slot 0 of its two, but for c0 when `late` (it began with another unit).  c0 == c1:
+// one CTA finished the unit.
+struct Pieces {
+  int c0, c1, late, pad;
+};
+
 template <bool TREE, int TILE, int ROWS>
 struct Walk {  // position in the list of tiles
   Span s;
   int g, h, tile;
-  __device__ __forceinline__ void start(const AttendParams& p, const Found& f, int64_t at) {
+  __device__ __forceinline__ void start(const AttendParams& p, const Found& f, uint32_t at) {
     g = f.group;
     s = span_of<TREE, TILE, ROWS>(p, g);
-    const int64_t rel = at - f.before;
+    const uint32_t rel = at - f.before;
     h = static_cast<int>(rel / s.n);
     tile = static_cast<int>(rel % s.n);
   }
@@ -380,67 +389,67 @@ struct Walk {  // position in the list of tiles
   __device__ __forceinline__ int key() const { return key_of_tile<TILE>(s, tile); }
 };
 
-// Joins the pieces of every unit that more than one CTA worked on.  kJoinRows rows of a unit (batch
-// element, row block, key head) per CTA, one or two per warp: a row's pieces are a chain of loads, and
-// rows are what there is to run side by side.  Units that one CTA finished are left alone.
-constexpr int kJoinRows = 8;
+// Joins the pieces of every unit that more than one CTA worked on: a warp per row, its pieces' weights
+// first (a lane per piece), then their numerators, several loads in flight.
+constexpr int kJoinRows = 4;
 
 template <typename T, bool I8, int D, bool TREE, int TILE, int ROWS>
-__global__ void __launch_bounds__(kCounters) join_kernel(const __grid_constant__ AttendParams p, int workers) {
-  __shared__ int64_t red[4];
+__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ AttendParams p) {
   __shared__ TreeMasks tm;
-  const int unit = blockIdx.x / (ROWS / kJoinRows), g = unit / p.kv_heads, h = unit % p.kv_heads, groups = p.batch * p.row_blocks;
-  const int r0 = blockIdx.x % (ROWS / kJoinRows) * kJoinRows;
-  if (g % p.row_blocks * ROWS + r0 >= p.rows) return;
+  constexpr int E = D / 32, BLOCKS = ROWS / kJoinRows;
+  const int unit = p.first_unit + blockIdx.x / BLOCKS, g = unit / p.kv_heads, h = unit - g * p.kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x % BLOCKS * kJoinRows + warp;
+  const int row = g % p.row_blocks * ROWS + r;
   cudaGridDependencySynchronize();
-  const int64_t total = sum_tiles<TREE, TILE, ROWS>(p, groups, red);
-  int64_t u0 = sum_tiles<TREE, TILE, ROWS>(p, g, red);
-  const Span s = span_of<TREE, TILE, ROWS>(p, g);
-  u0 += static_cast<int64_t>(h) * s.n;
-  const int c0 = owner_of(total, workers, u0), c1 = owner_of(total, workers, u0 + s.n - 1);
-  if (c0 == c1) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (TREE) {
-    if (warp == 0) build_tree(p, s.b, s.off, lane, &tm);
-    __syncthreads();
-  }
-  const bool first_second = u0 > share_begin(total, workers, c0);  // its first CTA began with another unit
-  constexpr int E = D / 32;
-  const int r1 = min(p.rows - s.rb * ROWS, r0 + kJoinRows);
-  for (int r = r0 + warp; r < r1; r += kCounters / 32) {
-    float mx = -INFINITY, sum = 0.f, acc[E];
+  const Pieces at = p.pieces[unit];
+  if (at.c0 == at.c1 || row >= p.rows) return;  // the same for the warp; no barrier follows
+  if (at.c0 < 0 || at.c1 < at.c0 || at.c1 >= p.workers) return;  // never written: a wait was abandoned
+  // (a piece's slot) * ROWS + r, in rows of D + 4 words
+  auto slot = [&](int c) { return (static_cast<int64_t>(2 * c + (c == at.c0 ? at.late : 0)) * ROWS + r) * (D + 4); };
+  float mx = -INFINITY, sum = 0.f, acc[E];
+  for (int c = at.c0 + lane; c <= at.c1; c += 32) mx = fmaxf(mx, p.partial[slot(c) + D]);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int c = c0 + lane; c <= c1; c += 32)
-      mx = fmaxf(mx, p.partial[(static_cast<int64_t>(c * 2 + (c == c0 && first_second)) * ROWS + r) * (D + 2) + D]);
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
 #pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int c0 = at.c0; c0 <= at.c1; c0 += 32) {
+    float w = 0.f;
+    if (c0 + lane <= at.c1) {
+      const float2 st = *reinterpret_cast<const float2*>(p.partial + slot(c0 + lane) + D);
+      w = st.x == mx ? 1.f : ex2_approx(st.x - mx);
+      sum = fmaf(st.y, w, sum);
+    }
+    const int n = min(32, at.c1 - c0 + 1);
 #pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const float* src = p.partial + (static_cast<int64_t>(c * 2 + (c == c0 && first_second)) * ROWS + r) * (D + 2);
-      const float2 st = *reinterpret_cast<const float2*>(src + D);
-      const float wgt = st.x == mx ? 1.f : ex2_approx(st.x - mx);
-      sum = fmaf(st.y, wgt, sum);
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(src + lane * E + e);
-        acc[e] = fmaf(v.x, wgt, acc[e]);
-        acc[e + 1] = fmaf(v.y, wgt, acc[e + 1]);
+    for (int c = 0; c < n; ++c) {
+      const float wgt = __shfl_sync(0xffffffffu, w, c);
+      const float* src = p.partial + slot(c0 + c) + lane * E;
+      if (E == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src);
+        acc[0] = fmaf(v.x, wgt, acc[0]), acc[1] = fmaf(v.y, wgt, acc[1]), acc[E - 2] = fmaf(v.z, wgt, acc[E - 2]), acc[E - 1] = fmaf(v.w, wgt, acc[E - 1]);
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        acc[0] = fmaf(v.x, wgt, acc[0]), acc[1] = fmaf(v.y, wgt, acc[1]);
       }
     }
-    const int row = s.rb * ROWS + r, t = token_of(p, row), idx = s.off + t;
-    const float inv = idx >= 0 && idx < s.len && sum != 0.f ? 1.f / sum : 0.f;
-    T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + row - t * p.group) * p.tokens + t) * D + lane * E;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float a = inv == 0.f ? 0.f : acc[e] * inv, b = inv == 0.f ? 0.f : acc[e + 1] * inv;
-      bad |= !(fabsf(a) <= 3.0e38f) || !(fabsf(b) <= 3.0e38f);
-      *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(a, b);
-    }
-    __syncwarp();
-    if (__any_sync(0xffffffffu, bad)) plain_row<T, I8, D>(p, s.b, h, row, s.off, s.len, row_view(p, s.off, s.len, t, TREE ? &tm : nullptr), TREE);
   }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const int b = g / p.row_blocks, len = attend_len(p, b), off = attend_off(p, b, len);
+  const int t = token_of(p, row), idx = off + t;
+  const float inv = idx >= 0 && idx < len && sum != 0.f ? 1.f / sum : 0.f;
+  T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.heads + h * p.group + row - t * p.group) * p.tokens + t) * D + lane * E;
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    const float x = inv == 0.f ? 0.f : acc[e] * inv, y = inv == 0.f ? 0.f : acc[e + 1] * inv;
+    bad |= !(fabsf(x) <= 3.0e38f) || !(fabsf(y) <= 3.0e38f);
+    *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(x, y);
+  }
+  __syncwarp();
+  if (!__any_sync(0xffffffffu, bad)) return;
+  if (TREE) build_tree(p, b, off, lane, &tm);  // warps of one CTA write the same values
+  plain_row<T, I8, D>(p, b, h, row, off, len, row_view(p, off, len, t, TREE ? &tm : nullptr), TREE);
 }
 
 // Copy map of K or V: [line, key, lines of a row, head, batch element or page], boxes of `box` keys and
@@ -451,7 +460,7 @@ int attend_map(CUtensorMap* m, const AttendParams& p, const void* base, const in
 // few_rows.cuh
 int launch_few_rows_f16(const AttendParams& p, int head_dim, bool i8, int device, cudaStream_t st);
 int launch_few_rows_bf16(const AttendParams& p, int head_dim, bool i8, int device, cudaStream_t st);
-uint64_t few_rows_workspace(int rows, int head_dim);
+uint64_t few_rows_workspace(int batch, int kv_heads, int rows, int head_dim);
 // wide_rows.cuh
 int launch_wide_rows_f16(const AttendParams& p, int head_dim, int device, cudaStream_t st);
 int launch_wide_rows_bf16(const AttendParams& p, int head_dim, int device, cudaStream_t st);

@@ -133,33 +133,38 @@ __device__ __forceinline__ bool wide_wait(uint32_t bar, uint32_t parity, volatil
   return true;
 }
 
-// What one CTA does next: tiles [tile, tile + count) of one unit.  Every role walks the same list: an
-// equal, contiguous share of all tiles, or (when there are many units) every gridDim.x-th unit from the
-// back, where causal rows see the most keys.
+// What one CTA does next.  Every role walks the same list: first every gridDim.x-th of the whole units
+// [0, first_unit), from the back (causal rows see the most keys there), then an equal, contiguous share
+// of the tiles of the units from first_unit on.
 template <bool TREE>
 struct Segments {
   Walk<TREE, kWideTile, kWideRows> walk;
-  int64_t left;  // shares: tiles; else units
-  int unit;
+  int unit, units;           // next whole unit and how many there are
+  uint32_t at, end;          // share of tiles
+  Found found;               // group of the share's first tile
+  __device__ __forceinline__ bool more() const { return unit < units || at < end; }
+  __device__ __forceinline__ bool whole() const { return unit < units; }
+  __device__ __forceinline__ int count() const { return whole() ? walk.s.n : static_cast<int>(min(static_cast<uint32_t>(walk.s.n - walk.tile), end - at)); }
   __device__ __forceinline__ void take(const AttendParams& p) {
-    const int at = p.batch * p.row_blocks * p.kv_heads - 1 - unit;
-    walk.g = at / p.kv_heads;
-    walk.h = at - walk.g * p.kv_heads;
-    walk.tile = 0;
-    walk.s = span_of<TREE, kWideTile, kWideRows>(p, walk.g);
-  }
-  __device__ __forceinline__ int count(const AttendParams& p) const {
-    return p.workers ? static_cast<int>(min(static_cast<int64_t>(walk.s.n - walk.tile), left)) : walk.s.n;
+    if (whole()) {
+      const int u = units - 1 - unit;
+      walk.g = u / p.kv_heads;
+      walk.h = u - walk.g * p.kv_heads;
+      walk.tile = 0;
+      walk.s = span_of<TREE, kWideTile, kWideRows>(p, walk.g);
+    } else if (at < end) {
+      walk.start(p, found, at);
+    }
   }
   __device__ __forceinline__ void advance(const AttendParams& p) {
-    if (p.workers) {
-      const int n = count(p);
-      left -= n;
-      walk.tile += n - 1;
-      walk.next(p);
-    } else if (--left > 0) {
+    if (whole()) {
       unit += gridDim.x;
       take(p);
+    } else {
+      const int n = count();
+      at += n;
+      walk.tile += n - 1;
+      walk.next(p);
     }
   }
 };
@@ -209,7 +214,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_MISC + 4);
   volatile uint32_t* there = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_THERE);
-  int64_t* red = reinterpret_cast<int64_t*>(smem + C::OFF_RED);
+  uint32_t* red = reinterpret_cast<uint32_t*>(smem + C::OFF_RED);
   Found* found = reinterpret_cast<Found*>(smem + C::OFF_RED + 32);
   const uint32_t bars = base + C::OFF_BAR;
   auto full = [&](int i) { return bars + 8 * i; };
@@ -238,22 +243,19 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // This CTA's part: an equal share of all tiles, or (when there are many units) one unit.
   Segments<TREE> seg;
+  seg.unit = blockIdx.x;
+  seg.units = p.first_unit;
+  seg.at = seg.end = 0;
+  uint32_t total = 0, share_from = 0;
   if (p.workers) {
-    const int64_t total = sum_tiles<TREE, kWideTile, kWideRows>(p, p.batch * p.row_blocks, red);
-    const int64_t w0 = share_begin(total, gridDim.x, blockIdx.x), w1 = share_begin(total, gridDim.x, blockIdx.x + 1);
-    seg.left = w1 - w0;
-    if (seg.left > 0) {
-      const Found f = find_group<TREE, kWideTile, kWideRows>(p, w0, red, found);
-      seg.walk.start(p, f, w0);
-    }
-  } else {
-    const int units = p.batch * p.row_blocks * p.kv_heads;
-    seg.unit = blockIdx.x;
-    seg.left = (units - 1 - seg.unit) / static_cast<int>(gridDim.x) + 1;  // no more CTAs than units
-    seg.take(p);
+    const int g0 = p.first_unit / p.kv_heads;  // shared units begin with a group
+    total = sum_tiles<TREE, kWideTile, kWideRows>(p, g0, p.batch * p.row_blocks, red);
+    share_from = seg.at = share_begin(total, p.workers, blockIdx.x);
+    seg.end = share_begin(total, p.workers, blockIdx.x + 1);
+    if (seg.at < seg.end) seg.found = find_group<TREE, kWideTile, kWideRows>(p, g0, seg.at, red, found);
   }
+  seg.take(p);
 
   if (warp >= 16) setmaxnreg_dec<kHelperRegs>();
   if (warp == COPY_WARP) {
@@ -263,9 +265,9 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       uint32_t st = 0, ph = 1;
       int n = 0;  // K and V tiles issued
       bool ok = true;
-      for (; ok && seg.left > 0; seg.advance(p)) {
+      for (; ok && seg.more(); seg.advance(p)) {
         const Span& s = seg.walk.s;
-        const int count = seg.count(p), from = seg.walk.tile;
+        const int count = seg.count(), from = seg.walk.tile;
         for (int u = 0; ok && u < count; ++u) {
           const int j0 = key_of_tile<kWideTile>(s, from + u);
           int pages[kWideTile / 16];
@@ -342,9 +344,9 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       if (stage >= ST) stage -= ST, phase ^= 1;
     };
     bool ok = true;
-    for (; ok && seg.left > 0; seg.advance(p), ++nq) {
+    for (; ok && seg.more(); seg.advance(p), ++nq) {
       const Span& s = seg.walk.s;
-      const int count = seg.count(p), from = seg.walk.tile;
+      const int count = seg.count(), from = seg.walk.tile;
       const Reach r0 = reach_of<TREE>(p, s, 0), r1 = reach_of<TREE>(p, s, 1);
       bool more0 = false, more1 = false;
       int w0 = 0, w1 = 0;  // widths of tile u for the two row tiles, 0: not needed
@@ -409,13 +411,12 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     TreeMasks* tm = reinterpret_cast<TreeMasks*>(smem + C::OFF_TREE) + i;
     const int box = p.table ? min(p.page, kWideTile) : kWideTile;
     const uint32_t all = (1u << (kWideTile / box)) - 1;
-    const int64_t share_from = seg.left;
     uint32_t nt = 0, ns = 0, nq = 0;  // key tiles, those that this row tile needed, and segments so far
     int tree_b = -1;
     bool ok = true;
-    for (; ok && seg.left > 0; seg.advance(p)) {
+    for (; ok && seg.more(); seg.advance(p)) {
       const Span& s = seg.walk.s;
-      const int count = seg.count(p), from = seg.walk.tile, h = seg.walk.h;
+      const int count = seg.count(), from = seg.walk.tile, h = seg.walk.h;
       const Reach reach = reach_of<TREE>(p, s, i);
       const int row0 = s.rb * kWideRows + i * 128;
       if (TREE && s.b != tree_b) {
@@ -558,9 +559,11 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       tc_fence_after();
       const int idx = s.off + t;
       const bool valid = r < p.rows && idx >= 0 && idx < s.len;
-      if (p.workers && (from != 0 || count != s.n)) {
-        const int slot = blockIdx.x * 2 + (seg.left != share_from ? 1 : 0);
-        float* dst = p.partial + (static_cast<int64_t>(slot) * kWideRows + i * 128 + row) * (D + 2);
+      if (!seg.whole() && from == 0 && tid == 0)
+        p.pieces[seg.walk.g * p.kv_heads + h] = Pieces{static_cast<int>(blockIdx.x), static_cast<int>(owner_of(total, p.workers, seg.at + s.n - 1)), seg.at != share_from, 0};
+      if (!seg.whole() && (from != 0 || count != s.n)) {
+        const int slot = blockIdx.x * 2 + (seg.at != share_from ? 1 : 0);
+        float* dst = p.partial + (static_cast<int64_t>(slot) * kWideRows + i * 128 + row) * (D + 4);
 #pragma unroll
         for (int c = 0; c < FEATURES; c += 32) {
           uint32_t o[32];
@@ -626,6 +629,18 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (tid == 0 && *abort_flag != 0 && p.host_status != nullptr) atomicCAS_system(p.host_status, 0, *abort_flag);
 }
 
+// Whole rounds of units over the CTAs are worked on unit by unit; what is left over (in groups: all key
+// heads of some rows) is shared out by tiles, or nothing is, when there are so many rounds that the last,
+// partial one hardly counts.
+struct WidePlan {
+  int64_t units, whole;
+};
+inline WidePlan wide_plan(int batch, int kv_heads, int rows) {
+  const int64_t units = static_cast<int64_t>(batch) * kv_heads * ((rows + kWideRows - 1) / kWideRows);
+  if (units >= kWideShareBelow) return {units, units};
+  return {units, units / kWideWorkers * kWideWorkers / kv_heads * kv_heads};
+}
+
 template <typename T, int D, bool TREE>
 int launch_wide(AttendParams p, int device, cudaStream_t st) {
   using C = Wide<D, TREE>;
@@ -638,14 +653,20 @@ int launch_wide(AttendParams p, int device, cudaStream_t st) {
   if ((rc = attend_map(&tk, p, p.k, p.k_stride, 128, D / 64, 2, box, lines))) return rc;
   if ((rc = attend_map(&tv, p, p.v, p.v_stride, 128, D / 64, 2, box, lines))) return rc;
   if ((rc = allow_smem<wide_rows_kernel<T, D, TREE>>(C::SMEM, device))) return rc;
-  const int64_t units = static_cast<int64_t>(p.batch) * p.row_blocks * p.kv_heads;
-  const bool share = units < kWideShareBelow;
-  p.workers = share ? kWideWorkers : 0;
-  cudaError_t e = launch_chained(wide_rows_kernel<T, D, TREE>, dim3(share || units > kWideWorkers ? kWideWorkers : static_cast<unsigned>(units)), dim3(kWideThreads), C::SMEM, st, tk, tv, p);
+  const WidePlan plan = wide_plan(p.batch, p.kv_heads, p.rows);
+  const int64_t most = plan.units * (((p.table ? p.width * p.page : p.kv_len) + kWideTile - 1) / kWideTile + 2);
+  if (most >= (1ll << 31)) return fail(PK_ERR_BAD_ARG, "attention: too many keys and rows for one call; split it over the batch");
+  p.first_unit = static_cast<int>(plan.whole);
+  p.workers = plan.whole < plan.units ? kWideWorkers : 0;
+  p.pieces = reinterpret_cast<Pieces*>(p.partial);
+  p.partial += (plan.units * (sizeof(Pieces) / sizeof(float)) + 63) / 64 * 64;
+  cudaError_t e = launch_chained(wide_rows_kernel<T, D, TREE>, dim3(p.workers || plan.units > kWideWorkers ? kWideWorkers : static_cast<unsigned>(plan.units)),
+                                 dim3(kWideThreads), C::SMEM, st, tk, tv, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "attention kernel launch failed: %s", cuda_err(e));
-  if (!share) return PK_OK;
-  e = launch_chained(join_kernel<T, false, D, TREE, kWideTile, kWideRows>, dim3(static_cast<unsigned>(units) * (kWideRows / kJoinRows)), dim3(kCounters), 0, st, p, p.workers);
+  if (!p.workers) return PK_OK;
+  e = launch_chained(join_kernel<T, false, D, TREE, kWideTile, kWideRows>, dim3(static_cast<unsigned>(plan.units - plan.whole) * (kWideRows / kJoinRows)),
+                     dim3(32 * kJoinRows), 0, st, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "join kernel launch failed: %s", cuda_err(e));
   return PK_OK;

@@ -4,9 +4,9 @@
 namespace pk {
 
 uint64_t wide_rows_workspace(int batch, int kv_heads, int rows, int head_dim) {
-  const int64_t units = static_cast<int64_t>(batch) * kv_heads * ((rows + kWideRows - 1) / kWideRows);
-  if (units >= kWideShareBelow) return 0;
-  return static_cast<uint64_t>(kWideWorkers) * 2 * kWideRows * (head_dim + 2) * sizeof(float);
+  const WidePlan plan = wide_plan(batch, kv_heads, rows);
+  if (plan.whole == plan.units) return 0;
+  return (plan.units * sizeof(Pieces) + 255) / 256 * 256 + static_cast<uint64_t>(kWideWorkers) * 2 * kWideRows * (head_dim + 4) * sizeof(float);
 }
 
 int launch_wide_rows_f16(const AttendParams& p, int head_dim, int device, cudaStream_t st) {
