@@ -11,7 +11,6 @@ operator registry; all arithmetic happens inside ``libpiper_b200.so``.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
 
 import torch
 
@@ -120,31 +119,47 @@ def _(query, key, value, scale, is_causal):
     return torch.empty_like(query, memory_format=torch.contiguous_format)
 
 
-@torch.library.custom_op("piper_b200::window_attention", mutates_args=())
-def window_attention_op(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, lengths: Optional[torch.Tensor],
-                        window: int, sinks: int, scale: float) -> torch.Tensor:
+# Registered with the library's own define / impl: the calls these serve last tens of microseconds, and the
+# wrappers that custom_op puts around a Python kernel cost as much again.
+_LIBRARY = torch.library.Library("piper_b200", "FRAGMENT")
+_LIBRARY.define("window_attention(Tensor query, Tensor key, Tensor value, Tensor? lengths, int window, int sinks, float scale) -> Tensor")
+_WINDOW_WORKSPACE: dict[tuple, int] = {}  # bytes by what the size depends on
+
+
+def _window_attention(query, key, value, lengths, window, sinks, scale):
     _require_cuda(query, "window_attention")
     out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
     device = query.device.index
     poll_device_fault(device)
-    p = _cabi.PkWindowProblem()
-    p.batch, p.heads, p.q_len, p.head_dim = query.shape
-    p.kv_heads, p.kv_len = key.shape[1], key.shape[2]
-    p.dtype, p.window, p.sinks, p.scale = _DTYPE[query.dtype], window, sinks, scale
-    p.q, p.k, p.v, p.out = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr()
-    p.q_stride, p.k_stride, p.v_stride = ((C.c_int64 * 3)(*t.stride()[:3]) for t in (query, key, value))
-    p.lengths = lengths.data_ptr() if lengths is not None else None
-    p.device, p.stream = device, torch.cuda.current_stream(query.device).cuda_stream
-    n = C.c_uint64(0)
     lib = _cabi.lib()
-    _cabi.check(lib.pk_window_workspace_bytes(C.byref(p), C.byref(n)))
+    batch, heads, q_len, head_dim = query.shape
+    _, kv_heads, kv_len, _ = key.shape
+    qs, ks, vs = query.stride()[:3], key.stride()[:3], value.stride()[:3]
+    k, v = key.data_ptr(), value.data_ptr()
+    p = _cabi.PkWindowProblem(batch, heads, kv_heads, q_len, kv_len, head_dim, _DTYPE[query.dtype], window, sinks, scale,
+                              query.data_ptr(), k, v, qs, ks, vs, lengths.data_ptr() if lengths is not None else None, out.data_ptr(),
+                              None, 0, device, torch.cuda.current_stream(query.device).cuda_stream)
+    size = (batch, heads, kv_heads, q_len, kv_len, head_dim, k & 15, v & 15, ks, vs)
+    nbytes = _WINDOW_WORKSPACE.get(size)
+    if nbytes is None:
+        n = C.c_uint64(0)
+        _cabi.check(lib.pk_window_workspace_bytes(C.byref(p), C.byref(n)))
+        if len(_WINDOW_WORKSPACE) >= 4096:
+            _WINDOW_WORKSPACE.clear()
+        nbytes = _WINDOW_WORKSPACE[size] = n.value
     # allocated on the stream that uses it, like the scratch of _run
-    ws = torch.empty(max(1, n.value), dtype=torch.uint8, device=query.device)
-    p.workspace, p.workspace_bytes = ws.data_ptr(), n.value
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
     _cabi.check(lib.pk_window_attention_fwd(C.byref(p)))
     return out
 
 
-@window_attention_op.register_fake
+_LIBRARY.impl("window_attention", _window_attention, "CompositeExplicitAutograd")
+
+
+@torch.library.register_fake("piper_b200::window_attention", lib=_LIBRARY)
 def _(query, key, value, lengths, window, sinks, scale):
     return torch.empty_like(query, memory_format=torch.contiguous_format)
+
+
+window_attention_op = torch.ops.piper_b200.window_attention.default

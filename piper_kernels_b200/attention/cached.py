@@ -78,18 +78,17 @@ def cache_attention(
     _ops._require_cuda(query, "cache_attention")
     _ops.poll_device_fault(query.device.index)
     out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    q = _cabi.PkCacheQuery()
-    q.heads, q.tokens, q.layer, q.dtype = heads, tokens, layer, _ops._DTYPE[query.dtype]
-    q.window, q.sinks, q.scale = 0 if window is None else limit, sinks, converted_scale
-    q.q, q.out = query.data_ptr(), out.data_ptr()
-    q.q_stride = (C.c_int64 * 3)(*query.stride()[:3])
-    if tree is not None:
-        q.tree, q.tree_stride = tree.data_ptr(), tree_stride
+    q = _cabi.PkCacheQuery(heads, tokens, layer, _ops._DTYPE[query.dtype], 0 if window is None else limit, sinks, converted_scale, query.data_ptr(),
+                           query.stride()[:3], None if tree is None else tree.data_ptr(), tree_stride, out.data_ptr(), None, 0)
     c = cache.handle()
-    n = C.c_uint64(0)
     lib = _cabi.lib()
-    _cabi.check(lib.pk_cache_attention_workspace_bytes(C.byref(c), C.byref(q), C.byref(n)))
-    ws = torch.empty(n.value, dtype=torch.uint8, device=query.device)
-    q.workspace, q.workspace_bytes = ws.data_ptr(), n.value
+    nbytes = cache.workspaces.get((heads, tokens))
+    if nbytes is None:
+        n = C.c_uint64(0)
+        _cabi.check(lib.pk_cache_attention_workspace_bytes(C.byref(c), C.byref(q), C.byref(n)))
+        nbytes = cache.workspaces[heads, tokens] = n.value
+    # allocated on the stream that uses it
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+    q.workspace, q.workspace_bytes = ws.data_ptr(), nbytes
     _cabi.check(lib.pk_cache_attention_fwd(C.byref(c), C.byref(q)))
     return out

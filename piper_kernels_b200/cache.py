@@ -23,6 +23,7 @@ _DTYPE = {torch.float16: _cabi.PK_F16, torch.bfloat16: _cabi.PK_BF16, torch.int8
 PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_BATCH = 4096
 _OP = "PageCache"
+_STRIDES = C.c_int64 * 4
 
 
 class PageCache:
@@ -102,6 +103,7 @@ class PageCache:
                 raise ValueError(f"{_OP} tensors must share a device, got {self.device}/{tensor.device} for {name}")
             setattr(self, name, tensor)
         self.refused = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
+        self.workspaces: dict[tuple[int, int], int] = {}  # bytes that cache_attention needs, by (heads, tokens)
         self._scratch = torch.zeros(4 * self.batch + 4, dtype=torch.int32, device=self.device)
         c = self._c = _cabi.PkCache()
         c.layers, c.pages, c.kv_heads, c.page_size, c.head_dim = keys.shape
@@ -168,7 +170,7 @@ class PageCache:
         ks, vs = (t.stride()[:4] if layer is None else (0, *t.stride()[:3]) for t in (key, value))
         at = -1 if layer is None else self.check_layer(layer)
         _cabi.check(_cabi.lib().pk_cache_write(C.byref(self.handle()), at, key.data_ptr(), value.data_ptr(),
-                                               (C.c_int64 * 4)(*ks), (C.c_int64 * 4)(*vs), _DTYPE[key.dtype], key.shape[-2]))
+                                               _STRIDES(*ks), _STRIDES(*vs), _DTYPE[key.dtype], key.shape[-2]))
 
     def read(self, first: torch.Tensor, count: int, *, layer: int | None = None,
              dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:

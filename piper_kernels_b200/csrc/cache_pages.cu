@@ -250,51 +250,63 @@ __device__ __forceinline__ uint2 quantise8(uint4 raw, float* scale) {
   }
   const float s = __fadd_rn(__fdiv_rn(__uint_as_float(top), 127.f), 1e-7f);
   *scale = s;
+  // rint(x / s): |x / s| <= 127, so no clamp, and 1.5 * 2^23 + integer has the code in its low byte.  x times
+  // the rounded reciprocal lies within 2.4e-5 of the quotient and rounds like it, unless it is that near a
+  // half-integer: then (one value in some thousands) the quotient itself is rounded.
+  const float inv = __fdiv_rn(1.f, s), magic = 12582912.f;
   uint32_t code[8];
+  float near = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    // |x / s| <= 127, so no clamp; 1.5 * 2^23 + integer has the code in its low byte
-    code[i] = __float_as_uint(__fadd_rn(__fdiv_rn(x[i], s), 12582912.f)) & 0xffu;
+    const float q = __fmul_rn(x[i], inv), m = __fadd_rn(q, magic);
+    near = fmaxf(near, fabsf(__fsub_rn(q, __fsub_rn(m, magic))));
+    code[i] = __float_as_uint(m) & 0xffu;
+  }
+  if (near > 0.4999f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) code[i] = __float_as_uint(__fadd_rn(__fdiv_rn(x[i], s), magic)) & 0xffu;
   }
   return make_uint2(code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24, code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24);
 }
 
+constexpr int kDeep = 4;  // rows per thread: their loads are issued together
+
+// blockIdx.x: (layer, sequence, head); blockIdx.y: rows [y * ROWS * kDeep, ...).
 template <typename T, bool I8, int D>
 __global__ void __launch_bounds__(256) write_kernel(const Pages c, const Source s) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES;
+  const int sub = threadIdx.x % LANES, head = blockIdx.x % c.kv_heads, rest = blockIdx.x / c.kv_heads, b = rest % c.batch, layer = rest / c.batch;
   cudaGridDependencySynchronize();
-  const int sub = threadIdx.x % LANES;
-  const int64_t chunks = (s.tokens + ROWS - 1) / ROWS, items = chunks * s.layers * c.batch * c.kv_heads;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int t = static_cast<int>(item % chunks) * ROWS + threadIdx.x / LANES;
-    int64_t rest = item / chunks;
-    const int head = static_cast<int>(rest % c.kv_heads);
-    rest /= c.kv_heads;
-    const int b = static_cast<int>(rest % c.batch), layer = static_cast<int>(rest / c.batch);
-    const int start = c.starts[b], len = length_of(c, b);
-    if (static_cast<int>(item % chunks) * ROWS >= len - start || start < 0) continue;  // the same for the whole CTA
-    int page = -1;
-    const bool in = t < s.tokens && t < len - start;
-    const int at = start + t;
-    if (in) page = c.table[static_cast<int64_t>(b) * c.width + (at >> c.shift)];
-    const bool stored = in && is_page(c, page);
-    uint4 k = make_uint4(0, 0, 0, 0), v = k;
-    if (stored) {
-      k = load8(s.key + layer * s.ks[0] + b * s.ks[1] + head * s.ks[2] + t * s.ks[3] + sub * 8, s.vec);
-      v = load8(s.value + layer * s.vs[0] + b * s.vs[1] + head * s.vs[2] + t * s.vs[3] + sub * 8, s.vec);
+  const int start = c.starts[b], added = min(length_of(c, b) - start, s.tokens);
+  const uint16_t* key = s.key + layer * s.ks[0] + b * s.ks[1] + head * s.ks[2] + sub * 8;
+  const uint16_t* value = s.value + layer * s.vs[0] + b * s.vs[1] + head * s.vs[2] + sub * 8;
+  for (int t0 = blockIdx.y * ROWS * kDeep; t0 < added && start >= 0; t0 += gridDim.y * ROWS * kDeep) {
+    int64_t row[kDeep];
+    uint4 k[kDeep], v[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const int t = t0 + i * ROWS + threadIdx.x / LANES, at = start + t;
+      row[i] = -1;
+      k[i] = v[i] = make_uint4(0, 0, 0, 0);
+      if (t >= added) continue;
+      k[i] = load8(key + t * s.ks[3], s.vec);
+      v[i] = load8(value + t * s.vs[3], s.vec);
+      const int page = c.table[static_cast<int64_t>(b) * c.width + (at >> c.shift)];
+      if (is_page(c, page)) row[i] = block_row(c, s.layer0 + layer, page, head) + (at & (c.page - 1));
     }
-    const int64_t row = stored ? block_row(c, s.layer0 + layer, page, head) + (at & (c.page - 1)) : 0;
-    if (I8) {
-      float ks, vs;
-      const uint2 kc = quantise8<T, D>(k, &ks), vc = quantise8<T, D>(v, &vs);
-      if (stored) {
-        *reinterpret_cast<uint2*>(c.keys + row * D + sub * 8) = kc;
-        *reinterpret_cast<uint2*>(c.values + row * D + sub * 8) = vc;
-        if (sub == 0) c.key_scales[row] = ks, c.value_scales[row] = vs;
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      if (I8) {
+        float ks, vs;
+        const uint2 kc = quantise8<T, D>(k[i], &ks), vc = quantise8<T, D>(v[i], &vs);
+        if (row[i] < 0) continue;
+        *reinterpret_cast<uint2*>(c.keys + row[i] * D + sub * 8) = kc;
+        *reinterpret_cast<uint2*>(c.values + row[i] * D + sub * 8) = vc;
+        if (sub == 0) c.key_scales[row[i]] = ks, c.value_scales[row[i]] = vs;
+      } else if (row[i] >= 0) {
+        *reinterpret_cast<uint4*>(c.keys + row[i] * D * 2 + sub * 16) = k[i];
+        *reinterpret_cast<uint4*>(c.values + row[i] * D * 2 + sub * 16) = v[i];
       }
-    } else if (stored) {
-      *reinterpret_cast<uint4*>(c.keys + row * D * 2 + sub * 16) = k;
-      *reinterpret_cast<uint4*>(c.values + row * D * 2 + sub * 16) = v;
     }
   }
 }
@@ -338,31 +350,34 @@ __device__ __forceinline__ void store8(void* out, int dtype, int64_t at, const f
 }
 
 template <typename T, bool I8, int D>
-__global__ void __launch_bounds__(256) read_kernel(const Pages c, int layer0, int layers, const int32_t* __restrict__ first, int count, void* key, void* value, int dtype) {
+__global__ void __launch_bounds__(256) read_kernel(const Pages c, int layer0, const int32_t* __restrict__ first, int count, void* key, void* value, int dtype) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES;
+  const int sub = threadIdx.x % LANES, head = blockIdx.x % c.kv_heads, rest = blockIdx.x / c.kv_heads, b = rest % c.batch, layer = rest / c.batch;
   cudaGridDependencySynchronize();
-  const int sub = threadIdx.x % LANES;
-  const int64_t chunks = (count + ROWS - 1) / ROWS, items = chunks * layers * c.batch * c.kv_heads;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int t = static_cast<int>(item % chunks) * ROWS + threadIdx.x / LANES;
-    if (t >= count) continue;
-    const int64_t outer = item / chunks;  // (layer, batch, head)
-    const int head = static_cast<int>(outer % c.kv_heads), b = static_cast<int>(outer / c.kv_heads % c.batch);
-    const int layer = static_cast<int>(outer / c.kv_heads / c.batch);
-    const int64_t at = static_cast<int64_t>(first[b]) + t;
-    float k[8], v[8];
+  const int64_t first_row = first[b], out0 = static_cast<int64_t>(blockIdx.x) * count;
+  const int len = length_of(c, b);
+  for (int t0 = blockIdx.y * ROWS * kDeep; t0 < count; t0 += gridDim.y * ROWS * kDeep) {
+    float k[kDeep][8], v[kDeep][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
-    if (at >= 0 && at < length_of(c, b)) {
+    for (int i = 0; i < kDeep; ++i) {
+      const int t = t0 + i * ROWS + threadIdx.x / LANES;
+      const int64_t at = first_row + t;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) k[i][x] = v[i][x] = 0.f;
+      if (t >= count || at < 0 || at >= len) continue;
       const int page = c.table[static_cast<int64_t>(b) * c.width + (at >> c.shift)];
-      if (is_page(c, page)) {
-        const int64_t row = block_row(c, layer0 + layer, page, head) + (at & (c.page - 1));
-        fetch8<T, I8>(c.keys, c.key_scales, row, D, sub, k);
-        fetch8<T, I8>(c.values, c.value_scales, row, D, sub, v);
-      }
+      if (!is_page(c, page)) continue;
+      const int64_t row = block_row(c, layer0 + layer, page, head) + (at & (c.page - 1));
+      fetch8<T, I8>(c.keys, c.key_scales, row, D, sub, k[i]);
+      fetch8<T, I8>(c.values, c.value_scales, row, D, sub, v[i]);
     }
-    store8(key, dtype, (outer * count + t) * D + sub * 8, k);
-    store8(value, dtype, (outer * count + t) * D + sub * 8, v);
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const int t = t0 + i * ROWS + threadIdx.x / LANES;
+      if (t >= count) continue;
+      store8(key, dtype, (out0 + t) * D + sub * 8, k[i]);
+      store8(value, dtype, (out0 + t) * D + sub * 8, v[i]);
+    }
   }
 }
 
@@ -529,21 +544,22 @@ int launched(cudaError_t e, const char* what) {
 
 unsigned copy_grid(int64_t items) { return static_cast<unsigned>(items < 148 * 8 ? (items > 0 ? items : 1) : 148 * 8); }
 
+dim3 row_grid(const Pages& p, int layers, int rows) {
+  const int per = 256 / (p.dim / 8) * kDeep, blocks = (rows + per - 1) / per;
+  return dim3(static_cast<unsigned>(layers) * p.batch * p.kv_heads, blocks < 1024 ? blocks : 1024);
+}
+
 template <typename T, bool I8>
 cudaError_t launch_write(const Pages& p, const Source& s, cudaStream_t st) {
-  const int rows = 256 / (p.dim / 8);
-  const int64_t items = static_cast<int64_t>((s.tokens + rows - 1) / rows) * s.layers * p.batch * p.kv_heads;
-  const dim3 grid(copy_grid(items));
+  const dim3 grid = row_grid(p, s.layers, s.tokens);
   return p.dim == 128 ? launch_chained(write_kernel<T, I8, 128>, grid, dim3(256), 0, st, p, s)
                       : launch_chained(write_kernel<T, I8, 64>, grid, dim3(256), 0, st, p, s);
 }
 template <typename T, bool I8>
 cudaError_t launch_read(const Pages& p, int layer0, int layers, const int32_t* first, int count, void* key, void* value, int dtype, cudaStream_t st) {
-  const int rows = 256 / (p.dim / 8);
-  const int64_t items = static_cast<int64_t>((count + rows - 1) / rows) * layers * p.batch * p.kv_heads;
-  const dim3 grid(copy_grid(items));
-  return p.dim == 128 ? launch_chained(read_kernel<T, I8, 128>, grid, dim3(256), 0, st, p, layer0, layers, first, count, key, value, dtype)
-                      : launch_chained(read_kernel<T, I8, 64>, grid, dim3(256), 0, st, p, layer0, layers, first, count, key, value, dtype);
+  const dim3 grid = row_grid(p, layers, count);
+  return p.dim == 128 ? launch_chained(read_kernel<T, I8, 128>, grid, dim3(256), 0, st, p, layer0, first, count, key, value, dtype)
+                      : launch_chained(read_kernel<T, I8, 64>, grid, dim3(256), 0, st, p, layer0, first, count, key, value, dtype);
 }
 template <int ROW_BYTES, bool I8>
 cudaError_t launch_move(const Pages& p, const Paths& paths, cudaStream_t st) {
