@@ -230,20 +230,20 @@ template <>
 __device__ __forceinline__ float2 two_floats<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
 // Eight values of a row as 8-bit codes.  The row's maximum is taken over the bit patterns of the
-// magnitudes (ordered like the values, NaN above infinity) by the row's D / 8 lanes.
+// magnitudes (ordered like the values, NaN above infinity) by the row's D / 8 lanes.  Bound by
+// instructions, hence the packed arithmetic.
 template <typename T, int D>
 __device__ __forceinline__ uint2 quantise8(uint4 raw, float* scale) {
-  float x[8];
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  float2 x[4];
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = two_floats<T>(w[i]);
-    x[2 * i] = f.x, x[2 * i + 1] = f.y;
-    top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+    x[i] = two_floats<T>(w[i]);
+    top = max(top, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu));
   }
-#pragma unroll
-  for (int o = 1; o < D / 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  constexpr uint32_t kLanes = D / 8, kMask = kLanes == 16 ? 0xffffu : 0xffu;
+  top = __reduce_max_sync(kMask << (threadIdx.x & 31 & ~(kLanes - 1)), top);
   if (top >= 0x7f800000u) {
     *scale = __int_as_float(0x7fc00000);
     return make_uint2(0, 0);
@@ -251,27 +251,36 @@ __device__ __forceinline__ uint2 quantise8(uint4 raw, float* scale) {
   const float s = __fadd_rn(__fdiv_rn(__uint_as_float(top), 127.f), 1e-7f);
   *scale = s;
   // rint(x / s): |x / s| <= 127, so no clamp, and 1.5 * 2^23 + integer has the code in its low byte.  x times
-  // the rounded reciprocal lies within 2.4e-5 of the quotient and rounds like it, unless it is that near a
-  // half-integer: then (one value in some thousands) the quotient itself is rounded.
-  const float inv = __fdiv_rn(1.f, s), magic = 12582912.f;
-  uint32_t code[8];
+  // the approximate reciprocal lies within 127 * 2 * 2^-23 = 3.1e-5 of the quotient and rounds like it, unless
+  // it is that near a half-integer: then (one value in some thousands) the quotient itself is rounded.
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  const float2 inv2 = make_float2(inv, inv), magic = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f), neg = make_float2(-1.f, -1.f);
+  float2 m[4];
   float near = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = __fmul_rn(x[i], inv), m = __fadd_rn(q, magic);
-    near = fmaxf(near, fabsf(__fsub_rn(q, __fsub_rn(m, magic))));
-    code[i] = __float_as_uint(m) & 0xffu;
+  for (int i = 0; i < 4; ++i) {
+    const float2 q = __fmul2_rn(x[i], inv2);
+    m[i] = __fadd2_rn(q, magic);
+    const float2 d = __ffma2_rn(__fadd2_rn(m[i], minus), neg, q);
+    near = fmaxf(near, fmaxf(fabsf(d.x), fabsf(d.y)));
   }
   if (near > 0.4999f) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) code[i] = __float_as_uint(__fadd_rn(__fdiv_rn(x[i], s), magic)) & 0xffu;
+    for (int i = 0; i < 4; ++i) m[i] = make_float2(__fadd_rn(__fdiv_rn(x[i].x, s), 12582912.f), __fadd_rn(__fdiv_rn(x[i].y, s), 12582912.f));
   }
-  return make_uint2(code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24, code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24);
+  uint32_t two[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) two[i] = __byte_perm(__float_as_uint(m[i].x), __float_as_uint(m[i].y), 0x0040);
+  return make_uint2(__byte_perm(two[0], two[1], 0x5410), __byte_perm(two[2], two[3], 0x5410));
 }
 
-constexpr int kDeep = 4;  // rows per thread: their loads are issued together
+// Rows per thread whose loads are issued together.  Storing: two (8-bit rows 31.8 us against 37.5 with one
+// and 33.7 with four, 8 prompts of up to 2047 rows, 8 heads); gathering: one (36.0 / 37.5 / 49.0 us; its
+// output alone, 134 MB, takes a fill kernel 39 us).
+constexpr int kStoreDeep = 2, kGatherDeep = 1;
 
-// blockIdx.x: (layer, sequence, head); blockIdx.y: rows [y * ROWS * kDeep, ...).
+// blockIdx.x: (layer, sequence, head); blockIdx.y: a block of rows.
 template <typename T, bool I8, int D>
 __global__ void __launch_bounds__(256) write_kernel(const Pages c, const Source s) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES;
@@ -280,11 +289,11 @@ __global__ void __launch_bounds__(256) write_kernel(const Pages c, const Source 
   const int start = c.starts[b], added = min(length_of(c, b) - start, s.tokens);
   const uint16_t* key = s.key + layer * s.ks[0] + b * s.ks[1] + head * s.ks[2] + sub * 8;
   const uint16_t* value = s.value + layer * s.vs[0] + b * s.vs[1] + head * s.vs[2] + sub * 8;
-  for (int t0 = blockIdx.y * ROWS * kDeep; t0 < added && start >= 0; t0 += gridDim.y * ROWS * kDeep) {
-    int64_t row[kDeep];
-    uint4 k[kDeep], v[kDeep];
+  for (int t0 = blockIdx.y * ROWS * kStoreDeep; t0 < added && start >= 0; t0 += gridDim.y * ROWS * kStoreDeep) {
+    int64_t row[kStoreDeep];
+    uint4 k[kStoreDeep], v[kStoreDeep];
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) {
+    for (int i = 0; i < kStoreDeep; ++i) {
       const int t = t0 + i * ROWS + threadIdx.x / LANES, at = start + t;
       row[i] = -1;
       k[i] = v[i] = make_uint4(0, 0, 0, 0);
@@ -295,7 +304,7 @@ __global__ void __launch_bounds__(256) write_kernel(const Pages c, const Source 
       if (is_page(c, page)) row[i] = block_row(c, s.layer0 + layer, page, head) + (at & (c.page - 1));
     }
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) {
+    for (int i = 0; i < kStoreDeep; ++i) {
       if (I8) {
         float ks, vs;
         const uint2 kc = quantise8<T, D>(k[i], &ks), vc = quantise8<T, D>(v[i], &vs);
@@ -356,10 +365,10 @@ __global__ void __launch_bounds__(256) read_kernel(const Pages c, int layer0, co
   cudaGridDependencySynchronize();
   const int64_t first_row = first[b], out0 = static_cast<int64_t>(blockIdx.x) * count;
   const int len = length_of(c, b);
-  for (int t0 = blockIdx.y * ROWS * kDeep; t0 < count; t0 += gridDim.y * ROWS * kDeep) {
-    float k[kDeep][8], v[kDeep][8];
+  for (int t0 = blockIdx.y * ROWS * kGatherDeep; t0 < count; t0 += gridDim.y * ROWS * kGatherDeep) {
+    float k[kGatherDeep][8], v[kGatherDeep][8];
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) {
+    for (int i = 0; i < kGatherDeep; ++i) {
       const int t = t0 + i * ROWS + threadIdx.x / LANES;
       const int64_t at = first_row + t;
 #pragma unroll
@@ -372,7 +381,7 @@ __global__ void __launch_bounds__(256) read_kernel(const Pages c, int layer0, co
       fetch8<T, I8>(c.values, c.value_scales, row, D, sub, v[i]);
     }
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) {
+    for (int i = 0; i < kGatherDeep; ++i) {
       const int t = t0 + i * ROWS + threadIdx.x / LANES;
       if (t >= count) continue;
       store8(key, dtype, (out0 + t) * D + sub * 8, k[i]);
@@ -544,20 +553,20 @@ int launched(cudaError_t e, const char* what) {
 
 unsigned copy_grid(int64_t items) { return static_cast<unsigned>(items < 148 * 8 ? (items > 0 ? items : 1) : 148 * 8); }
 
-dim3 row_grid(const Pages& p, int layers, int rows) {
-  const int per = 256 / (p.dim / 8) * kDeep, blocks = (rows + per - 1) / per;
+dim3 row_grid(const Pages& p, int layers, int rows, int deep) {
+  const int per = 256 / (p.dim / 8) * deep, blocks = (rows + per - 1) / per;
   return dim3(static_cast<unsigned>(layers) * p.batch * p.kv_heads, blocks < 1024 ? blocks : 1024);
 }
 
 template <typename T, bool I8>
 cudaError_t launch_write(const Pages& p, const Source& s, cudaStream_t st) {
-  const dim3 grid = row_grid(p, s.layers, s.tokens);
+  const dim3 grid = row_grid(p, s.layers, s.tokens, kStoreDeep);
   return p.dim == 128 ? launch_chained(write_kernel<T, I8, 128>, grid, dim3(256), 0, st, p, s)
                       : launch_chained(write_kernel<T, I8, 64>, grid, dim3(256), 0, st, p, s);
 }
 template <typename T, bool I8>
 cudaError_t launch_read(const Pages& p, int layer0, int layers, const int32_t* first, int count, void* key, void* value, int dtype, cudaStream_t st) {
-  const dim3 grid = row_grid(p, layers, count);
+  const dim3 grid = row_grid(p, layers, count, kGatherDeep);
   return p.dim == 128 ? launch_chained(read_kernel<T, I8, 128>, grid, dim3(256), 0, st, p, layer0, first, count, key, value, dtype)
                       : launch_chained(read_kernel<T, I8, 64>, grid, dim3(256), 0, st, p, layer0, first, count, key, value, dtype);
 }
