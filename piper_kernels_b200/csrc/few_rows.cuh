@@ -133,54 +133,49 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 
   if (warp == kConsumers / 32) {
     // ---------------------------------------------------------------- producer
-    if (lane == 0) {
-      const int box = p.table ? min(p.page, C::TILE) : C::TILE;
-      int last = -1;
-      bool ok = true;
-      for (uint32_t w = w0; w < w1; ++w, walk.next(p)) {
-        const int i = static_cast<int>(w - w0), st = i % kStages;
-        if (i >= kStages && !mbar_wait_bounded(bars + 8 * (kStages + st), ((i / kStages) - 1) & 1, abort_flag, 61)) { ok = false; break; }
-        const uint32_t full = bars + 8 * st, dst = base + st * C::STAGE;
-        const int j0 = walk.key();
-        int scale_boxes = 0;
-        if (!p.table) {
-          there[st] = 1u;
-          mbar_expect_tx(full, C::STAGE);
-          tma_load_5d(dst, &tm_k, full, 0, j0, 0, p.k_stride[1] ? walk.h : 0, p.k_stride[0] ? walk.s.b : 0);
-          tma_load_5d(dst + C::KV_BYTES, &tm_v, full, 0, j0, 0, p.v_stride[1] ? walk.h : 0, p.v_stride[0] ? walk.s.b : 0);
-        } else {
-          int pages[C::TILE / 16];
-          uint32_t mask = 0;
-#pragma unroll
-          for (int x = 0; x < C::TILE / 16; ++x) {
-            const int j = j0 + x * box;
-            // a page that is not there, or lies behind the sequence, reads as zeros (outside the map)
-            pages[x] = (x * box < C::TILE && j < walk.s.len) ? attend_page(p, walk.s.b, j) : -1;
-            if (pages[x] >= 0) mask |= 1u << x;
-            if (I8 && pages[x] >= 0) ++scale_boxes;
-          }
-          there[st] = mask;
-          mbar_expect_tx(full, C::STAGE + scale_boxes * 2 * box * 4);
-#pragma unroll
-          for (int x = 0; x < C::TILE / 16; ++x) {
-            if (x * box >= C::TILE) break;
-            const int row = (j0 + x * box) & (p.page - 1);
-            const int c4 = pages[x] >= 0 ? p.page_base + pages[x] : 0x7fffffff;
-            tma_load_5d(dst + x * box * C::ROW_BYTES, &tm_k, full, 0, row, 0, walk.h, c4);
-            tma_load_5d(dst + C::KV_BYTES + x * box * C::ROW_BYTES, &tm_v, full, 0, row, 0, walk.h, c4);
-            if (I8 && pages[x] >= 0) {
-              const int64_t at = (static_cast<int64_t>(pages[x]) * p.kv_heads + walk.h) * p.page + row;
-              const uint32_t sdst = base + C::OFF_SCALE + st * C::SCALE_BYTES + x * box * 4;
-              bulk_load(sdst, p.k_scale + at, box * 4, full);
-              bulk_load(sdst + C::TILE * 4, p.v_scale + at, box * 4, full);
-            }
-          }
-        }
-        last = i;
+    // Of a paged tile every page is a copy of its own, issued by a lane of its own; the pages of the next
+    // tile are looked up while this one's stage is waited for.
+    const int box = p.table ? min(p.page, C::TILE) : C::TILE, boxes = C::TILE / box;
+    auto look_up = [&]() {
+      const int j = walk.key() + lane * box;
+      return p.table && lane < boxes && j < walk.s.len ? attend_page(p, walk.s.b, j) : -1;
+    };
+    int last = -1, page = look_up();
+    bool ok = true;
+    for (uint32_t w = w0; w < w1; ++w) {
+      const int i = static_cast<int>(w - w0), st = i % kStages, j0 = walk.key(), h = walk.h, b = walk.s.b;
+      walk.next(p);
+      const int next = w + 1 < w1 ? look_up() : -1;
+      if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * (kStages + st), ((i / kStages) - 1) & 1, abort_flag, 61))) { ok = false; break; }
+      const uint32_t full = bars + 8 * st, dst = base + st * C::STAGE;
+      const uint32_t mask = p.table ? __ballot_sync(0xffffffffu, page >= 0) : 1u;
+      if (lane == 0) {
+        there[st] = mask;
+        mbar_expect_tx(full, C::STAGE + (I8 ? __popc(mask) * 2 * box * 4 : 0));
       }
-      if (!ok)  // giving up: let the copies that were issued land before the CTA returns
-        for (int i = max(0, last - kStages + 1); i <= last; ++i) mbar_wait_quiet(bars + 8 * (i % kStages), (i / kStages) & 1, 100000);
+      __syncwarp();
+      if (!p.table) {
+        if (lane == 0) {
+          tma_load_5d(dst, &tm_k, full, 0, j0, 0, p.k_stride[1] ? h : 0, p.k_stride[0] ? b : 0);
+          tma_load_5d(dst + C::KV_BYTES, &tm_v, full, 0, j0, 0, p.v_stride[1] ? h : 0, p.v_stride[0] ? b : 0);
+        }
+      } else if (lane < boxes) {
+        // a page that is not there, or lies behind the sequence, reads as zeros (outside the map)
+        const int row = (j0 + lane * box) & (p.page - 1), c4 = page >= 0 ? p.page_base + page : 0x7fffffff;
+        tma_load_5d(dst + lane * box * C::ROW_BYTES, &tm_k, full, 0, row, 0, h, c4);
+        tma_load_5d(dst + C::KV_BYTES + lane * box * C::ROW_BYTES, &tm_v, full, 0, row, 0, h, c4);
+        if (I8 && page >= 0) {
+          const int64_t at = (static_cast<int64_t>(page) * p.kv_heads + h) * p.page + row;
+          const uint32_t sdst = base + C::OFF_SCALE + st * C::SCALE_BYTES + lane * box * 4;
+          bulk_load(sdst, p.k_scale + at, box * 4, full);
+          bulk_load(sdst + C::TILE * 4, p.v_scale + at, box * 4, full);
+        }
+      }
+      page = next;
+      last = i;
     }
+    if (!ok)  // giving up: let the copies that were issued land before the CTA returns
+      for (int i = max(0, last - kStages + 1); i <= last; ++i) mbar_wait_quiet(bars + 8 * (i % kStages), (i / kStages) & 1, 100000);
     return;
   }
 

@@ -260,54 +260,48 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (warp >= 16) setmaxnreg_dec<kHelperRegs>();
   if (warp == COPY_WARP) {
     // ---------------------------------------------------------------- copies
-    if (lane == 0) {
-      const int box = p.table ? min(p.page, kWideTile) : kWideTile;
-      uint32_t st = 0, ph = 1;
-      int n = 0;  // K and V tiles issued
-      bool ok = true;
-      for (; ok && seg.more(); seg.advance(p)) {
-        const Span& s = seg.walk.s;
-        const int count = seg.count(), from = seg.walk.tile;
-        for (int u = 0; ok && u < count; ++u) {
-          const int j0 = key_of_tile<kWideTile>(s, from + u);
-          int pages[kWideTile / 16];
-          uint32_t mask = 1u;
-          if (p.table) {
-            mask = 0;
-#pragma unroll
-            for (int x = 0; x < kWideTile / 16; ++x) {
-              const int j = j0 + x * box;
-              pages[x] = (x * box < kWideTile && j < s.len) ? attend_page(p, s.b, j) : -1;
-              if (pages[x] >= 0) mask |= 1u << x;
-            }
-          }
-          there[(n / 2) % kThere] = mask;
+    // Of a paged tile every page and half of the features is a copy of its own, issued by a lane of its
+    // own; the pages of the next tile are looked up while this one's stages are waited for.
+    const int box = p.table ? min(p.page, kWideTile) : kWideTile, boxes = kWideTile / box;
+    const int x = lane % 8, hf = lane / 8;
+    const bool mine = x < boxes && hf < D / 64;
+    uint32_t st = 0, ph = 1;
+    int n = 0;  // K and V tiles issued
+    bool ok = true;
+    for (; ok && seg.more(); seg.advance(p)) {
+      const Span& s = seg.walk.s;
+      const int count = seg.count(), from = seg.walk.tile, h = seg.walk.h;
+      auto look_up = [&](int u) {
+        const int j = key_of_tile<kWideTile>(s, from + u) + x * box;
+        return p.table && mine && u < count && j < s.len ? attend_page(p, s.b, j) : -1;
+      };
+      int page = look_up(0);
+      for (int u = 0; ok && u < count; ++u) {
+        const int j0 = key_of_tile<kWideTile>(s, from + u), next = look_up(u + 1);
+        const uint32_t mask = p.table ? __ballot_sync(0xffffffffu, page >= 0) & 0xffu : 1u;
+        if (lane == 0) there[(n / 2) % kThere] = mask;
 #pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv, ++n) {
-            if (n >= ST && !(ok = wide_wait(empty(st), ph, abort_flag, 71))) break;
-            const uint32_t dst = base + C::OFF_RING + st * C::TILE_BYTES;
-            const CUtensorMap* tmap = kv ? &tm_v : &tm_k;
-            mbar_expect_tx(full(st), C::TILE_BYTES);
-            if (!p.table) {
-              const int64_t sh = kv ? p.v_stride[1] : p.k_stride[1], sb = kv ? p.v_stride[0] : p.k_stride[0];
-              tma_load_5d(dst, tmap, full(st), 0, j0, 0, sh ? seg.walk.h : 0, sb ? s.b : 0);
-            } else {
-#pragma unroll
-              for (int x = 0; x < kWideTile / 16; ++x) {
-                if (x * box >= kWideTile) break;
-                const int row = (j0 + x * box) & (p.page - 1);
-                const int c4 = pages[x] >= 0 ? p.page_base + pages[x] : 0x7fffffff;
-#pragma unroll
-                for (int hf = 0; hf < D / 64; ++hf) tma_load_5d(dst + hf * C::HALF + x * box * 128, tmap, full(st), 0, row, hf, seg.walk.h, c4);
-              }
-            }
-            if (++st == ST) st = 0, ph ^= 1;
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          if (n >= ST && !(ok = WIDE_ALL(wide_wait(empty(st), ph, abort_flag, 71)))) break;
+          const uint32_t dst = base + C::OFF_RING + st * C::TILE_BYTES;
+          const CUtensorMap* tmap = kv ? &tm_v : &tm_k;
+          if (lane == 0) mbar_expect_tx(full(st), C::TILE_BYTES);
+          __syncwarp();
+          if (p.table) {
+            // a page that is not there, or lies behind the sequence, reads as zeros (outside the map)
+            if (mine)
+              tma_load_5d(dst + hf * C::HALF + x * box * 128, tmap, full(st), 0, (j0 + x * box) & (p.page - 1), hf, h, page >= 0 ? p.page_base + page : 0x7fffffff);
+          } else if (lane == 0) {
+            const int64_t sh = kv ? p.v_stride[1] : p.k_stride[1], sb = kv ? p.v_stride[0] : p.k_stride[0];
+            tma_load_5d(dst, tmap, full(st), 0, j0, 0, sh ? h : 0, sb ? s.b : 0);
           }
+          if (++st == ST) st = 0, ph ^= 1;
         }
+        page = next;
       }
-      if (*abort_flag != 0) {  // let the copies that were issued land before the CTA returns
-        for (int i = max(0, n - ST); i < n; ++i) mbar_wait_quiet(full(i % ST), (i / ST) & 1, 100000);
-      }
+    }
+    if (*abort_flag != 0) {  // let the copies that were issued land before the CTA returns
+      for (int i = max(0, n - ST); i < n; ++i) mbar_wait_quiet(full(i % ST), (i / ST) & 1, 100000);
     }
   } else if (warp == MMA_WARP) {
     // ---------------------------------------------------------------- products
