@@ -112,8 +112,8 @@ __device__ __forceinline__ void build_tree(const AttendParams& p, int b, int off
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int t = lane + 32 * i, mine = __popcll(mask[i]) - 1;
-    uint64_t m = mask[i], keep = 0;
-    while (m) {  // at most one turn per level
+    uint64_t m = p.window < kNoWindow ? mask[i] : 0, keep = p.window < kNoWindow ? 0 : mask[i];
+    while (m) {  // a window: at most one turn per level
       const int a = __ffsll(static_cast<long long>(m)) - 1;
       m &= m - 1;
       const int d = tm->depth[a];

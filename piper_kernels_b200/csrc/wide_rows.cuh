@@ -557,19 +557,29 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         p.pieces[seg.walk.g * p.kv_heads + h] = Pieces{static_cast<int>(blockIdx.x), static_cast<int>(owner_of(total, p.workers, seg.at + s.n - 1)), seg.at != share_from, 0};
       if (!seg.whole() && (from != 0 || count != s.n)) {
         const int slot = blockIdx.x * 2 + (seg.at != share_from ? 1 : 0);
-        float* dst = p.partial + (static_cast<int64_t>(slot) * kWideRows + i * 128 + row) * (D + 4);
+        float* dst = p.partial + (static_cast<int64_t>(slot) * kWideRows + i * 128) * (D + 4);
+        // 32 features at a time through this warp's rows of the query tile, so that whole lines leave
+        constexpr int STRIDE = FEATURES * 2;  // bytes of a row's half in the query tile: this half's 16-bit pieces
+        static_assert(STRIDE >= 64, "eight lanes write 32 features of a row");
+#pragma unroll 1
+        for (int c = 0; c < FEATURES; c += STRIDE / 4) {
+          uint32_t o[STRIDE / 4];
 #pragma unroll
-        for (int c = 0; c < FEATURES; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_addr + c, o);
+          for (int e = 0; e < STRIDE / 4; e += 16) tmem_ld16(o_addr + c + e, o + e);
           tmem_wait_ld();
-          if (r < p.rows) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 2)
-              *reinterpret_cast<float2*>(dst + half * FEATURES + c + e) = begun ? make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])) : make_float2(0.f, 0.f);
+          for (int e = 0; e < STRIDE / 16; ++e)
+            *reinterpret_cast<uint4*>(q_piece(row, e)) = begun ? make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]) : make_uint4(0, 0, 0, 0);
+          __syncwarp();
+#pragma unroll
+          for (int a = 0; a < 32 / PER; ++a) {
+            const int piece = lane % PIECES, rl = w4 * 32 + a * PER + lane / PIECES;
+            const uint4 x = *reinterpret_cast<const uint4*>(q_piece(rl, piece));
+            if (row0 + rl < p.rows) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(rl) * (D + 4) + half * FEATURES + c + piece * 4) = x;
           }
+          __syncwarp();
         }
-        if (r < p.rows && half == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m, l);
+        if (r < p.rows && half == 0) *reinterpret_cast<float2*>(dst + static_cast<int64_t>(row) * (D + 4) + D) = make_float2(m, l);
         tc_fence_before();
         continue;
       }
