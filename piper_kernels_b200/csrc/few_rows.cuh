@@ -43,7 +43,9 @@ struct Few {
   static constexpr int ROWS = 16 * WM;
   static constexpr int ESZ = I8 ? 1 : 2;
   static constexpr int ROW_BYTES = D * ESZ;
-  static constexpr int TILE = ROW_BYTES > 128 ? 64 : 128;  // keys per stage: 16 to 32 KB of K and V
+  // Keys per stage: 16 to 32 KB of K and V where the warps share them out; fewer where every warp takes all of
+  // them for its own rows (a stage's time counts when there are few).
+  static constexpr int TILE = ROW_BYTES > 128 || WM > 1 ? 64 : 128;
   static constexpr int LINE = ROW_BYTES > 128 ? 128 : ROW_BYTES;  // swizzled line
   static constexpr int HALVES = ROW_BYTES / LINE;
   static constexpr int KV_BYTES = TILE * ROW_BYTES;

@@ -407,7 +407,10 @@ __global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_const
   // (a piece's slot) * ROWS + r, in rows of D + 4 words
   auto slot = [&](int c) { return (static_cast<int64_t>(2 * c + (c == at.c0 ? at.late : 0)) * ROWS + r) * (D + 4); };
   float mx = -INFINITY, sum = 0.f, acc[E];
-  for (int c = at.c0 + lane; c <= at.c1; c += 32) mx = fmaxf(mx, p.partial[slot(c) + D]);
+  float2 first = make_float2(-INFINITY, 0.f);  // maximum and sum of this lane's first piece
+  if (at.c0 + lane <= at.c1) first = *reinterpret_cast<const float2*>(p.partial + slot(at.c0 + lane) + D);
+  mx = first.x;
+  for (int c = at.c0 + 32 + lane; c <= at.c1; c += 32) mx = fmaxf(mx, p.partial[slot(c) + D]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
 #pragma unroll
@@ -415,12 +418,12 @@ __global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_const
   for (int c0 = at.c0; c0 <= at.c1; c0 += 32) {
     float w = 0.f;
     if (c0 + lane <= at.c1) {
-      const float2 st = *reinterpret_cast<const float2*>(p.partial + slot(c0 + lane) + D);
+      const float2 st = c0 == at.c0 ? first : *reinterpret_cast<const float2*>(p.partial + slot(c0 + lane) + D);
       w = st.x == mx ? 1.f : ex2_approx(st.x - mx);
       sum = fmaf(st.y, w, sum);
     }
     const int n = min(32, at.c1 - c0 + 1);
-#pragma unroll 4
+#pragma unroll 8
     for (int c = 0; c < n; ++c) {
       const float wgt = __shfl_sync(0xffffffffu, w, c);
       const float* src = p.partial + slot(c0 + c) + lane * E;
