@@ -4,9 +4,9 @@
 //
 // What bounds it: every K and V row is read once for the few query rows that see it, 4 * rows / 2
 // operations per byte, so device memory does.  The kernel is built to keep copies in flight:
-//   - A producer warp fills a ring of three 64-key stages (K and V, up to 32 KB each) with TMA,
-//     one copy per page; two CTAs per SM keep up to 192 KB on the way.
-//   - The keys of all batch elements and heads form one list of 64-key tiles; every CTA takes an
+//   - A producer warp fills a ring of three stages of 64 or 128 keys (K and V, up to 32 KB each) with
+//     TMA, one copy per page; two CTAs per SM keep up to 192 KB on the way.
+//   - The keys of all batch elements and heads form one list of such tiles; every CTA takes an
 //     equal, contiguous share of it, whatever the lengths are (they are read on the device: nothing
 //     about them is known to the host).  The ring runs on across the borders between sequences.
 //   - A sequence that several CTAs share leaves pieces (un-normalised rows, maximum, sum) in the
@@ -22,6 +22,11 @@
 // gets p / scale (the way the 8-bit attention of fused_attention.cu treats its key scales), so that
 // p stays in the range of a 16-bit float whatever the scales are.  p is rounded to the query's
 // 16-bit type for the product; maxima, sums and accumulators are 32-bit.
+// Measured: 64 single tokens (32 / 8 heads of 128 features) over 1088 to 8192 bfloat16 rows, 1.22 GB: 195 us,
+// 6.3 TB/s (0.96 of the measured copy).  48 tokens (40 / 8 heads) over 8-bit rows, window 4096, 417 MB: 126 us,
+// 3.3 TB/s: there the conversions to 16 bits (about 170 of 560 instructions for 16 keys of a warp) and the
+// latency of two warps per scheduler bound it, not memory.  One token over 1000 rows: 6.6 us and 5.8 us
+// for the join.
 
 #pragma once
 

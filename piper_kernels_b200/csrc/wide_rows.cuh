@@ -19,10 +19,17 @@
 //     has grown by more than 2^8.  The exponentials start with the reference of the tile before, without
 //     waiting for this tile's maximum; only when a row has to raise it (the first tile, and rarely later)
 //     they are evaluated again, and the accumulator is rescaled.
-//   - A part of the exponentials is evaluated on the FMA pipe beside the exponential unit.
-// Tried and slower (prompt of 8192, 32 heads, no window): one warpgroup per row tile MEASURED1; 64-key tiles
-// with two score buffers per row tile, with one or two warpgroups per row tile and one or two issuing
-// warps, 660 to 870 us: the smaller tiles halve what is in flight per buffer and every hand-over costs the same.
+//   - A few of the exponentials are evaluated on the FMA pipe beside the exponential unit.
+// Measured: 4 prompts of 8192 tokens, 32 query and 8 key heads of 128 features, window 1024, float16:
+// 720 us, 719 TFLOP/s of visible pairs (0.44 of the measured 1652); the last 2048 tokens of 32760, 40 / 8
+// heads, window 4096, bfloat16: 195 us, 895 TFLOP/s.  A tile's chain takes about 4000 cycles where the two row
+// tiles' products fill 2048: 2700 in the softmax (with one or two warps of a row tile per scheduler most of
+// it is latency; taking the exponentials out altogether makes the kernel 6 % faster), the rest in the
+// products and in the hand-overs around them.
+// Tried and slower (one prompt of 8192, 32 / 8 heads, no window, 582 us): one warpgroup per row tile, 595 us
+// with this order of work and 670 with the maximum first; 64-key tiles with two score buffers per row tile,
+// with one or two warpgroups per row tile and one or two issuing warps, 660 to 870 us (half is in flight
+// per buffer, and every hand-over costs the same); more of the exponentials on the FMA pipe, 590 to 650 us.
 // V is read as it lies in memory (keys in rows): the B operand is taken transposed.
 #pragma once
 
@@ -40,6 +47,8 @@ static_assert((4 * kSoftmaxRegs + kHelperRegs) * 128 <= kWideThreads * kWideLaun
 constexpr float kWideRaise = 8.f;
 constexpr int kThere = 8;  // a copy is issued at most STAGES / 2 + 1 key tiles ahead of a tile whose V is still in use
 constexpr int kWideWorkers = 148;
+// From four rounds of units on, the partial last round costs less than sharing it out (768 ragged units: 118
+// against 135 us); below, sharing pays (320 units: 213 against 231 us).
 constexpr int64_t kWideShareBelow = 4 * kWideWorkers;
 
 #define WIDE_ALL(x) __all_sync(0xffffffffu, (x))
@@ -94,7 +103,7 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t addr, int half) {
          (2ull << 61);
 }
 
-// 2^x for two values on the FMA pipe (the exponential unit alone would set the pace): x = n + r with
+// 2^x for two values on the FMA pipe beside the exponential unit (an eighth of them: 1 %, more is slower): x = n + r with
 // n the nearest integer and |r| <= 1/2; 2^r by a polynomial of degree 4, fitted here for the least
 // largest relative error with value 1 at 0 (2.9e-6, measured over r in 32-bit arithmetic); n goes into
 // the exponent.  Below -127 the result is 0 (r = 0 there).  A NaN or infinity may come out as any huge
@@ -121,11 +130,17 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// A bounded wait with little code (the roles' loops should stay in the instruction caches): gives up
-// after some 2^24 probes, or when another wait has been given up.
+// A bounded wait with little code (it is in every role's loop): gives up after some seconds, or when
+// another wait has been given up.  The limit is generous because a softmax warp may be away evaluating
+// rows one by one (plain_row) while the others wait for it.
+constexpr long long kWideWaitCycles = 4 * kWaitCycleLimit;
 __device__ __forceinline__ bool wide_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int where) {
+  long long since = 0;
   for (int n = 0; !mbar_try_wait(bar, parity); ++n) {
-    if ((n & 63) == 63 && (*abort_flag != 0 || n > (1 << 24))) {
+    if ((n & 63) != 63) continue;
+    const long long now = clock64();
+    if (since == 0) since = now;
+    if (*abort_flag != 0 || now - since > kWideWaitCycles) {
       *abort_flag = where;
       return false;
     }

@@ -36,8 +36,9 @@ def attend(q, k, v, visible, scale, dtype, value_step=0.0):
     - the result: half a step, h = eps / 2 relative;
     - each probability: h relative, and where a float16 is subnormal 2^-25 absolute (relative to the largest
       probability of the row, which is held at 1 or more): h * sum w|v| + n * 2^-25 * max|v|;
-    - a score: a sum of d products in 32 bits, (d + 4) * 2^-24 * scale * sum|q k|, and the exponential's
-      2^-21: as a relative change of every weight, twice (the quotient).
+    - a score: a sum of d products in 32 bits, (d + 4) * 2^-24 * scale * sum|q k|, and the exponential,
+      2^-18 (the exponential unit is within 2^-21; a polynomial that takes a part of the work has a largest
+      relative error of 2.9e-6 = 2^-18.4): as a relative change of every weight, twice (the quotient).
     ``value_step``: the largest 8-bit row maximum; codes up to it share one reference exponent.
     """
     q, k, v = q.double(), k.double(), v.double()
@@ -45,7 +46,7 @@ def attend(q, k, v, visible, scale, dtype, value_step=0.0):
     w = torch.nan_to_num(torch.softmax(s, -1))
     size = v.abs()
     h = torch.finfo(dtype).eps / 2
-    weight = (q.shape[1] + 4) * 2.0**-24 * torch.where(visible, scale * (q.abs() @ k.abs().T), 0).amax(-1, keepdim=True) + 2.0**-21
+    weight = (q.shape[1] + 4) * 2.0**-24 * torch.where(visible, scale * (q.abs() @ k.abs().T), 0).amax(-1, keepdim=True) + 2.0**-18
     out = w @ v
     n = visible.sum(-1, keepdim=True)
     tiny = n * 2.0**-25 * max(float(size.max()), value_step) if dtype is torch.float16 else 0

@@ -115,6 +115,64 @@ def test_window_strides():
         same(q, kv[:, :1, 0].transpose(1, 2).expand(2, 2, 200, 64), kv[:, :1, 1].transpose(1, 2).expand(2, 2, 200, 64))
 
 
+def check_some(q, k, v, got, heads, **kw):
+    """A few heads of a call with many."""
+    group = q.shape[1] // k.shape[1]
+    for b, h in heads:
+        one = slice(b, b + 1)
+        check_window(q[one, h:h + 1], k[one, h // group:h // group + 1], v[one, h // group:h // group + 1], got=got[one, h:h + 1], **kw)
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,q_len,kv_len", [
+    (10, 32, 16, 100, 333),   # more units of 256 rows than SMs: whole rounds, the rest shared
+    (40, 32, 16, 80, 200),    # several rounds, none shared
+    (1, 2, 2, 3000, 3000),    # few units with many keys: all shared
+    (3, 7, 1, 333, 900),      # units that end inside a token's heads
+])
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, F16)])
+def test_window_units_over_the_sms(batch, heads, kv_heads, q_len, kv_len, dim, dtype):
+    q = normal(batch, heads, q_len, dim, dtype=dtype, seed=70)
+    k, v = (normal(batch, kv_heads, kv_len, dim, dtype=dtype, seed=s) for s in (71, 72))
+    some = [(0, 0), (batch - 1, heads - 1), (batch // 2, heads // 2), (batch // 3, 0)]
+    for kw in ({"window": 150, "sinks": 4}, {"window": 5000}):
+        check_some(q, k, v, pk.window_attention(q, k, v, **kw), some, **kw)
+
+
+@pytest.mark.parametrize("q_len", [1, 20, 300])
+@pytest.mark.parametrize("dim,dtype", [(128, F16), (64, BF16)])
+@pytest.mark.parametrize("jump", [0.02, 0.4, 3.0])
+def test_window_scores_that_keep_growing(q_len, dim, dtype, jump):
+    """Later keys score higher and higher (or far higher at once), so that the reference exponent of the
+    probabilities has to be raised again and again."""
+    q = normal(1, 4, q_len, dim, dtype=dtype, seed=73).abs()
+    k = (torch.linspace(0, 1, 700, device="cuda")[:, None] ** 2 * jump * 8 + 0.1 * normal(1, 2, 700, dim, dtype=torch.float32, seed=74)).to(dtype)
+    k[:, :, 400] += jump * 4
+    v = normal(1, 2, 700, dim, dtype=dtype, seed=75)
+    check_window(q, k, v, window=1000)
+    check_window(q, k.flip(2), v, window=300, sinks=70)
+
+
+def test_calls_from_two_threads():
+    from concurrent.futures import ThreadPoolExecutor
+
+    q = normal(2, 4, 300, 64, dtype=F16, seed=76)
+    k, v = (normal(2, 2, 300, 64, dtype=F16, seed=s) for s in (77, 78))
+    cache = filled(2, 40, 16, 2, 64, F16, [300, 77], [1, 1], seed=30)
+    torch.cuda.synchronize()
+
+    def work(_):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            a = pk.window_attention(q, k, v, window=90)
+            b = pk.cache_attention(q[:, :, :1], cache)
+            torch.cuda.current_stream().synchronize()
+        return a, b
+
+    want = work(0)
+    with ThreadPoolExecutor(2) as pool:
+        for a, b in pool.map(work, range(20)):
+            assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+
+
 def test_window_scale_and_large_scores():
     q = 30 * normal(1, 2, 90, 64, dtype=BF16, seed=18)
     k, v = (normal(1, 2, 90, 64, dtype=BF16, seed=s) for s in (19, 20))
@@ -242,6 +300,17 @@ def test_cached_trees(dim, dtype, store, tokens, heads, kv_heads):
     check_cached(q, cache, tree=trees)
     check_cached(q, cache, tree=trees, window=5, sinks=2)
     check_cached(q, cache, tree=some_tree(tokens, rng), window=200)
+
+
+def test_cached_large_trees_of_many_sequences():
+    """64 tokens of 8 heads per key head (512 rows: two units), lengths from the tree alone to long contexts."""
+    rng = random.Random(3)
+    lengths = [64, 1500, 300, 64 + 128, 70]
+    cache = filled(5, 160, 16, 2, 128, F16, lengths, [64, 64, 64, 64, 20], seed=32)
+    q = normal(5, 16, 64, 128, dtype=F16, seed=59)
+    trees = [some_tree(64, rng) for _ in range(5)]
+    check_cached(q, cache, tree=trees)
+    check_cached(q, cache, tree=trees, window=17, sinks=30)
 
 
 def test_cached_tree_that_is_a_chain_is_the_chain():
@@ -527,6 +596,46 @@ def test_write_takes_strided_rows_and_leaves_the_rest():
         for t in range(20, 23):
             allowed[1, cache.table[0, t // 16], t % 16] = True
         assert not (changed & ~allowed).any()
+
+
+def test_write_with_fewer_rows_than_were_added_leaves_the_others():
+    cache = pk.PageCache(2, 10, 16, 1, 64, dtype=F16)
+    cache.keys.fill_(7)
+    cache.extend(ints([20, 3]))
+    rows = normal(2, 1, 5, 64, dtype=F16, seed=55)
+    cache.write(rows, rows, layer=0)
+    k, _ = cache.read(ints([0, 0]), 20, layer=0)
+    assert torch.equal(k[0, :, :5], rows[0]) and (k[0, :, 5:] == 7).all()
+    assert torch.equal(k[1, :, :3], rows[1, :, :3]) and not k[1, :, 3:].any()
+
+
+def test_step_is_captured_and_replayed():
+    """A whole speculative step in one graph: room, rows, attention of the tree, the accepted path."""
+    cache = filled(2, 60, 16, 2, 64, BF16, [100, 33], [0, 0], seed=31, max_length=400)
+    eager = pk.PageCache.from_tensors(*(getattr(cache, n).clone() for n in ("keys", "values", "table", "lengths", "starts", "uses")))
+    q, k, v = (normal(2, h, 6, 64, dtype=BF16, seed=s) for h, s in ((4, 56), (2, 57), (2, 58)))
+    tree, counts = ints([-1, 0, 0, 1, 1, 3]), ints([6, 4])
+    paths, keep = ints([[0, 1, 3, 5], [0, 2, 0, 0]]), ints([4, 2])
+
+    def step(c):
+        c.extend(counts)
+        c.write(k, v, layer=0)
+        out = pk.cache_attention(q, c, tree=tree)
+        c.compact(paths, keep)
+        return out
+
+    kept = [t.clone() for t in (cache.keys, cache.values, cache.table, cache.lengths, cache.starts, cache.uses)]
+    step(cache)
+    for t, old in zip((cache.keys, cache.values, cache.table, cache.lengths, cache.starts, cache.uses), kept):
+        t.copy_(old)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(cache)
+    for _ in range(5):
+        k.add_(1)
+        graph.replay()
+        assert torch.equal(out, step(eager)) and state(cache) == state(eager)
+        assert torch.equal(cache.keys, eager.keys) and torch.equal(cache.values, eager.values)
 
 
 def test_read_outside_a_sequence_is_zero():
