@@ -15,21 +15,23 @@
 // Tensor memory holds one score tile of 128 columns and one accumulator per row tile, no more: a row
 // tile's scores, softmax and products follow one another, and the time of this chain is the kernel's.
 // So the softmax keeps it short:
-//   - Probabilities are relative to a reference exponent that follows the running maximum only when that
-//     has grown by more than 2^8.  The exponentials start with the reference of the tile before, without
-//     waiting for this tile's maximum; only when a row has to raise it (the first tile, and rarely later)
-//     they are evaluated again, and the accumulator is rescaled.
+//   - Probabilities are relative to a reference exponent that follows the running maximum only when the
+//     probabilities have grown too far (their sum over 64 keys tells: no maximum is taken on the way).  The
+//     exponentials start with the reference of the tile before; only when a row has to raise it (the first
+//     tile, and rarely later) the maximum is taken, the accumulator rescaled and they are evaluated again.
+//   - Tiles that every row sees whole take a path without branches.
 //   - A few of the exponentials are evaluated on the FMA pipe beside the exponential unit.
 // Measured: 4 prompts of 8192 tokens, 32 query and 8 key heads of 128 features, window 1024, float16:
-// 720 us, 719 TFLOP/s of visible pairs (0.44 of the measured 1652); the last 2048 tokens of 32760, 40 / 8
-// heads, window 4096, bfloat16: 195 us, 895 TFLOP/s.  A tile's chain takes about 4000 cycles where the two row
-// tiles' products fill 2048: 2700 in the softmax (with one or two warps of a row tile per scheduler most of
-// it is latency; taking the exponentials out altogether makes the kernel 6 % faster), the rest in the
-// products and in the hand-overs around them.
-// Tried and slower (one prompt of 8192, 32 / 8 heads, no window, 582 us): one warpgroup per row tile, 595 us
-// with this order of work and 670 with the maximum first; 64-key tiles with two score buffers per row tile,
-// with one or two warpgroups per row tile and one or two issuing warps, 660 to 870 us (half is in flight
-// per buffer, and every hand-over costs the same); more of the exponentials on the FMA pipe, 590 to 650 us.
+// 698 us, 741 TFLOP/s of visible pairs (0.45 of the measured 1652); the last 2048 tokens of 32760, 40 / 8
+// heads, window 4096, bfloat16: 180 us, 970 TFLOP/s (0.59).  A tile's chain takes some 3600 cycles where the two
+// row tiles' products fill 2048; two thirds of it are in the softmax, most of that latency (taking the
+// exponentials out altogether makes the kernel 6 % faster), the rest in the products and the hand-overs.
+// A unit's query rows in, first scores and rows out take about 9000 cycles, partly beside the other row tile.
+// Tried and slower (one prompt of 8192, 32 / 8 heads, no window, 532 us): the maximum taken beside the
+// exponentials, 543; narrower steps than 64 keys for a half, 575; one warpgroup per row tile, 595 us, and 670
+// with the maximum first; 64-key tiles with two score buffers per row tile, with one or two warpgroups per
+// row tile and one or two issuing warps, 660 to 870 us (half is in flight per buffer, and every hand-over
+// costs the same); all of a half's scores in registers at once, 710 us (they spill).
 // V is read as it lies in memory (keys in rows): the B operand is taken transposed.
 #pragma once
 
@@ -40,11 +42,10 @@ namespace {
 
 constexpr int kWideTile = 128;
 constexpr int kWideRows = 256;
-constexpr int kWideThreads = 5 * 128;  // four softmax warpgroups, one with the MMA and the copy warp
-// Registers of a thread after the split; setmaxnreg only moves what the CTA was launched with.
-constexpr int kWideLaunchRegs = 96, kSoftmaxRegs = 104, kHelperRegs = 64;
-static_assert((4 * kSoftmaxRegs + kHelperRegs) * 128 <= kWideThreads * kWideLaunchRegs, "register split exceeds the CTA's registers");
-constexpr float kWideRaise = 8.f;
+constexpr int kWideThreads = 4 * 128 + 64;  // four softmax warpgroups, the MMA and the copy warp
+// A row raises its reference exponent when its probabilities of 64 keys sum to more than this (2^12: the
+// largest of them fits every type).
+constexpr float kWideRaise = 4096.f;
 constexpr int kThere = 8;  // a copy is issued at most STAGES / 2 + 1 key tiles ahead of a tile whose V is still in use
 constexpr int kWideWorkers = 148;
 // From four rounds of units on, the partial last round costs less than sharing it out (768 ragged units: 118
@@ -202,7 +203,7 @@ __device__ __forceinline__ Reach reach_of(const AttendParams& p, const Span& s, 
 // How many of a tile's keys, from its first on, a row tile has to look at (a multiple of 32; 0: none).
 __device__ __forceinline__ int width_of(const Reach& r, int j0, int sinks) {
   const int end = j0 + kWideTile > r.lo ? r.hi : min(sinks, r.hi);
-  return max(0, min((end - j0 + 31) & ~31, kWideTile));
+  return max(0, min((end - j0 + 63) & ~63, kWideTile));
 }
 
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }  // bits [0, n)
@@ -272,7 +273,6 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   }
   seg.take(p);
 
-  if (warp >= 16) setmaxnreg_dec<kHelperRegs>();
   if (warp == COPY_WARP) {
     // ---------------------------------------------------------------- copies
     // Of a paged tile every page and half of the features is a copy of its own, issued by a lane of its
@@ -403,7 +403,6 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       }
     }
   } else if (warp < 16) {
-    setmaxnreg_inc<kSoftmaxRegs>();
     // ---------------------------------------------------------------- softmax
     // Row tile i; of each key tile the 64 keys of half `half`, of its features (query rows in, output
     // rows out) likewise.
@@ -462,7 +461,8 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       // keys that every row of this row tile sees
       const int t_first = token_of(p, min(row0, p.rows - 1)), t_last = token_of(p, min(row0 + 127, p.rows - 1));
       const int full_hi = TREE ? s.full_hi : min(s.len, s.off + t_first + 1), full_lo = TREE ? s.full_lo : s.off + t_last - p.window + 1;
-      float ref = -INFINITY, l = 0.f;  // reference exponent of the probabilities, sum of this half's
+      // Reference exponent of the probabilities (none yet; a row that sees nothing needs none), sum of this half's.
+      float ref = view.lim > 0 || view.mask != 0 ? -INFINITY : 0.f, l = 0.f;
       bool begun = false;
       for (int u = 0; u < count; ++u, ++nt) {
         const int j0 = key_of_tile<kWideTile>(s, from + u);
@@ -475,7 +475,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const bool clear = held == all && ((j0 >= full_lo && j0 + width <= full_hi) || j0 + width <= min(p.sinks, full_hi));
         uint32_t sr[32], pk[32];
         float* sc = reinterpret_cast<float*>(sr);
-        float top, shift;
+        float shift;
         float2 l0, l1;
         const float2 mul2 = make_float2(p.scale_log2, p.scale_log2);
         // 32 keys in sr: those that this row does not see get -inf, where any row of the warp needs it
@@ -491,14 +491,13 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           for (int e = 0; e < 32; ++e)
             if (!((bits >> e) & 1)) sc[e] = -INFINITY;
         };
-        auto pass = [&](int c) {  // exponentials relative to the reference, and the maximum beside them
+        auto pass = [&](int c, auto masked) {  // exponentials relative to the reference
           tmem_ld32(s_addr + 32 * c, sr);
           tmem_wait_ld();
-          if (!clear) mask32(c);
+          if (masked.value) mask32(c);
           const float2 shift2 = make_float2(shift, shift);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            top = max3f(top, sc[2 * e], sc[2 * e + 1]);
             const float2 x = __ffma2_rn(make_float2(sc[2 * e], sc[2 * e + 1]), mul2, shift2);
             const float2 y = e % kPolyEvery == kPolyEvery - 1 ? exp2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
             if (e & 1) l1 = __fadd2_rn(l1, y); else l0 = __fadd2_rn(l0, y);
@@ -506,10 +505,17 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           }
         };
         auto passes = [&]() {
-          top = -INFINITY, shift = ref == -INFINITY ? 0.f : -ref;
+          shift = ref == -INFINITY ? 0.f : -ref;
           l0 = l1 = make_float2(0.f, 0.f);
-          if (mine > 0) pass(0);
-          if (mine > 32) pass(1);
+          if (mine > 0) {
+            if (clear) {
+              pass(0, std::false_type{});
+              pass(1, std::false_type{});
+            } else {
+              pass(0, std::true_type{});
+              pass(1, std::true_type{});
+            }
+          }
         };
         passes();
         // V rows behind the sequence may hold anything (0 * NaN is a NaN): they become zeros before this
@@ -524,14 +530,20 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           }
           fence_proxy_async_smem();
         }
-        top *= p.scale_log2;
-        // Does a row of the row tile have to raise its reference?  (At the first tile every row that sees a key.)
-        if (!vote_barrier(1 + i, 256, ok && !(top > ref + kWideRaise))) {
-          tops[half * 128] = top;
+        // Does a row of the row tile have to raise its reference, or does one have none yet (its first tile)?
+        if (!vote_barrier(1 + i, 256, ok && ref != -INFINITY && !((l0.x + l0.y) + (l1.x + l1.y) > kWideRaise))) {
+          float top = -INFINITY;
+          for (int c = 0; c < 2 && mine > 0; ++c) {
+            tmem_ld32(s_addr + 32 * c, sr);
+            tmem_wait_ld();
+            if (!clear) mask32(c);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) top = max3f(top, sc[e], sc[e + 1]);
+          }
+          tops[half * 128] = top * p.scale_log2;
           ok = vote_barrier(1 + i, 256, ok && *abort_flag == 0);
           if (!ok) break;  // the row tile's warps leave together when a wait was abandoned
-          const float most = fmaxf(tops[0], tops[128]);
-          const float now = most > ref + kWideRaise ? most : ref, keep = now == ref ? 1.f : ex2_approx(ref - now);
+          const float now = fmaxf(ref, fmaxf(tops[0], tops[128])), keep = now == ref ? 1.f : ex2_approx(ref - now);
           ref = now;
           l *= keep;
           if (begun) {
@@ -546,12 +558,19 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
               tmem_st16(o_addr + c, o);
             }
           }
-          passes();
+          shift = ref == -INFINITY ? 0.f : -ref;
+          l0 = l1 = make_float2(0.f, 0.f);
+          if (mine > 0) {  // with the mask in any case: one copy of this code
+            pass(0, std::true_type{});
+            pass(1, std::true_type{});
+          }
         }
         begun = true;
         l += (l0.x + l0.y) + (l1.x + l1.y);
-        if (mine > 0) tmem_st16(s_addr, pk);
-        if (mine > 32) tmem_st16(s_addr + 16, pk + 16);
+        if (mine > 0) {
+          tmem_st16(s_addr, pk);
+          tmem_st16(s_addr + 16, pk + 16);
+        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_full(i));

@@ -152,6 +152,18 @@ def test_window_scores_that_keep_growing(q_len, dim, dtype, jump):
     check_window(q, k.flip(2), v, window=300, sinks=70)
 
 
+@pytest.mark.parametrize("q_len", [2, 300])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_window_scores_far_below_zero(q_len, dtype):
+    """Scores of some -300 and less, alone and beside others: 2^score is zero in 32 bits, the softmax is not."""
+    q = normal(1, 2, q_len, 64, dtype=dtype, seed=79).abs() + 1
+    k = -(normal(1, 2, 500, 64, dtype=dtype, seed=80).abs() + 1)
+    v = normal(1, 2, 500, 64, dtype=dtype, seed=81)
+    check_window(q, k, v, window=600, scale=2.0)
+    k[:, :, 200:260] *= 0.1
+    check_window(q, k, v, window=90, sinks=3, scale=2.0)
+
+
 def test_calls_from_two_threads():
     from concurrent.futures import ThreadPoolExecutor
 
