@@ -5,6 +5,8 @@
  * allocation the library ever makes is four bytes of pinned host memory per device, at the
  * first fused-kernel launch on that device (the fault word read by pk_poll_device_fault).
  *
+ * Beside that path: sliding-window attention and a paged K/V cache for serving (second half of the file).
+ *
  * The library replaces, for this one path, the operators that the reference project
  * (Boffee/piper-kernels) registers as
  *   piper_kernels::piper_attention(query, key, value, scale, is_causal, center_value)
