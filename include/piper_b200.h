@@ -243,9 +243,16 @@ typedef struct pk_cache {
   int32_t* uses;
   int32_t* refused;
   int32_t* scratch;
+  const void* maps; /* from pk_cache_maps, or NULL: attention then makes the copy maps it needs itself */
   int32_t device;
   void* stream;
 } pk_cache;
+
+/* Copy maps of keys and values for attention over this cache, into PK_CACHE_MAP_BYTES of host memory aligned
+ * to 64 bytes; valid while keys, values and the sizes stay what they are.  They spare every attention
+ * call the making of its own (some microseconds). */
+#define PK_CACHE_MAP_BYTES 768
+PK_API int pk_cache_maps(const pk_cache* c, void* maps);
 
 /* Room for counts[b] more rows (negative: none) of every sequence: starts = lengths, lengths +=
  * counts.  A partly filled last page that other sequences also name is replaced by a copy; when all

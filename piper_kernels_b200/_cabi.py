@@ -15,6 +15,7 @@ PK_OK = 0
 PK_ERR_BAD_ARG, PK_ERR_UNSUPPORTED_ARCH, PK_ERR_WORKSPACE, PK_ERR_CUDA, PK_ERR_DEVICE_STATUS = 1, 2, 3, 4, 5
 PK_F16, PK_BF16, PK_F32, PK_I8 = 0, 1, 2, 3
 PK_QK_PER_BLOCK, PK_QK_PER_THREAD = 0, 1
+PK_CACHE_MAP_BYTES = 768
 
 EXPORTS = (
     "pk_version", "pk_last_error",
@@ -24,7 +25,7 @@ EXPORTS = (
     "pk_piper_prepare_kv", "pk_piper_prepare_q", "pk_sage2pp_prepare_kv", "pk_sage2pp_prepare_q",
     "pk_poll_device_fault", "pk_debug_stalled_wait",
     "pk_window_workspace_bytes", "pk_window_attention_fwd",
-    "pk_cache_extend", "pk_cache_write", "pk_cache_read", "pk_cache_fork", "pk_cache_truncate", "pk_cache_compact",
+    "pk_cache_maps", "pk_cache_extend", "pk_cache_write", "pk_cache_read", "pk_cache_fork", "pk_cache_truncate", "pk_cache_compact",
     "pk_cache_attention_workspace_bytes", "pk_cache_attention_fwd",
 )
 
@@ -73,7 +74,7 @@ class PkCache(C.Structure):
         ("head_dim", C.c_int32), ("batch", C.c_int32), ("width", C.c_int32), ("dtype", C.c_int32),
         ("keys", C.c_void_p), ("values", C.c_void_p), ("key_scales", C.c_void_p), ("value_scales", C.c_void_p),
         ("table", C.c_void_p), ("lengths", C.c_void_p), ("starts", C.c_void_p), ("uses", C.c_void_p),
-        ("refused", C.c_void_p), ("scratch", C.c_void_p),
+        ("refused", C.c_void_p), ("scratch", C.c_void_p), ("maps", C.c_void_p),
         ("device", C.c_int32), ("stream", C.c_void_p),
     ]
 
@@ -125,6 +126,7 @@ def lib() -> C.CDLL:
         ptr, i32, i64 = C.c_void_p, C.c_int32, C.c_int64
         handle.pk_window_workspace_bytes.argtypes = [W, C.POINTER(C.c_uint64)]
         handle.pk_window_attention_fwd.argtypes = [W]
+        handle.pk_cache_maps.argtypes = [K, ptr]
         handle.pk_cache_extend.argtypes = [K, ptr]
         handle.pk_cache_write.argtypes = [K, i32, ptr, ptr, i64 * 4, i64 * 4, i32, i32]
         handle.pk_cache_read.argtypes = [K, i32, ptr, i32, ptr, ptr, i32]

@@ -77,10 +77,10 @@ def cache_attention(
 
     _ops._require_cuda(query, "cache_attention")
     _ops.poll_device_fault(query.device.index)
-    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
     q = _cabi.PkCacheQuery(heads, tokens, layer, _ops._DTYPE[query.dtype], 0 if window is None else limit, sinks, converted_scale, query.data_ptr(),
                            query.stride()[:3], None if tree is None else tree.data_ptr(), tree_stride, out.data_ptr(), None, 0)
-    c = cache.handle()
+    c = cache.mapped_handle()
     lib = _cabi.lib()
     nbytes = cache.workspaces.get((heads, tokens))
     if nbytes is None:

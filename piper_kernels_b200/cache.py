@@ -17,6 +17,7 @@ import ctypes as C
 import torch
 
 from . import _cabi
+from ._ops import raw_stream
 from .attention._validation import check_lengths, check_rows
 
 _DTYPE = {torch.float16: _cabi.PK_F16, torch.bfloat16: _cabi.PK_BF16, torch.int8: _cabi.PK_I8, torch.float32: _cabi.PK_F32}
@@ -112,6 +113,8 @@ class PageCache:
             if getattr(self, name) is not None:
                 setattr(c, name, getattr(self, name).data_ptr())
         c.refused, c.scratch = self.refused.data_ptr(), self._scratch.data_ptr()
+        c.device = self.device.index or 0
+        self._maps = None  # the pool's copy maps, made at the first attention
 
     @property
     def max_length(self) -> int:
@@ -123,7 +126,18 @@ class PageCache:
         if self.device.type != "cuda":
             raise RuntimeError("PageCache runs only on CUDA tensors (B200, sm_100a); there is no CPU path")
         c = _cabi.PkCache.from_buffer_copy(self._c)
-        c.device, c.stream = self.device.index, torch.cuda.current_stream(self.device).cuda_stream
+        c.stream = raw_stream(c.device)
+        return c
+
+    def mapped_handle(self) -> _cabi.PkCache:
+        """The same with the copy maps of keys and values, which are made once for the cache's life."""
+        c = self.handle()
+        if self._maps is None:
+            maps = C.create_string_buffer(_cabi.PK_CACHE_MAP_BYTES + 64)
+            at = -(-C.addressof(maps) // 64) * 64
+            _cabi.check(_cabi.lib().pk_cache_maps(C.byref(c), at))
+            self._maps = (maps, at)
+        c.maps = self._maps[1]
         return c
 
     def check_layer(self, layer: int) -> int:

@@ -43,7 +43,7 @@ int attend_map(CUtensorMap* m, const AttendParams& p, const void* base, const in
     // the whole pool, so that a page index outside it reads as zeros
     const uint64_t page = row * p.page;
     const uint64_t dims[5] = {static_cast<uint64_t>(line / esz), static_cast<uint64_t>(p.page), static_cast<uint64_t>(lines),
-                              static_cast<uint64_t>(p.kv_heads), static_cast<uint64_t>(p.page_base) + p.pages};
+                              static_cast<uint64_t>(p.kv_heads), static_cast<uint64_t>(p.pool_pages)};
     const uint64_t strides[4] = {row, static_cast<uint64_t>(line), page, page * p.kv_heads};
     return encode_map5(m, base, dims, strides, boxes, line, esz);
   }
@@ -53,6 +53,16 @@ int attend_map(CUtensorMap* m, const AttendParams& p, const void* base, const in
   const uint64_t strides[4] = {stride[2] ? static_cast<uint64_t>(stride[2]) * esz : row, static_cast<uint64_t>(line),
                                stride[1] ? static_cast<uint64_t>(stride[1]) * esz : row, stride[0] ? static_cast<uint64_t>(stride[0]) * esz : row};
   return encode_map5(m, base, dims, strides, boxes, line, esz);
+}
+
+int attend_maps(CUtensorMap* k, CUtensorMap* v, const AttendParams& p, int which, int row_bytes, int esz, int tile, bool whole_rows) {
+  if (p.maps) {
+    *k = p.maps[2 * which], *v = p.maps[2 * which + 1];
+    return PK_OK;
+  }
+  const int line = row_bytes > 128 ? 128 : row_bytes, lines = row_bytes / line, box = p.table && p.page < tile ? p.page : tile;
+  const int rc = attend_map(k, p, p.k, p.k_stride, line, lines, esz, box, whole_rows ? lines : 1);
+  return rc ? rc : attend_map(v, p, p.v, p.v_stride, line, lines, esz, box, whole_rows ? lines : 1);
 }
 
 namespace {
@@ -262,6 +272,23 @@ PK_API int pk_window_attention_fwd(const pk_window_problem* pp) {
   return attend(a, p.head_dim, p.dtype, false, p.device, st);
 }
 
+PK_API int pk_cache_maps(const pk_cache* c, void* maps) {
+  clear_error();
+  int rc = validate_cache(c);
+  if (rc) return rc;
+  if (!maps || (reinterpret_cast<uintptr_t>(maps) & 63)) return fail(PK_ERR_BAD_ARG, "cache maps: the maps need host memory aligned to 64 bytes");
+  static_assert(6 * sizeof(CUtensorMap) == PK_CACHE_MAP_BYTES, "three pairs of maps");
+  AttendParams a{};
+  a.table = c->table, a.page = c->page_size, a.kv_heads = c->kv_heads, a.pool_pages = c->layers * c->pages;
+  a.k = c->keys, a.v = c->values;
+  const int esz = c->dtype == PK_I8 ? 1 : 2;
+  CUtensorMap* m = static_cast<CUtensorMap*>(maps);
+  if ((rc = attend_maps(m, m + 1, a, 0, c->head_dim * esz, esz, 64, true))) return rc;
+  if ((rc = attend_maps(m + 2, m + 3, a, 1, c->head_dim * esz, esz, 128, true))) return rc;
+  if (esz == 1) return PK_OK;  // 8-bit rows have no kernel for many rows
+  return attend_maps(m + 4, m + 5, a, 2, c->head_dim * esz, esz, 128, false);
+}
+
 PK_API int pk_cache_attention_workspace_bytes(const pk_cache* c, const pk_cache_query* q, uint64_t* bytes) {
   clear_error();
   if (!bytes) return fail(PK_ERR_BAD_ARG, "null size pointer");
@@ -292,6 +319,8 @@ PK_API int pk_cache_attention_fwd(const pk_cache* c, const pk_cache_query* q) {
   a.lengths = c->lengths, a.starts = c->starts;
   a.table = c->table, a.width = c->width, a.page = c->page_size, a.pages = c->pages, a.page_base = q->layer * c->pages;
   a.page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
+  a.pool_pages = c->layers * c->pages;
+  a.maps = static_cast<const CUtensorMap*>(c->maps);
   a.k = c->keys, a.v = c->values;
   const int64_t layer_rows = static_cast<int64_t>(c->pages) * c->kv_heads * c->page_size * q->layer;
   if (i8) a.k_scale = c->key_scales + layer_rows, a.v_scale = c->value_scales + layer_rows;

@@ -526,8 +526,7 @@ int launch(AttendParams p, int device, cudaStream_t st) {
   p.key_align = p.table ? (p.page < C::TILE ? p.page : C::TILE) : 8;
   CUtensorMap tk, tv;
   int rc;
-  if ((rc = attend_map(&tk, p, p.k, p.k_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < C::TILE ? p.page : C::TILE) : C::TILE, C::HALVES))) return rc;
-  if ((rc = attend_map(&tv, p, p.v, p.v_stride, C::LINE, C::HALVES, C::ESZ, p.table ? (p.page < C::TILE ? p.page : C::TILE) : C::TILE, C::HALVES))) return rc;
+  if ((rc = attend_maps(&tk, &tv, p, C::TILE == 64 ? 0 : 1, C::ROW_BYTES, C::ESZ, C::TILE, true))) return rc;
   if ((rc = allow_smem<few_rows_kernel<T, I8, D, WM, TREE>>(C::SMEM, device))) return rc;
   // No more CTAs than there can be tiles.
   const int64_t units = static_cast<int64_t>(p.batch) * p.row_blocks * p.kv_heads;

@@ -36,7 +36,7 @@ struct AttendParams {
   const int32_t* starts;   // null (dense): off(b) = offset
   int kv_len, offset;
   const int32_t* table;  // [batch, width] pages; null: dense
-  int width, page, page_shift, pages, page_base;  // page_base: first page of the layer in the pool
+  int width, page, page_shift, pages, page_base, pool_pages;  // page_base: first page of the layer in the pool of pool_pages
   const void* k;
   const void* v;
   int64_t k_stride[3], v_stride[3];  // dense
@@ -53,6 +53,7 @@ struct AttendParams {
   struct Pieces* pieces;  // per unit
   int workers, first_unit;
   int32_t* host_status;  // pinned word that takes the site of an abandoned wait
+  const CUtensorMap* maps;  // host: K and V maps for 64- and 128-key tiles of few rows and for many rows, or null
 };
 
 // Token of a row (its query head within the group is the remainder).
@@ -459,6 +460,8 @@ __global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_const
 // `box_lines` lines.
 // `stride`: dense element strides (batch, head, key); paged caches are contiguous.
 int attend_map(CUtensorMap* m, const AttendParams& p, const void* base, const int64_t* stride, int line, int lines, int esz, int box, int box_lines);
+// Maps of K and V for tiles of `tile` keys: the prepared ones (number `which`), or new ones.
+int attend_maps(CUtensorMap* k, CUtensorMap* v, const AttendParams& p, int which, int row_bytes, int esz, int tile, bool whole_rows);
 
 // few_rows.cuh
 int launch_few_rows_f16(const AttendParams& p, int head_dim, bool i8, int device, cudaStream_t st);

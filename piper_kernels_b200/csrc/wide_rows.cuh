@@ -687,9 +687,7 @@ int launch_wide(AttendParams p, int device, cudaStream_t st) {
   p.key_align = p.table ? (p.page < kWideTile ? p.page : kWideTile) : 8;
   CUtensorMap tk, tv;
   int rc;
-  const int box = p.table ? (p.page < kWideTile ? p.page : kWideTile) : kWideTile, lines = p.table ? 1 : D / 64;
-  if ((rc = attend_map(&tk, p, p.k, p.k_stride, 128, D / 64, 2, box, lines))) return rc;
-  if ((rc = attend_map(&tv, p, p.v, p.v_stride, 128, D / 64, 2, box, lines))) return rc;
+  if ((rc = attend_maps(&tk, &tv, p, 2, D * 2, 2, kWideTile, !p.table))) return rc;
   if ((rc = allow_smem<wide_rows_kernel<T, D, TREE>>(C::SMEM, device))) return rc;
   const WidePlan plan = wide_plan(p.batch, p.kv_heads, p.rows);
   const int64_t most = plan.units * (((p.table ? p.width * p.page : p.kv_len) + kWideTile - 1) / kWideTile + 2);

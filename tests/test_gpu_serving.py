@@ -733,6 +733,28 @@ def test_page_work_of_a_large_batch():
     assert state(cache) == listed(model)
 
 
+@pytest.mark.parametrize("store", [F16, torch.int8])
+@pytest.mark.parametrize("tokens", [1, 9, 64])
+def test_prepared_copy_maps_change_nothing(store, tokens):
+    import ctypes as C
+
+    from piper_kernels_b200 import _cabi
+
+    cache = filled(2, 60, 32, 2, 128, store, [300, 64 + tokens], [tokens, tokens], layers=2, seed=33)
+    q = normal(2, 8, tokens, 128, dtype=F16, seed=64)
+    want = pk.cache_attention(q, cache, layer=1)
+    out = torch.empty_like(want)
+    c = cache.handle()  # without maps
+    assert not c.maps and cache.mapped_handle().maps
+    query = _cabi.PkCacheQuery(8, tokens, 1, _cabi.PK_F16, 0, 0, 128**-0.5, q.data_ptr(), q.stride()[:3], None, 0, out.data_ptr(), None, 0)
+    n = C.c_uint64()
+    _cabi.check(_cabi.lib().pk_cache_attention_workspace_bytes(C.byref(c), C.byref(query), C.byref(n)))
+    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    query.workspace, query.workspace_bytes = ws.data_ptr(), n.value
+    _cabi.check(_cabi.lib().pk_cache_attention_fwd(C.byref(c), C.byref(query)))
+    assert torch.equal(out, want)
+
+
 def test_two_streams_on_two_caches():
     caches = [filled(4, 100, 16, 2, 64, F16, [300, 20, 100, 7], [1] * 4, seed=20 + i) for i in range(2)]
     q = normal(4, 4, 1, 64, dtype=F16, seed=63)

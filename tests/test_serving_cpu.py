@@ -210,6 +210,7 @@ def test_cache_entries_refuse_before_the_device():
         assert lib.pk_cache_truncate(c, 256) == lib.pk_cache_fork(c, 256) == lib.pk_cache_compact(c, 256, 4, 4, 256) == _cabi.PK_ERR_BAD_ARG
         assert lib.pk_cache_write(c, 0, 256, 256, strides, strides, _cabi.PK_F16, 3) == lib.pk_cache_read(c, 0, 256, 3, 256, 256, _cabi.PK_F16) == _cabi.PK_ERR_BAD_ARG
     assert lib.pk_cache_extend(None, 256) == _cabi.PK_ERR_BAD_ARG
+    assert lib.pk_cache_maps(C.byref(c_cache(page_size=8)), 64) == lib.pk_cache_maps(C.byref(c_cache()), None) == lib.pk_cache_maps(C.byref(c_cache()), 72) == _cabi.PK_ERR_BAD_ARG
     query = _cabi.PkCacheQuery()
 
     def ask(cache=None, **over):
