@@ -27,7 +27,8 @@ def window_attention(
     ``i`` stands at position ``p = i + kv_len - q_len`` and sees key ``j`` when ``j <= p`` and either
     ``p - j < window`` or ``j < sinks``.  ``lengths`` (int32 ``[batch]``) says how many keys of each batch
     element exist (a right-padded batch); keys behind them are never looked at.  Rows that see no key and
-    rows at or behind their length are zero.  ``scale`` defaults to ``head_dim**-0.5``.  Inference only.
+    rows at or behind their length are zero.  ``scale`` defaults to ``head_dim**-0.5``.  Can be captured in a CUDA
+    graph once it has run on the device outside of one.  Inference only.
     """
     for name, tensor in (("query", query), ("key", key), ("value", value)):
         check_rows(_OP, name, tensor)

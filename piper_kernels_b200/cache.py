@@ -30,7 +30,8 @@ _STRIDES = C.c_int64 * 4
 class PageCache:
     """Keys and values of ``batch`` sequences in pages of ``page_size`` rows, for all layers of a model.
 
-    All state is in plain tensors, which a program may read, save and restore:
+    All state is in plain tensors, which a program may read, save, and restore in place (``copy_``; their
+    addresses are kept):
 
     ``keys``, ``values``              ``[layers, pages, kv_heads, page_size, head_dim]`` in ``dtype``
     ``key_scales``, ``value_scales``  ``[layers, pages, kv_heads, page_size]`` float32 for ``dtype=torch.int8`` (a
@@ -42,7 +43,8 @@ class PageCache:
                                       alone because it could not be done
 
     Calls run on the current stream of the cache's device.  They change the cache in place, so calls on
-    one cache from several streams need the caller's events between them.
+    one cache from several streams need the caller's events between them.  They can be captured in a CUDA
+    graph once :func:`cache_attention` has run on the device outside of one.
     """
 
     def __init__(self, batch: int, pages: int, page_size: int, kv_heads: int, head_dim: int, *, max_length: int | None = None,
