@@ -539,6 +539,9 @@ int launch(AttendParams p, int device, cudaStream_t st) {
   cudaError_t e = launch_chained(few_rows_kernel<T, I8, D, WM, TREE>, dim3(p.workers), dim3(kThreads), C::SMEM, st, tk, tv, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "attention kernel launch failed: %s", cuda_err(e));
+  // Units of one tile are never split.
+  const int keys = p.table ? p.width * p.page : p.kv_len;
+  if (keys <= C::TILE && (p.sinks == 0 || p.window >= keys)) return PK_OK;
   e = launch_chained(join_kernel<T, I8, D, TREE, C::TILE, C::ROWS>, dim3(static_cast<unsigned>(units) * (C::ROWS / kJoinRows)), dim3(32 * kJoinRows), 0, st, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "join kernel launch failed: %s", cuda_err(e));

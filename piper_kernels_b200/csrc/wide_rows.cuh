@@ -667,16 +667,22 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (tid == 0 && *abort_flag != 0 && p.host_status != nullptr) atomicCAS_system(p.host_status, 0, *abort_flag);
 }
 
-// Whole rounds of units over the CTAs are worked on unit by unit; what is left over (in groups: all key
-// heads of some rows) is shared out by tiles, or nothing is, when there are so many rounds that the last,
-// partial one hardly counts.
+// Whole rounds of units over the CTAs are worked on unit by unit.  What is left over (in groups: all key
+// heads of some rows) is shared out by tiles where that shortens the last round by more than the sharing
+// costs: starting, leaving pieces and joining them takes about as long as six key tiles (12 us).
 struct WidePlan {
   int64_t units, whole;
 };
-inline WidePlan wide_plan(int batch, int kv_heads, int rows) {
-  const int64_t units = static_cast<int64_t>(batch) * kv_heads * ((rows + kWideRows - 1) / kWideRows);
-  if (units >= kWideShareBelow) return {units, units};
-  return {units, units / kWideWorkers * kWideWorkers / kv_heads * kv_heads};
+inline WidePlan wide_plan(int batch, int kv_heads, int rows, int tiles) {
+  const int64_t units = static_cast<int64_t>(batch) * kv_heads * ((rows + kWideRows - 1) / kWideRows), left = units % kWideWorkers;
+  if (units >= kWideShareBelow || (kWideWorkers - left) * tiles <= 6 * kWideWorkers) return {units, units};
+  return {units, (units - left) / kv_heads * kv_heads};
+}
+// Key tiles of a unit, at most.
+inline int wide_tiles(const AttendParams& p) {
+  const int keys = p.table ? p.width * p.page : p.kv_len, span = kWideRows / p.group + 1;
+  const int seen = p.window < keys - span ? p.window + span : keys, sinks = p.window < keys ? (p.sinks < keys ? p.sinks : keys) : 0;
+  return (seen + kWideTile - 1) / kWideTile + (sinks + kWideTile - 1) / kWideTile;
 }
 
 template <typename T, int D, bool TREE>
@@ -689,7 +695,7 @@ int launch_wide(AttendParams p, int device, cudaStream_t st) {
   int rc;
   if ((rc = attend_maps(&tk, &tv, p, 2, D * 2, 2, kWideTile, !p.table))) return rc;
   if ((rc = allow_smem<wide_rows_kernel<T, D, TREE>>(C::SMEM, device))) return rc;
-  const WidePlan plan = wide_plan(p.batch, p.kv_heads, p.rows);
+  const WidePlan plan = wide_plan(p.batch, p.kv_heads, p.rows, wide_tiles(p));
   const int64_t most = plan.units * (((p.table ? p.width * p.page : p.kv_len) + kWideTile - 1) / kWideTile + 2);
   if (most >= (1ll << 31)) return fail(PK_ERR_BAD_ARG, "attention: too many keys and rows for one call; split it over the batch");
   p.first_unit = static_cast<int>(plan.whole);
