@@ -11,6 +11,7 @@
 //     about them is known to the host).  The ring runs on across the borders between sequences.
 //   - A sequence that several CTAs share leaves pieces (un-normalised rows, maximum, sum) in the
 //     workspace; a second small kernel joins them.
+//   - Few and short units get a cluster of CTAs each, which joins its own pieces (`cluster_of`).
 // The products use mma.sync: at up to 64 query rows the tensor work is far below the time of the
 // copies, and its fragments can be filled straight from the rows as they lie in memory.  The
 // contraction may visit features and keys in any order, as long as both operands use the same:
@@ -25,8 +26,7 @@
 // Measured: 64 single tokens (32 / 8 heads of 128 features) over 1088 to 8192 bfloat16 rows, 1.22 GB: 195 us,
 // 6.3 TB/s (0.96 of the measured copy).  48 tokens (40 / 8 heads) over 8-bit rows, window 4096, 417 MB: 126 us,
 // 3.3 TB/s: there the conversions to 16 bits (about 170 of 560 instructions for 16 keys of a warp) and the
-// latency of two warps per scheduler bound it, not memory.  One token over 1000 rows: 6.6 us and 5.8 us
-// for the join.
+// latency of two warps per scheduler bound it, not memory.  One token over 1000 rows: 9.2 us.
 
 #pragma once
 
@@ -41,6 +41,8 @@ constexpr int kThreads = kConsumers + 32;
 constexpr int kJoinCols = 32;          // output columns that the warps of a CTA join at a time
 constexpr float kRaise = 8.f;          // a row's reference exponent follows its maximum only beyond this
 constexpr int kMaxWorkers = 2 * 148;   // two CTAs per SM
+constexpr int kClusterWorkers = 256;   // CTAs of clusters that the SMs hold at once, two on each
+constexpr int kClusterTiles = 12;      // tiles of a CTA, at most, for a unit to be worked on by a cluster of its own
 
 template <typename T, bool I8, int D, int WM>
 struct Few {
@@ -109,10 +111,8 @@ __device__ __forceinline__ float rcp_approx(float x) {
 }
 
 template <typename T, bool I8, int D, int WM, bool TREE>
-__global__ void __launch_bounds__(kThreads, 2)
-few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttendParams p) {
+__device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttendParams& p, uint8_t* smem) {
   using C = Few<T, I8, D, WM>;
-  extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   uint32_t* red = reinterpret_cast<uint32_t*>(smem + C::OFF_RED);
   Found* found = reinterpret_cast<Found*>(smem + C::OFF_RED + 32);
@@ -130,13 +130,21 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   cudaGridDependencySynchronize();
   __syncthreads();
 
-  const int groups = p.batch * p.row_blocks;
-  const uint32_t total = sum_tiles<TREE, C::TILE, C::ROWS>(p, 0, groups, red);
-  const uint32_t w0 = share_begin(total, gridDim.x, blockIdx.x), w1 = share_begin(total, gridDim.x, blockIdx.x + 1);
-  if (w0 >= w1) return;
-  const Found f = find_group<TREE, C::TILE, C::ROWS>(p, 0, w0, red, found);
   Walk<TREE, C::TILE, C::ROWS> walk;
-  walk.start(p, f, w0);
+  uint32_t total = 0, w0, w1;
+  if (p.cluster) {  // an equal share of the cluster's unit
+    const uint32_t unit = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster;
+    walk.g = unit / p.kv_heads, walk.h = unit % p.kv_heads;
+    walk.s = span_of<TREE, C::TILE, C::ROWS>(p, walk.g);
+    w0 = share_begin(walk.s.n, p.cluster, rank), w1 = share_begin(walk.s.n, p.cluster, rank + 1);
+    walk.tile = w0;
+    if (w0 >= w1) return;
+  } else {
+    total = sum_tiles<TREE, C::TILE, C::ROWS>(p, 0, p.batch * p.row_blocks, red);
+    w0 = share_begin(total, gridDim.x, blockIdx.x), w1 = share_begin(total, gridDim.x, blockIdx.x + 1);
+    if (w0 >= w1) return;
+    walk.start(p, find_group<TREE, C::TILE, C::ROWS>(p, 0, w0, red, found), w0);
+  }
 
   if (warp == kConsumers / 32) {
     // ---------------------------------------------------------------- producer
@@ -421,7 +429,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 
     // -------- join the warps that shared the unit's keys; write rows, or a piece for the join kernel
     const bool whole = unit_from == 0 && unit_tiles == s.n;
-    if (unit_from == 0 && tid == 0) {
+    if (unit_from == 0 && tid == 0 && !p.cluster) {
       const uint32_t u0 = w - unit_tiles;  // (after an abandoned wait the pieces do not matter)
       const int last = whole ? static_cast<int>(blockIdx.x) : static_cast<int>(owner_of(total, gridDim.x, u0 + s.n - 1));
       p.pieces[walk.g * p.kv_heads + h] = Pieces{static_cast<int>(blockIdx.x), last, u0 != w0, 0};
@@ -434,7 +442,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       if (c4 == 0) ml[warp * 16 + g8 + 8 * x] = make_float2(m[x], l[x]);
     }
     ok = vote_barrier(1, kConsumers, ok && *abort_flag == 0);  // the same answer in every warp: they leave together
-    const int slot = blockIdx.x * 2 + (unit_from == 0 && w - unit_tiles != w0 ? 1 : 0);
+    const int slot = blockIdx.x * 2 + (unit_from == 0 && w - unit_tiles != w0 && !p.cluster ? 1 : 0);
     float* piece = p.partial + static_cast<int64_t>(slot) * C::ROWS * (D + 4);
     // thread -> (row, four consecutive columns) of the CTA's rows; a row's columns belong to 8 neighbouring threads
     bool bad[WM];
@@ -515,9 +523,51 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   if (tid == 0 && *abort_flag != 0 && p.host_status != nullptr) atomicCAS_system(p.host_status, 0, *abort_flag);
 }
 
+template <typename T, bool I8, int D, int WM, bool TREE>
+__device__ __noinline__ void join_cluster(const AttendParams& p, TreeMasks* tm) {
+  using C = Few<T, I8, D, WM>;
+  const int rank = blockIdx.x % p.cluster, first = blockIdx.x - rank, unit = blockIdx.x / p.cluster, g = unit / p.kv_heads;
+  const int pieces = min(span_of<TREE, C::TILE, C::ROWS>(p, g).n, p.cluster), warps = kThreads / 32;
+  if (pieces < 2) return;
+  for (int r = rank * warps + (threadIdx.x >> 5); r < C::ROWS; r += p.cluster * warps)
+    join_row<T, I8, D, TREE, C::ROWS>(p, Pieces{first, first + pieces - 1, 0, 0}, g, unit - g * p.kv_heads, r, tm);
+}
+
+template <typename T, bool I8, int D, int WM, bool TREE>
+__global__ void __launch_bounds__(kThreads, 2)
+few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttendParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  attend_share<T, I8, D, WM, TREE>(tm_k, tm_v, p, smem);
+  if (p.cluster < 2) return;
+  // every thread of the cluster comes here, on every path; the barrier makes the pieces visible to all of them
+  __syncwarp();
+  cluster_barrier();
+  join_cluster<T, I8, D, WM, TREE>(p, reinterpret_cast<TreeMasks*>(smem + Few<T, I8, D, WM>::OFF_TREE));
+}
+
 // ---------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------
+// Key tiles of a unit, at most.
+inline int64_t few_tiles(const AttendParams& p, int tile, int rows) {
+  const int64_t keys = p.table ? static_cast<int64_t>(p.width) * p.page : p.kv_len, span = p.tree ? p.tokens : rows / p.group + 1;
+  const int64_t seen = p.window < keys - span ? p.window + span + p.key_align : keys, sinks = p.window < keys ? (p.sinks < keys ? p.sinks : keys) : 0;
+  return (seen + tile - 1) / tile + (sinks + tile - 1) / tile;
+}
+// CTAs of the cluster that works on one unit and joins its pieces, or 0 to share all tiles out and join in a
+// second kernel.  A cluster saves that kernel and finding the shares, and leaves few pieces, but its unit may be
+// the longest by far and its CTAs copy 32 KB in 0.8 us (16 rows; 1.5 us at 32 rows, 2.6 us at 64) when few
+// others do; the limit keeps that to some 10 us.  Clusters have enough warps to join all rows at once;
+// 16 CTAs take about 1 us more to start than eight.  Cluster against shares, microseconds, 32 / 8 heads of 128
+// features, bfloat16: one token over 1024, 4096 and 16384 rows 8.9 / 11.4, 12.5 / 22.4, 24.0 / 25.2; 16 tokens
+// alike (a sequence each) 15.9 / 18.9, 48.7 / 53.4, 161 / 179; 16 tokens of one sequence (64 rows) 15.9 / 16.7,
+// 26.2 / 31.4, 65 / 49.
+inline int cluster_of(int64_t units, int64_t tiles, int rows) {
+  int n = tiles > 1 ? 16 : 1;
+  while (n > 1 && (units * n > kClusterWorkers || ((n == 16 ? 2 * n : n / 2) >= tiles && n / 2 * (kThreads / 32) >= rows))) n /= 2;
+  return units * n <= kMaxWorkers && tiles * rows <= static_cast<int64_t>(16 * kClusterTiles) * n ? n : 0;
+}
+
 template <typename T, bool I8, int D, int WM, bool TREE>
 int launch(AttendParams p, int device, cudaStream_t st) {
   using C = Few<T, I8, D, WM>;
@@ -527,21 +577,21 @@ int launch(AttendParams p, int device, cudaStream_t st) {
   CUtensorMap tk, tv;
   int rc;
   if ((rc = attend_maps(&tk, &tv, p, C::TILE == 64 ? 0 : 1, C::ROW_BYTES, C::ESZ, C::TILE, true))) return rc;
-  if ((rc = allow_smem<few_rows_kernel<T, I8, D, WM, TREE>>(C::SMEM, device))) return rc;
+  if ((rc = allow_smem<few_rows_kernel<T, I8, D, WM, TREE>, true>(C::SMEM, device))) return rc;
   // No more CTAs than there can be tiles.
   const int64_t units = static_cast<int64_t>(p.batch) * p.row_blocks * p.kv_heads;
   const int64_t most = units * (((p.table ? p.width * p.page : p.kv_len) + C::TILE - 1) / C::TILE + 2);
   if (most >= (1ll << 31)) return fail(PK_ERR_BAD_ARG, "attention: too many keys and rows for one call; split it over the batch");
   p.workers = static_cast<int>(most < kMaxWorkers ? most : kMaxWorkers);
+  p.cluster = cluster_of(units, few_tiles(p, C::TILE, C::ROWS), C::ROWS);
+  if (p.cluster) p.workers = static_cast<int>(units) * p.cluster;
   p.first_unit = 0;
   p.pieces = reinterpret_cast<Pieces*>(p.partial);
   p.partial += (units * (sizeof(Pieces) / sizeof(float)) + 63) / 64 * 64;
-  cudaError_t e = launch_chained(few_rows_kernel<T, I8, D, WM, TREE>, dim3(p.workers), dim3(kThreads), C::SMEM, st, tk, tv, p);
+  cudaError_t e = launch_clusters(p.cluster ? p.cluster : 1, few_rows_kernel<T, I8, D, WM, TREE>, dim3(p.workers), dim3(kThreads), C::SMEM, st, tk, tv, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "attention kernel launch failed: %s", cuda_err(e));
-  // Units of one tile are never split.
-  const int keys = p.table ? p.width * p.page : p.kv_len;
-  if (keys <= C::TILE && (p.sinks == 0 || p.window >= keys)) return PK_OK;
+  if (p.cluster) return PK_OK;
   e = launch_chained(join_kernel<T, I8, D, TREE, C::TILE, C::ROWS>, dim3(static_cast<unsigned>(units) * (C::ROWS / kJoinRows)), dim3(32 * kJoinRows), 0, st, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "join kernel launch failed: %s", cuda_err(e));

@@ -52,6 +52,7 @@ struct AttendParams {
   float* partial;
   struct Pieces* pieces;  // per unit
   int workers, first_unit;
+  int cluster;  // few rows: CTAs that share one unit and join its pieces themselves, or 0
   int32_t* host_status;  // pinned word that takes the site of an abandoned wait
   const CUtensorMap* maps;  // host: K and V maps for 64- and 128-key tiles of few rows and for many rows, or null
 };
@@ -123,6 +124,11 @@ __device__ __forceinline__ void build_tree(const AttendParams& p, int b, int off
     tm->sees[t] = keep;
   }
   __syncwarp();
+}
+
+// Barrier of all threads of a cluster; what they wrote before it, they all read after it.
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // Barrier `id` of `threads` threads; true when `good` holds in all of them.
@@ -390,21 +396,13 @@ struct Walk {  // position in the list of tiles
   __device__ __forceinline__ int key() const { return key_of_tile<TILE>(s, tile); }
 };
 
-// Joins the pieces of every unit that more than one CTA worked on: a warp per row, its pieces' weights
-// first (a lane per piece), then their numerators, several loads in flight.
-constexpr int kJoinRows = 4;
-
-template <typename T, bool I8, int D, bool TREE, int TILE, int ROWS>
-__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ AttendParams p) {
-  __shared__ TreeMasks tm;
-  constexpr int E = D / 32, BLOCKS = ROWS / kJoinRows;
-  const int unit = p.first_unit + blockIdx.x / BLOCKS, g = unit / p.kv_heads, h = unit - g * p.kv_heads;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x % BLOCKS * kJoinRows + warp;
-  const int row = g % p.row_blocks * ROWS + r;
-  cudaGridDependencySynchronize();
-  const Pieces at = p.pieces[unit];
-  if (at.c0 == at.c1 || row >= p.rows) return;  // the same for the warp; no barrier follows
-  if (at.c0 < 0 || at.c1 < at.c0 || at.c1 >= p.workers) return;  // never written: a wait was abandoned
+// Joins the pieces of row r of a unit (group g, key head h): a warp per row, its pieces' weights first (a
+// lane per piece), then their numerators, several loads in flight.
+template <typename T, bool I8, int D, bool TREE, int ROWS>
+__device__ __forceinline__ void join_row(const AttendParams& p, const Pieces at, int g, int h, int r, TreeMasks* tm) {
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31, row = g % p.row_blocks * ROWS + r;
+  if (row >= p.rows) return;  // the same for the warp
   // (a piece's slot) * ROWS + r, in rows of D + 4 words
   auto slot = [&](int c) { return (static_cast<int64_t>(2 * c + (c == at.c0 ? at.late : 0)) * ROWS + r) * (D + 4); };
   float mx = -INFINITY, sum = 0.f, acc[E];
@@ -452,8 +450,22 @@ __global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_const
   }
   __syncwarp();
   if (!__any_sync(0xffffffffu, bad)) return;
-  if (TREE) build_tree(p, b, off, lane, &tm);  // warps of one CTA write the same values
-  plain_row<T, I8, D>(p, b, h, row, off, len, row_view(p, off, len, t, TREE ? &tm : nullptr), TREE);
+  if (TREE) build_tree(p, b, off, lane, tm);  // warps of one CTA write the same values
+  plain_row<T, I8, D>(p, b, h, row, off, len, row_view(p, off, len, t, TREE ? tm : nullptr), TREE);
+}
+
+// Joins the pieces of every unit that more than one CTA worked on.
+constexpr int kJoinRows = 4;
+
+template <typename T, bool I8, int D, bool TREE, int TILE, int ROWS>
+__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ AttendParams p) {
+  __shared__ TreeMasks tm;
+  constexpr int BLOCKS = ROWS / kJoinRows;
+  const int unit = p.first_unit + blockIdx.x / BLOCKS, g = unit / p.kv_heads;
+  cudaGridDependencySynchronize();
+  const Pieces at = p.pieces[unit];
+  if (at.c0 == at.c1 || at.c0 < 0 || at.c1 < at.c0 || at.c1 >= p.workers) return;  // one CTA's; never written (a wait was abandoned)
+  join_row<T, I8, D, TREE, ROWS>(p, at, g, unit - g * p.kv_heads, blockIdx.x % BLOCKS * kJoinRows + (threadIdx.x >> 5), &tm);
 }
 
 // Copy map of K or V: [line, key, lines of a row, head, batch element or page], boxes of `box` keys and

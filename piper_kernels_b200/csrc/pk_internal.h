@@ -73,13 +73,14 @@ int32_t* fault_word_device_ptr(int device);
 int launch_fused(const pk_problem& p, const Layout& L, Algo algo, cudaStream_t stream,
                  const DebugDump* dump);
 
-// Lets a kernel use `bytes` of dynamic shared memory on `device` (set once per kernel and device).
-template <auto KERNEL>
+// Lets a kernel use `bytes` of dynamic shared memory, and clusters of 16 CTAs, on `device` (set once per kernel and device).
+template <auto KERNEL, bool CLUSTERS_OF_16 = false>
 int allow_smem(int bytes, int device) {
   static std::atomic<bool> done[64];
   const int dev = (device >= 0 && device < 64) ? device : 0;
   if (done[dev].load(std::memory_order_acquire)) return PK_OK;
-  const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && CLUSTERS_OF_16) e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return fail(PK_ERR_CUDA, "cudaFuncSetAttribute: %s", cuda_err(e));
   done[dev].store(true, std::memory_order_release);
   return PK_OK;
@@ -116,20 +117,29 @@ inline T* at(const pk_problem& p, size_t off) {
 // library's back-to-back kernels (a call is eight launches; small problems are bound by them).
 // Every kernel launched this way calls cudaGridDependencySynchronize() before it touches memory:
 // that returns once the predecessor has completed and its writes are visible.
+// `cluster` CTAs along x form a cluster (1: none).
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                                  Args&&... args) {
+inline cudaError_t launch_clusters(int cluster, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                                   Args&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(std::forward<Args>(args))...);
+}
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                                  Args&&... args) {
+  return launch_clusters(1, kernel, grid, block, smem, st, std::forward<Args>(args)...);
 }
 #endif
 

@@ -426,6 +426,37 @@ def test_cached_one_long_sequence_beside_short_ones():
     check_cached(q, cache, window=4096, sinks=4)
 
 
+@pytest.mark.parametrize("dim,dtype,store", [(128, BF16, BF16), (64, F16, torch.int8)])
+@pytest.mark.parametrize("batch,heads,kv_heads,tokens", [(3, 8, 2, 1), (3, 3, 3, 20), (3, 4, 2, 32), (40, 8, 8, 1), (60, 3, 3, 2)])
+@pytest.mark.parametrize("room", [None, 40000])
+def test_cached_units_of_one_cluster_and_shared_by_all(dim, dtype, store, batch, heads, kv_heads, tokens, room):
+    """The same sequences where each could be long (tiles are shared by all CTAs) and where none is (clusters of
+    16 to one CTAs, by the number of sequences), chains and trees."""
+    rng = random.Random(batch + tokens)
+    lengths = [(tokens, 1500, 700)[b % 3] if batch < 4 else tokens + rng.randrange(200) for b in range(batch)]
+    cache = filled(batch, sum(-(-n // 16) for n in lengths), 16, kv_heads, dim, store, lengths, [tokens] * batch, seed=tokens, max_length=room)
+    q = normal(batch, heads, tokens, dim, dtype=dtype, seed=83)
+    check_cached(q, cache)
+    check_cached(q, cache, window=130, sinks=9)
+    check_cached(q, cache, tree=some_tree(tokens, rng))
+
+
+@pytest.mark.parametrize("store", [F16, torch.int8])
+@pytest.mark.parametrize("room", [None, 40000])
+def test_cached_rows_that_are_not_finite_in_pieces(store, room):
+    """A row that one token of a tree sees and others do not, in one of many pieces of a sequence."""
+    cache = filled(2, 200, 16, 2, 64, store, [1400, 33], [3, 3], seed=5, max_length=room)
+    q = normal(2, 6, 3, 64, dtype=F16, seed=84)
+    tree = [-1, 0, 0]
+    want = check_cached(q, cache, tree=tree)
+    values = cache.value_scales if store is torch.int8 else cache.values
+    values[0, cache.table[0, 1399 // 16], :, 1399 % 16] = float("nan")
+    got = pk.cache_attention(q, cache, tree=torch.tensor(tree, dtype=torch.int32, device="cuda"))
+    assert got[0, :, 2].isnan().all() and torch.equal(got[1], want[1]) and not got[0, :, :2].isnan().any()
+    off = torch.finfo(F16).eps * 2
+    assert ((got - want)[0, :, :2].abs() <= off * want[0, :, :2].abs() + 1e-3).all()
+
+
 def test_cached_many_sequences():
     lengths = [1 + 7 * i % 90 for i in range(500)]
     cache = filled(500, 4000, 16, 1, 64, F16, lengths, [1] * 500, seed=12)
