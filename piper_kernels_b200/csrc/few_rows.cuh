@@ -23,8 +23,8 @@
 // gets p / scale (the way the 8-bit attention of fused_attention.cu treats its key scales), so that
 // p stays in the range of a 16-bit float whatever the scales are.  p is rounded to the query's
 // 16-bit type for the product; maxima, sums and accumulators are 32-bit.
-// Measured: 64 single tokens (32 / 8 heads of 128 features) over 1088 to 8192 bfloat16 rows, 1.22 GB: 195 us,
-// 6.3 TB/s (0.96 of the measured copy).  48 tokens (40 / 8 heads) over 8-bit rows, window 4096, 417 MB: 126 us,
+// Measured: 64 single tokens (32 / 8 heads of 128 features) over 1088 to 8192 bfloat16 rows, 1.22 GB: 197 us,
+// 6.2 TB/s (0.95 of the measured copy).  48 tokens (40 / 8 heads) over 8-bit rows, window 4096, 417 MB: 126 us,
 // 3.3 TB/s: there the conversions to 16 bits (about 170 of 560 instructions for 16 keys of a warp) and the
 // latency of two warps per scheduler bound it, not memory.  One token over 1000 rows: 9.2 us.
 

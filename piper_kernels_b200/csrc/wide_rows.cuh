@@ -22,8 +22,8 @@
 //   - Tiles that every row sees whole take a path without branches.
 //   - A few of the exponentials are evaluated on the FMA pipe beside the exponential unit.
 // Measured: 4 prompts of 8192 tokens, 32 query and 8 key heads of 128 features, window 1024, float16:
-// 698 us, 741 TFLOP/s of visible pairs (0.45 of the measured 1652); the last 2048 tokens of 32760, 40 / 8
-// heads, window 4096, bfloat16: 180 us, 970 TFLOP/s (0.59).  A tile's chain takes some 3600 cycles where the two
+// 697 us, 743 TFLOP/s of visible pairs (0.45 of the measured 1652); the last 2048 tokens of 32760, 40 / 8
+// heads, window 4096, bfloat16: 182 us, 957 TFLOP/s (0.58).  A tile's chain takes some 3600 cycles where the two
 // row tiles' products fill 2048; two thirds of it are in the softmax, most of that latency (taking the
 // exponentials out altogether makes the kernel 6 % faster), the rest in the products and the hand-overs.
 // A unit's query rows in, first scores and rows out take about 9000 cycles, partly beside the other row tile.
