@@ -41,8 +41,8 @@ constexpr int kThreads = kConsumers + 32;
 constexpr int kJoinCols = 32;          // output columns that the warps of a CTA join at a time
 constexpr float kRaise = 8.f;          // a row's reference exponent follows its maximum only beyond this
 constexpr int kMaxWorkers = 2 * 148;   // two CTAs per SM
-constexpr int kClusterWorkers = 256;   // CTAs of clusters that the SMs hold at once, two on each
-constexpr int kClusterTiles = 12;      // tiles of a CTA, at most, for a unit to be worked on by a cluster of its own
+constexpr int kClusterWorkers = 256;   // CTAs of clusters of eight that the SMs hold at once
+constexpr int kClusterTiles = 12;      // tiles of 16 rows for a CTA, at most, for a unit to get a cluster of its own
 
 template <typename T, bool I8, int D, int WM>
 struct Few {
@@ -557,15 +557,19 @@ inline int64_t few_tiles(const AttendParams& p, int tile, int rows) {
 // CTAs of the cluster that works on one unit and joins its pieces, or 0 to share all tiles out and join in a
 // second kernel.  A cluster saves that kernel and finding the shares, and leaves few pieces, but its unit may be
 // the longest by far and its CTAs copy 32 KB in 0.8 us (16 rows; 1.5 us at 32 rows, 2.6 us at 64) when few
-// others do; the limit keeps that to some 10 us.  Clusters have enough warps to join all rows at once;
-// 16 CTAs take about 1 us more to start than eight.  Cluster against shares, microseconds, 32 / 8 heads of 128
-// features, bfloat16: one token over 1024, 4096 and 16384 rows 8.9 / 11.4, 12.5 / 22.4, 24.0 / 25.2; 16 tokens
-// alike (a sequence each) 15.9 / 18.9, 48.7 / 53.4, 161 / 179; 16 tokens of one sequence (64 rows) 15.9 / 16.7,
-// 26.2 / 31.4, 65 / 49.
+// others do; the limit keeps that to some 10 us.  Above 16 rows it has warps enough to join all rows at once
+// (16 tokens of 4 sequences, 64 rows, over 256: 18.8 us with eight CTAs each, 15.6 us shared); 16 CTAs take about
+// 1 us more to start than eight, and only some eight such clusters are held at once (two sequences: 25 us).
+// Cluster against shares, microseconds, 32 / 8 heads of 128 features, bfloat16: one token over 1024, 4096 and
+// 16384 rows 8.9 / 11.4, 12.5 / 22.4, 24.0 / 25.2; 16 single tokens over 256, 512 and 1024 rows 10.4 / 11.9,
+// 12.0 / 14.9, 15.9 / 18.9, over 128 to 1024 rows 15.3 / 19.0, one over 1024 beside 15 over 128 14.3 / 11.8;
+// 16 tokens of one sequence (64 rows) over 1024 and 4096 rows 15.9 / 16.7, 26.2 / 31.4.
 inline int cluster_of(int64_t units, int64_t tiles, int rows) {
+  constexpr int WARPS = kThreads / 32;
   int n = tiles > 1 ? 16 : 1;
-  while (n > 1 && (units * n > kClusterWorkers || ((n == 16 ? 2 * n : n / 2) >= tiles && n / 2 * (kThreads / 32) >= rows))) n /= 2;
-  return units * n <= kMaxWorkers && tiles * rows <= static_cast<int64_t>(16 * kClusterTiles) * n ? n : 0;
+  while (n > 1 && (units * n > (n == 16 ? kClusterWorkers / 2 : kClusterWorkers) || ((n == 16 ? 2 * n : n / 2) >= tiles && n / 2 * WARPS >= rows))) n /= 2;
+  if (units * n > kMaxWorkers || tiles * rows > static_cast<int64_t>(16 * kClusterTiles) * n) return 0;
+  return tiles <= 1 || rows <= 16 || n * WARPS >= rows ? n : 0;
 }
 
 template <typename T, bool I8, int D, int WM, bool TREE>
