@@ -1,0 +1,84 @@
+"""Serving operators on a B200 at the places where a result could be lost: single keys far above the rest,
+values that are not finite side by side, values near the type's largest, shared pages when the pool runs
+out, waits that run out."""
+
+import pytest
+import torch
+
+import piper_kernels_b200 as pk
+from _serving import attend, check, tree_visible, window_visible
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+LN2 = 0.6931471805599453
+
+
+def normal(*shape, dtype, seed):
+    gen = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=gen).to(dtype).cuda()
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def cache_of(k, v, tokens, page=16):
+    """A cache whose sequences hold the rows of k and v, the last ``tokens`` of them added last."""
+    batch, kv_heads, n, dim = k.shape
+    cache = pk.PageCache(batch, batch * -(-n // page), page, kv_heads, dim, dtype=k.dtype, max_length=n)
+    for count in (n - tokens, tokens):
+        cache.extend(ints([count] * batch))
+        at = slice(0, count) if count == n - tokens else slice(n - tokens, n)
+        if count:
+            cache.write(k[:, :, at].contiguous(), v[:, :, at].contiguous(), layer=0)
+    return cache
+
+
+def check_rows(got, q, k, v, *, window, scale, heads=None):
+    group, visible = q.shape[1] // k.shape[1], window_visible(q.shape[2], k.shape[2], window, 0, k.shape[2]).cuda()
+    for b in range(q.shape[0]):
+        for h in range(q.shape[1]) if heads is None else heads:
+            want, off = attend(q[b, h], k[b, h // group], v[b, h // group], visible, scale, q.dtype)
+            check(got[b, h], want, off, f"batch {b} head {h}")
+
+
+@pytest.mark.parametrize("gap", [13, 100, 128, 129, 140, 200, 255, 256, 261, 300, 400, 512, 520, 700])
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("rows", ["all", "one"])
+def test_single_key_far_above_the_rest(gap, dim, dtype, rows):
+    """Head h's key at place h of the second 128-key tile scores ``gap`` (base 2) above all others, in every query
+    row or in one of them; prompt rows (two row tiles, the second with few rows) and rows over a cache."""
+    heads, n_q, n_k = 32, 140, 300
+    q = torch.zeros(1, heads, n_q, dim, device="cuda")
+    q[:, :, slice(None) if rows == "all" else 77] = 1
+    k = torch.zeros(1, heads, n_k, dim, device="cuda")
+    # the first rows of the chunk stand at 160: some rows of either kind do not see all of the tile
+    k[0, torch.arange(heads), 128 + torch.arange(heads)] = gap * LN2 / dim
+    q, k, v = q.to(dtype), k.to(dtype), normal(1, heads, n_k, dim, dtype=dtype, seed=gap)
+    check_rows(pk.window_attention(q, k, v, window=400, scale=1.0), q, k, v, window=400, scale=1.0)
+    check_rows(pk.cache_attention(q, cache_of(k, v, n_q), scale=1.0), q, k, v, window=400, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("place", [14, 15, 30, 79])
+def test_single_key_far_above_the_rest_in_shared_units(dtype, place):
+    """The same in long rows whose key tiles several CTAs share, with random keys, for single rows of the last tile."""
+    q, k = normal(1, 2, 700, 128, dtype=dtype, seed=1).abs(), 0.1 * normal(1, 2, 2500, 128, dtype=dtype, seed=2)
+    v = normal(1, 2, 2500, 128, dtype=dtype, seed=3)
+    k[0, 0, 1280 + place] += 14
+    k[0, 1, 128 + place] += 20
+    check_rows(pk.window_attention(q, k, v, window=3000), q, k, v, window=3000, scale=128**-0.5)
+
+
+def test_single_key_far_above_the_rest_in_a_tree():
+    """64 drafted tokens (128 rows of a key head), one of which scores far above the context in the rows below it."""
+    q = torch.ones(1, 32, 64, 64, device="cuda", dtype=F16)
+    k = torch.zeros(1, 16, 300, 64, device="cuda", dtype=F16)
+    k[0, torch.arange(16), 236 + torch.arange(16)] = 150 * LN2 / 64  # draft tokens 0 to 15
+    v = normal(1, 16, 300, 64, dtype=F16, seed=4)
+    tree = [-1] + [(t - 1) // 2 for t in range(1, 64)]
+    got = pk.cache_attention(q, cache_of(k, v, 64), scale=1.0, tree=ints(tree))
+    visible = tree_visible(64, 236, 300, tree, None, 0).cuda()
+    for h in range(32):
+        want, off = attend(q[0, h], k[0, h // 2], v[0, h // 2], visible, 1.0, F16)
+        check(got[0, h], want, off, f"head {h}")
