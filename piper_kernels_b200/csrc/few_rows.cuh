@@ -492,6 +492,7 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
             const bool valid = idx >= 0 && idx < s.len;
             const float r = valid && sum != 0.f ? 1.f / sum : 0.f;
             float v[4];
+            bad[it] |= valid && !(sum <= 3.0e38f);  // 1 / infinity would make zeros of a row of NaN
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               v[y] = r == 0.f ? 0.f : acc[y] * r;

@@ -439,9 +439,10 @@ __device__ __forceinline__ void join_row(const AttendParams& p, const Pieces at,
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   const int b = g / p.row_blocks, len = attend_len(p, b), off = attend_off(p, b, len);
   const int t = token_of(p, row), idx = off + t;
-  const float inv = idx >= 0 && idx < len && sum != 0.f ? 1.f / sum : 0.f;
+  const bool valid = idx >= 0 && idx < len;
+  const float inv = valid && sum != 0.f ? 1.f / sum : 0.f;
   T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.heads + h * p.group + row - t * p.group) * p.tokens + t) * D + lane * E;
-  bool bad = false;
+  bool bad = valid && !(sum <= 3.0e38f);  // 1 / infinity would make zeros of a row of NaN
 #pragma unroll
   for (int e = 0; e < E; e += 2) {
     const float x = inv == 0.f ? 0.f : acc[e] * inv, y = inv == 0.f ? 0.f : acc[e + 1] * inv;

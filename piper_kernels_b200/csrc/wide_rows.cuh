@@ -110,7 +110,7 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t addr, int half) {
 // largest relative error with value 1 at 0 (2.9e-6, measured over r in 32-bit arithmetic); n goes into
 // the exponent, which holds [-127, 127]: x is limited to that.  Below, the result is 0 (r = 0 there).  Above, it
 // is 2^127, like every x beyond kWideRaise a reason to raise the reference and evaluate again.  A NaN comes
-// out as the largest finite number.
+// out as the largest finite number: the row's sum is then no smaller (the row is evaluated again).
 constexpr int kPolyEvery = 8;
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
   float a, b;
@@ -622,7 +622,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       // The query tile has been read by every product: its place takes the output rows, from where
       // they leave as whole lines (a thread's own row would be written 16 bytes at a time).
       const float inv = valid && begun && l != 0.f ? 1.f / l : 0.f;
-      bool bad = false;
+      bool bad = valid && !(l <= 3.0e38f);  // 1 / infinity would make zeros of a row of NaN
 #pragma unroll
       for (int c = 0; c < FEATURES; c += 32) {
         uint32_t o[32];

@@ -82,3 +82,27 @@ def test_single_key_far_above_the_rest_in_a_tree():
     for h in range(32):
         want, off = attend(q[0, h], k[0, h // 2], v[0, h // 2], visible, 1.0, F16)
         check(got[0, h], want, off, f"head {h}")
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("n_q,n_k,window", [(300, 300, 400), (300, 300, 40), (300, 2600, 3000), (9, 300, 400)])
+@pytest.mark.parametrize("apart", [1, 16, 64])
+def test_two_nan_keys_make_every_row_that_sees_them_nan(dim, dtype, n_q, n_k, window, apart):
+    """Head h: key rows at place h of a tile and ``apart`` behind it are NaN; whole units, units whose key tiles
+    several CTAs share, few rows, and rows over a cache."""
+    heads = 32
+    q, k, v = (normal(1, heads, n, dim, dtype=dtype, seed=s) for n, s in ((n_q, 5), (n_k, 6), (n_k, 7)))
+    h = torch.arange(heads, device="cuda")
+    first = (128 if n_k == 300 else 2304) + h
+    clean = k.clone()
+    k[0, h, first] = k[0, h, first + apart] = float("nan")
+    visible = window_visible(n_q, n_k, window, 0, n_k).cuda()
+    calls = [pk.window_attention(q, k, v, window=window)]
+    if n_k == 300:
+        calls.append(pk.cache_attention(q, cache_of(k, v, n_q), window=window))
+    for got in calls:
+        for i in range(heads):
+            lost = visible[:, first[i]] | visible[:, first[i] + apart]
+            assert lost.any() and got[0, i][lost].isnan().all()
+            want, off = attend(q[0, i], clean[0, i], v[0, i], visible, dim**-0.5, dtype)
+            check(got[0, i][~lost], want[~lost], off[~lost], f"head {i}")
