@@ -256,8 +256,8 @@ PK_API int pk_cache_maps(const pk_cache* c, void* maps);
 
 /* Room for counts[b] more rows (negative: none) of every sequence: starts = lengths, lengths +=
  * counts.  A partly filled last page that other sequences also name is replaced by a copy; when all
- * of its owners are extended in this call the first of them keeps it.  New pages are the lowest
- * free ones, in the order of the sequences.  A sequence that would pass width * page_size rows, or
+ * of its owners are extended in this call the longest of them (the first of these) keeps it.  New pages are
+ * the lowest free ones, in the order of the sequences.  A sequence that would pass width * page_size rows, or
  * for which the free pages (counted from the first sequence on) do not suffice, is refused: it is
  * not extended (starts = lengths). */
 PK_API int pk_cache_extend(const pk_cache* c, const int32_t* counts);

@@ -152,8 +152,8 @@ class PageCache:
 
         ``starts`` becomes the old and ``lengths`` the new length.  New pages are the lowest free ones, in the
         order of the sequences.  A partly filled last page that other sequences also use is replaced by a copy;
-        when all of its owners are extended, the first of them keeps it.  A sequence that would pass
-        ``max_length``, or that the free pages (counted from the first sequence on) do not reach, is refused.
+        when all of its owners are extended, the longest of them (the first of these) keeps it.  A sequence that
+        would pass ``max_length``, or that the free pages (counted from the first sequence on) do not reach, is refused.
         """
         check_lengths(_OP, "counts", counts, self.batch, self.device, optional=False)
         _cabi.check(_cabi.lib().pk_cache_extend(C.byref(self.handle()), counts.data_ptr()))

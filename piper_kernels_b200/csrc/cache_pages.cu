@@ -90,17 +90,24 @@ __global__ void __launch_bounds__(kPlan) extend_kernel(const Pages c, const int3
     tail[b] = is_page(c, page) ? page : -1;
   }
   __syncthreads();
-  // A last page that others name too is replaced; when all that name it grow, the first keeps it.
+  // A last page that others name too is replaced; when all that name it grow, the longest of them keeps it (the
+  // first of these): its new rows lie behind all rows of an owner that gets no page for its copy and stays.
   for (int b = tid; b < c.batch; b += kPlan) {
     bool copy = false;
     const int page = tail[b];
     if (page >= 0) {
       const int users = c.uses[page];
       if (users > 1) {
-        int growing = 0, first = b;
-        for (int o = 0; o < c.batch; ++o)
-          if (tail[o] == page) ++growing, first = min(first, o);
-        copy = growing < users || first != b;
+        const int held = length_of(c, b) & (c.page - 1);
+        int growing = 0;
+        bool keeps = true;
+        for (int o = 0; o < c.batch; ++o) {
+          if (tail[o] != page) continue;
+          ++growing;
+          const int other = length_of(c, o) & (c.page - 1);
+          keeps = keeps && (other < held || (other == held && o >= b));
+        }
+        copy = growing < users || !keeps;
       }
     }
     copies[b] = copy;

@@ -2,11 +2,14 @@
 values that are not finite side by side, values near the type's largest, shared pages when the pool runs
 out, waits that run out."""
 
+import random
+
 import pytest
 import torch
 
 import piper_kernels_b200 as pk
 from _serving import attend, check, tree_visible, window_visible
+from _serving_edges import LongestKeeps, unequal_owners
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
@@ -106,3 +109,55 @@ def test_two_nan_keys_make_every_row_that_sees_them_nan(dim, dtype, n_q, n_k, wi
             assert lost.any() and got[0, i][lost].isnan().all()
             want, off = attend(q[0, i], clean[0, i], v[0, i], visible, dim**-0.5, dtype)
             check(got[0, i][~lost], want[~lost], off[~lost], f"head {i}")
+
+
+class TaggedCache:
+    """A cache and its list model, whose rows hold numbers of their own; every row is compared after every call."""
+
+    def __init__(self, batch, pages, page, width):
+        self.cache = pk.PageCache(batch, pages, page, 1, 64, layers=2, dtype=F16, max_length=width * page)
+        self.model = LongestKeeps(batch, pages, page, width)
+        self.rows, self.tag = [[] for _ in range(batch)], 0
+
+    def call(self, what, argument):
+        m, c = self.model, self.cache
+        getattr(m, what)(argument)
+        getattr(c, what)(ints(argument))
+        if what == "fork":
+            self.rows = [list(self.rows[p]) for p in argument]
+        self.rows = [rows[: m.start[b]] for b, rows in enumerate(self.rows)]
+        if what == "extend":
+            added = [m.length[b] - m.start[b] for b in range(m.batch)]
+            data = torch.zeros(2, m.batch, 1, max(1, *added), 64, dtype=F16)
+            for b, n in enumerate(added):
+                for t in range(n):
+                    self.tag = self.tag % 2047 + 1
+                    self.rows[b].append(self.tag)
+                    data[:, b, 0, t] = self.tag
+            c.write(data.cuda(), -data.cuda())
+        assert [c.table.tolist(), c.lengths.tolist(), c.starts.tolist(), c.uses.tolist(), c.refused.tolist()] == [
+            m.table(), m.length, m.start, m.uses(), m.refused]
+        longest = max(1, *m.length)
+        want = torch.tensor([rows + [0] * (longest - len(rows)) for rows in self.rows], dtype=F16, device="cuda")
+        k, v = c.read(ints([0] * m.batch), longest)
+        want = want[None, :, None, :, None].expand_as(k)
+        assert torch.equal(k, want) and torch.equal(v, -want)
+
+
+def test_extend_leaves_the_rows_of_a_refused_owner():
+    for pages in (1, 2):
+        c = TaggedCache(2, pages, 16, 1)
+        c.call("extend", [9, 0])
+        c.call("fork", [0, 0])
+        c.call("truncate", [5, 9])
+        c.call("extend", [1, 1])
+        assert c.cache.refused.tolist() == [2 - pages, 0]
+
+
+@pytest.mark.parametrize("seed", range(4, 10))
+def test_sequences_of_different_lengths_that_share_a_last_page(seed):
+    rng = random.Random(seed)
+    batch = rng.choice([2, 3, 5])
+    c = TaggedCache(batch, batch + rng.randrange(3), 16, 3)
+    for what, argument in unequal_owners(rng, batch, 16, 60):
+        c.call(what, argument)
