@@ -618,7 +618,8 @@ PK_API int pk_cache_extend(const pk_cache* c, const int32_t* counts) {
   PK_CACHE_ENTRY(c, p);
   if (!counts) return fail(PK_ERR_BAD_ARG, "cache extend: null counts");
   const int smem = (3 * p.batch + 1) * static_cast<int>(sizeof(int));
-  if (smem > 48 * 1024 && (rc = allow_smem<extend_kernel>((3 * kMaxBatch + 1) * static_cast<int>(sizeof(int)), c->device))) return rc;
+  // beside it the kernel has shared memory of fixed size, and the two must not pass 48 KB without leave
+  if (smem > 40 * 1024 && (rc = allow_smem<extend_kernel>((3 * kMaxBatch + 1) * static_cast<int>(sizeof(int)), c->device))) return rc;
   if ((rc = launched(launch_chained(extend_kernel, dim3(1), dim3(kPlan), smem, st, p, counts), "extend"))) return rc;
   const int64_t items = static_cast<int64_t>(p.layers) * p.kv_heads * p.batch;
   const cudaError_t e = c->dtype == PK_I8 ? launch_chained(copy_tails_kernel<1>, dim3(copy_grid(items)), dim3(256), 0, st, p)

@@ -3,6 +3,9 @@ values that are not finite side by side, values near the type's largest, shared 
 out, waits that run out."""
 
 import random
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -13,6 +16,7 @@ from _serving_edges import LongestKeeps, unequal_owners
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
+ROOT = Path(__file__).resolve().parents[1]
 LN2 = 0.6931471805599453
 
 
@@ -161,3 +165,16 @@ def test_sequences_of_different_lengths_that_share_a_last_page(seed):
     c = TaggedCache(batch, batch + rng.randrange(3), 16, 3)
     for what, argument in unequal_owners(rng, batch, 16, 60):
         c.call(what, argument)
+
+
+def test_extend_of_nearly_the_largest_batch():
+    """In a process of its own: leave for more shared memory, once given, stays with the kernel."""
+    code = """
+import torch
+import piper_kernels_b200 as pk
+for batch in (3400, 4084, 4085, 4090, 4095, 4096):
+    cache = pk.PageCache(batch, batch, 16, 1, 64, dtype=torch.float16, max_length=16)
+    cache.extend(torch.ones(batch, dtype=torch.int32, device="cuda"))
+    assert cache.table.flatten().tolist() == list(range(batch)) and int(cache.lengths.sum()) == batch, batch
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT)
