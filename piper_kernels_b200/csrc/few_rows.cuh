@@ -496,7 +496,7 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               v[y] = r == 0.f ? 0.f : acc[y] * r;
-              bad[it] |= !(fabsf(v[y]) <= 3.0e38f);
+              bad[it] |= !holds<T>(v[y]);
             }
             T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.b) * p.heads + h * p.group + row - t * p.group) * p.tokens + t) * D + pass * kJoinCols + col;
             *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
@@ -507,7 +507,7 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
     }
 #pragma unroll
     for (int it = 0; it < WM; ++it) {
-      // rows with a value that is not finite, evaluated again from their own keys
+      // rows with a value that their type does not hold, evaluated again from their own keys
       const uint32_t vote = __ballot_sync(0xffffffffu, bad[it]);
       __syncwarp();
 #pragma unroll 1

@@ -198,10 +198,21 @@ __device__ __forceinline__ __half from_f32(float a) { return __float2half_rn(a);
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32(float a) { return __float2bfloat16_rn(a); }
 
+// Whether a result is a number that T holds.  The sums take the probabilities as they are and the products take
+// them rounded to T, relative to a reference that may lie far below the maximum: so the quotient may pass the
+// largest |v| by half a step of T, and where that is T's largest number (65504; from 65520 on float16 rounds to
+// infinity) the rounded result would be infinite.  Such a row is evaluated again.
+template <typename T>
+__device__ __forceinline__ bool holds(float x);
+template <>
+__device__ __forceinline__ bool holds<__half>(float x) { return fabsf(x) < 65520.f; }
+template <>
+__device__ __forceinline__ bool holds<__nv_bfloat16>(float x) { return fabsf(x) <= 3.0e38f; }
+
 // One output row from its visible keys alone, one key after the other, by one warp; lane i holds
 // features [i * D/32, (i+1) * D/32).  The tiled kernels multiply whole tiles, so that an infinity
 // or NaN in a V row that this query row must not see would still reach it (0 * NaN); a row that
-// comes out of them with a value that is not finite is evaluated again here (its features
+// comes out of them with a value that its type does not hold is evaluated again here (its features
 // [first, last) are written).  Rare, and slow.
 template <typename T, bool I8, int D>
 __device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, int row, int off, int len, RowView view, bool tree, int first = 0, int last = D) {
@@ -446,7 +457,7 @@ __device__ __forceinline__ void join_row(const AttendParams& p, const Pieces at,
 #pragma unroll
   for (int e = 0; e < E; e += 2) {
     const float x = inv == 0.f ? 0.f : acc[e] * inv, y = inv == 0.f ? 0.f : acc[e + 1] * inv;
-    bad |= !(fabsf(x) <= 3.0e38f) || !(fabsf(y) <= 3.0e38f);
+    bad |= !holds<T>(x) || !holds<T>(y);
     *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(x, y);
   }
   __syncwarp();

@@ -634,7 +634,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
             x[y] = inv != 0.f ? __uint_as_float(o[e + y]) * inv : 0.f;
-            bad |= !(fabsf(x[y]) <= 3.0e38f);
+            bad |= !holds<T>(x[y]);
           }
           *reinterpret_cast<uint4*>(q_piece(row, (c + e) / 8)) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
         }
@@ -653,7 +653,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       }
       uint32_t vote = __ballot_sync(0xffffffffu, bad);
       __syncwarp();
-      while (vote) {  // rows with a value that is not finite, evaluated again from their own keys
+      while (vote) {  // rows with a value that their type does not hold, evaluated again from their own keys
         const int src = __ffs(vote) - 1, rr = row0 + w4 * 32 + src;
         vote &= vote - 1;
         plain_row<T, false, D>(p, s.b, h, rr, s.off, s.len, row_view(p, s.off, s.len, token_of(p, rr), TREE ? tm : nullptr), TREE, half * FEATURES, half * FEATURES + FEATURES);

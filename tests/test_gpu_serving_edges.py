@@ -178,3 +178,63 @@ for batch in (3400, 4084, 4085, 4090, 4095, 4096):
     assert cache.table.flatten().tolist() == list(range(batch)) and int(cache.lengths.sum()) == batch, batch
 """
     subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n_q,n_k", [(1, 200), (9, 300), (40, 1500), (140, 300), (300, 2600)])
+def test_results_up_to_the_largest_number_of_float16(dim, n_q, n_k):
+    """Every value is +-65504 and a later key's weight is up to 2^12 times the first ones': the result is finite, and as
+    near 65504 as two roundings allow (probabilities, 2^-11 relative, and the result, 2^-11: ``attend``).  Single
+    tokens, few rows, prompt rows and units that several CTAs share; also over a cache."""
+    heads = 24
+    q = torch.ones(1, heads, n_q, dim, device="cuda", dtype=F16)
+    k = torch.zeros(1, heads, n_k, dim, device="cuda")
+    h = torch.arange(heads, device="cuda")
+    k[0, h, n_k - n_q - h] = (0.5 * h[:, None] + 0.3) * LN2 / dim
+    v = torch.full((1, heads, n_k, dim), 65504.0, device="cuda")
+    v[..., dim // 2:] *= -1
+    k, v = k.to(F16), v.to(F16)
+    calls = [pk.window_attention(q, k, v, window=n_k, scale=1.0)]
+    if n_k <= 300:
+        calls.append(pk.cache_attention(q, cache_of(k, v, n_q), scale=1.0))
+    for got in calls:
+        assert got.isfinite().all()
+        check_rows(got, q, k, v, window=n_k, scale=1.0, heads=(0, 7, 23))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [5, 12, 40])
+@pytest.mark.parametrize("n_q,n_k", [(1, 200), (9, 300), (40, 1500), (140, 300), (1000, 4000)])
+def test_largest_number_of_float16_under_random_weights(dim, window, n_q, n_k):
+    """The same with scores anywhere in [0, 12) (base 2) and few keys to a row, so that a rounded probability
+    decides the quotient."""
+    heads = 48
+    gen = torch.Generator().manual_seed(n_q + window)
+    q = torch.ones(1, heads, n_q, dim, device="cuda", dtype=F16)
+    k = (12 * LN2 / dim * torch.rand(1, heads, n_k, 1, generator=gen).cuda()).expand(1, heads, n_k, dim).to(F16)
+    v = torch.full((1, heads, n_k, dim), 65504.0, device="cuda", dtype=F16)
+    v[..., dim // 2:] *= -1
+    calls = [pk.window_attention(q, k, v, window=window, scale=1.0)]
+    if n_k <= 300:
+        calls.append(pk.cache_attention(q, cache_of(k, v, n_q), window=window, scale=1.0))
+    for got in calls:
+        assert got.isfinite().all()
+        check_rows(got, q, k, v, window=window, scale=1.0, heads=(0, 11, 47))
+
+
+@pytest.mark.parametrize("n_q,n_k", [(140, 300), (300, 2600)])
+def test_largest_number_of_float16_in_prompt_rows(n_q, n_k):
+    """The same with one key that outweighs all others together, by every factor that does not yet raise the
+    reference of its tile."""
+    heads = 256
+    gen = torch.Generator().manual_seed(n_q)
+    gaps = 10.5 + 1.45 * torch.rand(heads, generator=gen).cuda()
+    q = torch.ones(1, heads, n_q, 64, device="cuda", dtype=F16)
+    k = torch.full((1, heads, n_k, 64), -20 * LN2 / 64, device="cuda")
+    k[:, :, :4] = 0
+    k[0, torch.arange(heads), n_k - n_q - torch.arange(heads) % 30] = gaps[:, None] * LN2 / 64
+    k = k.to(F16)
+    v = torch.full((1, heads, n_k, 64), 65504.0, device="cuda", dtype=F16)
+    for got in (pk.window_attention(q, k, v, window=n_k, scale=1.0), pk.cache_attention(q, cache_of(k, v, n_q), scale=1.0)):
+        assert got.isfinite().all()
+        check_rows(got, q, k, v, window=n_k, scale=1.0, heads=range(0, heads, 17))
