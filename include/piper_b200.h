@@ -223,7 +223,7 @@ PK_API int pk_window_attention_fwd(const pk_window_problem* p);
  * contiguous device memory that the caller owns; the library keeps nothing.
  *   keys, values [layers, pages, kv_heads, page_size, head_dim]; PK_I8 also key_scales,
  *   value_scales [layers, pages, kv_heads, page_size] f32 (value = code * scale, scale >= 0)
- *   table [batch, width]: page of each page_size rows of a sequence, -1 where there is none
+ *   table [batch, width]: page of each page_size rows of a sequence, -1 where there is none (fewer than 2^31 entries)
  *   lengths [batch], starts [batch]: rows [starts, lengths) are the ones added last
  *   uses [pages]: how many table entries name the page; 0: free
  *   refused [batch]: set to 1 (0) by extend, fork and compact for a sequence that was left alone

@@ -90,6 +90,8 @@ class PageCache:
             raise ValueError(f"{_OP} holds at most {MAX_BATCH} sequences, got {self.batch}")
         if self.width * self.page_size >= 2**30:
             raise ValueError(f"{_OP} sequences must stay below 2^30 rows, got {self.width * self.page_size}")
+        if self.batch * self.width >= 2**31:
+            raise ValueError(f"{_OP} table must have fewer than 2^31 entries, got {self.batch} x {self.width}")
         scales = (self.layers, self.pages, self.kv_heads, self.page_size) if self.dtype is torch.int8 else None
         wanted = {"keys": (keys, self.dtype, keys.shape), "values": (values, self.dtype, keys.shape),
                   "table": (table, torch.int32, (self.batch, self.width)), "lengths": (lengths, torch.int32, (self.batch,)),

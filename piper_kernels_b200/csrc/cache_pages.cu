@@ -598,6 +598,8 @@ int validate_cache(const pk_cache* c) {
   if (c->dtype != PK_F16 && c->dtype != PK_BF16 && c->dtype != PK_I8) return fail(PK_ERR_BAD_ARG, "cache dtype must be float16, bfloat16 or int8");
   if (c->batch > kMaxBatch) return fail(PK_ERR_BAD_ARG, "cache: at most %d sequences, got %d", kMaxBatch, c->batch);
   if (static_cast<int64_t>(c->width) * c->page_size >= (1 << 30)) return fail(PK_ERR_BAD_ARG, "cache: a sequence must stay below 2^30 rows");
+  // `extend` sums the pages that all sequences want in 32 bits
+  if (static_cast<int64_t>(c->batch) * c->width >= (1ll << 31)) return fail(PK_ERR_BAD_ARG, "cache: the table must have fewer than 2^31 entries");
   if (static_cast<int64_t>(c->layers) * c->pages >= (1ll << 31) - 1 || static_cast<int64_t>(c->layers) * c->kv_heads * c->batch >= (1ll << 31))
     return fail(PK_ERR_BAD_ARG, "cache: too many pages or heads");
   if (!c->keys || !c->values || !c->table || !c->lengths || !c->starts || !c->uses || !c->refused || !c->scratch) return fail(PK_ERR_BAD_ARG, "cache: null pointer");

@@ -1,11 +1,15 @@
-"""CPU tests of the serving operators' edges: the list model of shared last pages."""
+"""CPU tests of the serving operators' edges: the list model of shared last pages, refusals."""
 
+import ctypes as C
 import random
 
 import pytest
+import torch
 
+import piper_kernels_b200 as pk
 from _serving import ListCache
 from _serving_edges import LongestKeeps, unequal_owners
+from piper_kernels_b200 import _cabi
 
 
 def test_longest_owner_keeps_a_shared_page():
@@ -45,3 +49,23 @@ def test_equal_owners_are_as_in_the_list_model():
             m.truncate([keep] * 6)
         a, b = models
         assert (a.own, a.length, a.start, a.refused) == (b.own, b.length, b.start, b.refused)
+
+
+def test_tables_that_32_bits_cannot_count_are_refused():
+    lib, n = _cabi.lib(), C.c_uint64()
+    query = _cabi.PkCacheQuery(4, 1, 0, _cabi.PK_F16, 0, 0, 0.1, 256)
+
+    def ask(batch, width):
+        c = _cabi.PkCache(1, 10, 2, 16, 64, batch, width, _cabi.PK_F16)
+        for name in ("keys", "values", "table", "lengths", "starts", "uses", "refused", "scratch"):
+            setattr(c, name, 256)
+        return lib.pk_cache_attention_workspace_bytes(C.byref(c), C.byref(query), C.byref(n))
+
+    assert ask(4096, 2**19 - 1) == ask(1, 2**26 - 1) == ask(4095, 2**19) == _cabi.PK_OK
+    assert ask(4096, 2**19) == ask(33, 2**26 - 1) == _cabi.PK_ERR_BAD_ARG
+    assert b"table" in lib.pk_last_error()
+    make = {n: torch.empty(s, dtype=d, device="meta") for n, s, d in (
+        ("keys", (1, 4, 1, 16, 64), torch.float16), ("values", (1, 4, 1, 16, 64), torch.float16), ("lengths", 4096, torch.int32),
+        ("starts", 4096, torch.int32), ("uses", 4, torch.int32))}
+    with pytest.raises(ValueError, match="table must have fewer than"):
+        pk.PageCache.from_tensors(table=torch.empty(4096, 2**19, dtype=torch.int32, device="meta"), **make)
