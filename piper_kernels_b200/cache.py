@@ -13,6 +13,7 @@ A decoding step is a run of calls without a host round trip, which can be captur
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -25,6 +26,7 @@ PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_BATCH = 4096
 _OP = "PageCache"
 _STRIDES = C.c_int64 * 4
+_MAKING_MAPS = threading.Lock()
 
 
 class PageCache:
@@ -136,12 +138,16 @@ class PageCache:
     def mapped_handle(self) -> _cabi.PkCache:
         """The same with the copy maps of keys and values, which are made once for the cache's life."""
         c = self.handle()
-        if self._maps is None:
-            maps = C.create_string_buffer(_cabi.PK_CACHE_MAP_BYTES + 64)
-            at = -(-C.addressof(maps) // 64) * 64
+        maps = self._maps
+        if maps is None:
+            memory = C.create_string_buffer(_cabi.PK_CACHE_MAP_BYTES + 64)
+            at = -(-C.addressof(memory) // 64) * 64
             _cabi.check(_cabi.lib().pk_cache_maps(C.byref(c), at))
-            self._maps = (maps, at)
-        c.maps = self._maps[1]
+            with _MAKING_MAPS:  # of two threads that made maps the first one's stay: they may be in use already
+                if self._maps is None:
+                    self._maps = (memory, at)
+                maps = self._maps
+        c.maps = maps[1]
         return c
 
     def check_layer(self, layer: int) -> int:

@@ -69,3 +69,23 @@ def test_tables_that_32_bits_cannot_count_are_refused():
         ("starts", 4096, torch.int32), ("uses", 4, torch.int32))}
     with pytest.raises(ValueError, match="table must have fewer than"):
         pk.PageCache.from_tensors(table=torch.empty(4096, 2**19, dtype=torch.int32, device="meta"), **make)
+
+
+def test_copy_maps_of_two_threads_are_one(monkeypatch):
+    """A second thread asks for the maps while the first one's are being made: what either was given stays alive."""
+    cache = pk.PageCache(1, 2, 16, 1, 64, dtype=torch.float16, device="cpu")
+    given, inner = [], []
+
+    class Library:
+        def pk_cache_maps(self, c, at):
+            given.append(at)
+            if len(given) == 1:
+                inner.append(cache.mapped_handle())
+            return _cabi.PK_OK
+
+    monkeypatch.setattr(cache, "handle", _cabi.PkCache)
+    monkeypatch.setattr(_cabi, "lib", Library)
+    outer = cache.mapped_handle()
+    assert outer.maps == inner[0].maps == cache.mapped_handle().maps and outer.maps in given
+    start = C.addressof(cache._maps[0])
+    assert start <= outer.maps <= start + 64 and outer.maps % 64 == 0
