@@ -304,6 +304,15 @@ typedef struct pk_cache_query {
 PK_API int pk_cache_attention_workspace_bytes(const pk_cache* c, const pk_cache_query* q, uint64_t* bytes);
 PK_API int pk_cache_attention_fwd(const pk_cache* c, const pk_cache_query* q);
 
+/* Stalled-wait drill of the two attention operators (test aid): the ordinary call with every wait limited to
+ * `wait_cycles` SM cycles (at most 1.5e9) and, for `copy` >= 0, with copy number `copy` of every CTA left out (a
+ * K and V tile; with more than 64 rows of a key head on 16-bit keys, a K or a V tile).  A CTA that gives up a
+ * wait lets its copies and products end, releases tensor memory, fills the rows that it has not finished with
+ * NaN and returns; pk_poll_device_fault then reports the wait.  Rows of other CTAs are as in the ordinary
+ * call.  Nothing traps, faults or spins without a limit. */
+PK_API int pk_debug_window_stall(const pk_window_problem* p, int64_t wait_cycles, int32_t copy);
+PK_API int pk_debug_cache_stall(const pk_cache* c, const pk_cache_query* q, int64_t wait_cycles, int32_t copy);
+
 #ifdef __cplusplus
 }
 #endif

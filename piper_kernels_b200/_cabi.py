@@ -26,7 +26,7 @@ EXPORTS = (
     "pk_poll_device_fault", "pk_debug_stalled_wait",
     "pk_window_workspace_bytes", "pk_window_attention_fwd",
     "pk_cache_maps", "pk_cache_extend", "pk_cache_write", "pk_cache_read", "pk_cache_fork", "pk_cache_truncate", "pk_cache_compact",
-    "pk_cache_attention_workspace_bytes", "pk_cache_attention_fwd",
+    "pk_cache_attention_workspace_bytes", "pk_cache_attention_fwd", "pk_debug_window_stall", "pk_debug_cache_stall",
 )
 
 
@@ -135,6 +135,8 @@ def lib() -> C.CDLL:
         handle.pk_cache_compact.argtypes = [K, ptr, i64, i32, ptr]
         handle.pk_cache_attention_workspace_bytes.argtypes = [K, Q, C.POINTER(C.c_uint64)]
         handle.pk_cache_attention_fwd.argtypes = [K, Q]
+        handle.pk_debug_window_stall.argtypes = [W, i64, i32]
+        handle.pk_debug_cache_stall.argtypes = [K, Q, i64, i32]
         for name in EXPORTS[2:]:
             getattr(handle, name).restype = C.c_int
         _lib = handle

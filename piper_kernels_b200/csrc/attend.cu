@@ -206,24 +206,12 @@ int validate_query(const pk_cache* c, const pk_cache_query* q, bool launching) {
   return PK_OK;
 }
 
-}  // namespace
-}  // namespace pk
+struct Drill {  // the stalled-wait drill: see pk_debug_window_stall
+  int64_t wait_cycles = 0;
+  int skip_copy = -1;
+};
 
-using namespace pk;
-
-extern "C" {
-
-PK_API int pk_window_workspace_bytes(const pk_window_problem* p, uint64_t* bytes) {
-  clear_error();
-  if (!bytes) return fail(PK_ERR_BAD_ARG, "null size pointer");
-  const int rc = validate_window(p, false);
-  if (rc) return rc;
-  *bytes = dense_layout(*p).total;
-  return PK_OK;
-}
-
-PK_API int pk_window_attention_fwd(const pk_window_problem* pp) {
-  clear_error();
+int window_fwd(const pk_window_problem* pp, const Drill& drill) {
   int rc = validate_window(pp, true);
   if (rc) return rc;
   const pk_window_problem& p = *pp;
@@ -234,6 +222,7 @@ PK_API int pk_window_attention_fwd(const pk_window_problem* pp) {
   const DenseLayout l = dense_layout(p);
   char* ws = static_cast<char*>(p.workspace);
   AttendParams a{};
+  a.wait_cycles = drill.wait_cycles, a.skip_copy = drill.skip_copy;
   a.q = p.q;
   a.out = p.out;
   a.batch = p.batch, a.heads = p.heads, a.kv_heads = p.kv_heads, a.group = p.heads / p.kv_heads, a.tokens = p.q_len;
@@ -272,6 +261,74 @@ PK_API int pk_window_attention_fwd(const pk_window_problem* pp) {
   return attend(a, p.head_dim, p.dtype, false, p.device, st);
 }
 
+int cache_fwd(const pk_cache* c, const pk_cache_query* q, const Drill& drill) {
+  int rc = validate_query(c, q, true);
+  if (rc) return rc;
+  const DeviceGuard g(c->device);
+  if (g.err != cudaSuccess) return fail(PK_ERR_CUDA, "cudaSetDevice(%d): %s", c->device, cuda_err(g.err));
+  if ((rc = check_arch(c->device))) return rc;
+  const cudaStream_t st = static_cast<cudaStream_t>(c->stream);
+  const bool i8 = c->dtype == PK_I8;
+  AttendParams a{};
+  a.wait_cycles = drill.wait_cycles, a.skip_copy = drill.skip_copy;
+  a.q = q->q;
+  memcpy(a.q_stride, q->q_stride, sizeof(a.q_stride));
+  const int64_t qdims[3] = {c->batch, q->heads, q->tokens};
+  a.q_vec = rows_aligned(q->q, q->q_stride, qdims);
+  a.out = q->out;
+  a.batch = c->batch, a.heads = q->heads, a.kv_heads = c->kv_heads, a.group = q->heads / c->kv_heads, a.tokens = q->tokens;
+  a.rows = a.group * a.tokens;
+  a.group_inv = ~0ull / a.group + 1;  // not used for groups of one
+  a.lengths = c->lengths, a.starts = c->starts;
+  a.table = c->table, a.width = c->width, a.page = c->page_size, a.pages = c->pages, a.page_base = q->layer * c->pages;
+  a.page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
+  a.pool_pages = c->layers * c->pages;
+  a.maps = static_cast<const CUtensorMap*>(c->maps);
+  a.k = c->keys, a.v = c->values;
+  const int64_t layer_rows = static_cast<int64_t>(c->pages) * c->kv_heads * c->page_size * q->layer;
+  if (i8) a.k_scale = c->key_scales + layer_rows, a.v_scale = c->value_scales + layer_rows;
+  a.tree = q->tree, a.tree_stride = q->tree_stride;
+  a.window = q->window > 0 && q->window < kNoWindow ? q->window : kNoWindow;
+  a.sinks = q->sinks;
+  a.scale_log2 = q->scale * kLog2e;
+  a.partial = static_cast<float*>(q->workspace);
+  a.host_status = fault_word_device_ptr(c->device);
+  return attend(a, c->head_dim, q->dtype, i8, c->device, st);
+}
+
+int check_drill(int64_t wait_cycles, int32_t copy) {
+  if (wait_cycles <= 0 || wait_cycles > kWaitCycleLimit) return fail(PK_ERR_BAD_ARG, "stall: wait_cycles must be in [1, %lld], got %lld", kWaitCycleLimit, static_cast<long long>(wait_cycles));
+  if (copy < -1) return fail(PK_ERR_BAD_ARG, "stall: copy must be -1 or more, got %d", copy);
+  return PK_OK;
+}
+
+}  // namespace
+}  // namespace pk
+
+using namespace pk;
+
+extern "C" {
+
+PK_API int pk_window_workspace_bytes(const pk_window_problem* p, uint64_t* bytes) {
+  clear_error();
+  if (!bytes) return fail(PK_ERR_BAD_ARG, "null size pointer");
+  const int rc = validate_window(p, false);
+  if (rc) return rc;
+  *bytes = dense_layout(*p).total;
+  return PK_OK;
+}
+
+PK_API int pk_window_attention_fwd(const pk_window_problem* p) {
+  clear_error();
+  return window_fwd(p, Drill{});
+}
+
+PK_API int pk_debug_window_stall(const pk_window_problem* p, int64_t wait_cycles, int32_t copy) {
+  clear_error();
+  const int rc = check_drill(wait_cycles, copy);
+  return rc ? rc : window_fwd(p, Drill{wait_cycles, copy});
+}
+
 PK_API int pk_cache_maps(const pk_cache* c, void* maps) {
   clear_error();
   int rc = validate_cache(c);
@@ -300,37 +357,13 @@ PK_API int pk_cache_attention_workspace_bytes(const pk_cache* c, const pk_cache_
 
 PK_API int pk_cache_attention_fwd(const pk_cache* c, const pk_cache_query* q) {
   clear_error();
-  int rc = validate_query(c, q, true);
-  if (rc) return rc;
-  const DeviceGuard g(c->device);
-  if (g.err != cudaSuccess) return fail(PK_ERR_CUDA, "cudaSetDevice(%d): %s", c->device, cuda_err(g.err));
-  if ((rc = check_arch(c->device))) return rc;
-  const cudaStream_t st = static_cast<cudaStream_t>(c->stream);
-  const bool i8 = c->dtype == PK_I8;
-  AttendParams a{};
-  a.q = q->q;
-  memcpy(a.q_stride, q->q_stride, sizeof(a.q_stride));
-  const int64_t qdims[3] = {c->batch, q->heads, q->tokens};
-  a.q_vec = rows_aligned(q->q, q->q_stride, qdims);
-  a.out = q->out;
-  a.batch = c->batch, a.heads = q->heads, a.kv_heads = c->kv_heads, a.group = q->heads / c->kv_heads, a.tokens = q->tokens;
-  a.rows = a.group * a.tokens;
-  a.group_inv = ~0ull / a.group + 1;  // not used for groups of one
-  a.lengths = c->lengths, a.starts = c->starts;
-  a.table = c->table, a.width = c->width, a.page = c->page_size, a.pages = c->pages, a.page_base = q->layer * c->pages;
-  a.page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
-  a.pool_pages = c->layers * c->pages;
-  a.maps = static_cast<const CUtensorMap*>(c->maps);
-  a.k = c->keys, a.v = c->values;
-  const int64_t layer_rows = static_cast<int64_t>(c->pages) * c->kv_heads * c->page_size * q->layer;
-  if (i8) a.k_scale = c->key_scales + layer_rows, a.v_scale = c->value_scales + layer_rows;
-  a.tree = q->tree, a.tree_stride = q->tree_stride;
-  a.window = q->window > 0 && q->window < kNoWindow ? q->window : kNoWindow;
-  a.sinks = q->sinks;
-  a.scale_log2 = q->scale * kLog2e;
-  a.partial = static_cast<float*>(q->workspace);
-  a.host_status = fault_word_device_ptr(c->device);
-  return attend(a, c->head_dim, q->dtype, i8, c->device, st);
+  return cache_fwd(c, q, Drill{});
+}
+
+PK_API int pk_debug_cache_stall(const pk_cache* c, const pk_cache_query* q, int64_t wait_cycles, int32_t copy) {
+  clear_error();
+  const int rc = check_drill(wait_cycles, copy);
+  return rc ? rc : cache_fwd(c, q, Drill{wait_cycles, copy});
 }
 
 }  // extern "C"

@@ -110,6 +110,32 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
+// Rows of NaN and marked pieces for what a CTA leaves undone after a wait was given up: the tiles [w, w1) of its
+// share, which began with w0.
+template <typename T, bool I8, int D, int WM, bool TREE>
+__device__ __noinline__ void leave_undone(const AttendParams& p, Walk<TREE, Few<T, I8, D, WM>::TILE, Few<T, I8, D, WM>::ROWS> walk, uint32_t w, uint32_t w0,
+                                          uint32_t w1, uint32_t total) {
+  using C = Few<T, I8, D, WM>;
+  while (w < w1) {
+    const Span& s = walk.s;
+    const int from = walk.tile, n = static_cast<int>(min(static_cast<uint32_t>(s.n - from), w1 - w));
+    const bool whole = from == 0 && n == s.n;
+    const int slot = blockIdx.x * 2 + (from == 0 && w != w0 && !p.cluster ? 1 : 0);
+    for (int r = threadIdx.x; r < C::ROWS; r += kConsumers) {
+      if (s.rb * C::ROWS + r >= p.rows) continue;
+      if (whole) nan_row<T, D, D>(p, s.b, walk.h, s.rb * C::ROWS + r, 0);
+      else *reinterpret_cast<float2*>(p.partial + (static_cast<int64_t>(slot) * C::ROWS + r) * (D + 4) + D) = make_float2(-INFINITY, kUndone);
+    }
+    if (from == 0 && threadIdx.x == 0 && !p.cluster) {
+      const int last = whole ? static_cast<int>(blockIdx.x) : static_cast<int>(owner_of(total, gridDim.x, w + s.n - 1));
+      p.pieces[walk.g * p.kv_heads + walk.h] = Pieces{static_cast<int>(blockIdx.x), last, w != w0, 0};
+    }
+    w += n;
+    walk.tile = from + n - 1;
+    walk.next(p);
+  }
+}
+
 template <typename T, bool I8, int D, int WM, bool TREE>
 __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttendParams& p, uint8_t* smem) {
   using C = Few<T, I8, D, WM>;
@@ -156,12 +182,11 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
       return p.table && lane < boxes && j < walk.s.len ? attend_page(p, walk.s.b, j) : -1;
     };
     int last = -1, page = look_up();
-    bool ok = true;
     for (uint32_t w = w0; w < w1; ++w) {
       const int i = static_cast<int>(w - w0), st = i % kStages, j0 = walk.key(), h = walk.h, b = walk.s.b;
       walk.next(p);
       const int next = w + 1 < w1 ? look_up() : -1;
-      if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * (kStages + st), ((i / kStages) - 1) & 1, abort_flag, 61))) { ok = false; break; }
+      if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * (kStages + st), ((i / kStages) - 1) & 1, abort_flag, 61, p.wait_cycles))) break;
       const uint32_t full = bars + 8 * st, dst = base + st * C::STAGE;
       const uint32_t mask = p.table ? __ballot_sync(0xffffffffu, page >= 0) : 1u;
       if (lane == 0) {
@@ -169,7 +194,8 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
         mbar_expect_tx(full, C::STAGE + (I8 ? __popc(mask) * 2 * box * 4 : 0));
       }
       __syncwarp();
-      if (!p.table) {
+      if (i == p.skip_copy) {  // drill
+      } else if (!p.table) {
         if (lane == 0) {
           tma_load_5d(dst, &tm_k, full, 0, j0, 0, p.k_stride[1] ? h : 0, p.k_stride[0] ? b : 0);
           tma_load_5d(dst + C::KV_BYTES, &tm_v, full, 0, j0, 0, p.v_stride[1] ? h : 0, p.v_stride[0] ? b : 0);
@@ -189,8 +215,8 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
       page = next;
       last = i;
     }
-    if (!ok)  // giving up: let the copies that were issued land before the CTA returns
-      for (int i = max(0, last - kStages + 1); i <= last; ++i) mbar_wait_quiet(bars + 8 * (i % kStages), (i / kStages) & 1, 100000);
+    // The CTA may end early, when its other warps give up a wait: not before the copies that were issued have landed.
+    for (int i = max(0, last - kStages + 1); i <= last; ++i) mbar_wait_quiet(bars + 8 * (i % kStages), (i / kStages) & 1, 100000);
     return;
   }
 
@@ -210,7 +236,7 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
   bool ok = true;
 
   uint32_t w = w0;
-  for (int i = 0; ok && w < w1;) {
+  for (int i = 0; w < w1;) {
     // -------- a new unit: rows [rb * ROWS, ...) of key head h of batch element b
     const Span s = walk.s;
     const int h = walk.h, unit_from = walk.tile;
@@ -260,9 +286,9 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
 
     const int unit_tiles = static_cast<int>(min(static_cast<uint32_t>(s.n - walk.tile), w1 - w));
     const int box = p.table ? min(p.page, C::TILE) : C::TILE;
-    for (int u = 0; u < unit_tiles; ++u, ++i, ++w) {
+    for (int u = 0; u < unit_tiles; ++u, ++i) {
       const int st = i % kStages;
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * st, (i / kStages) & 1, abort_flag, 62));
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * st, (i / kStages) & 1, abort_flag, 62, p.wait_cycles));
       if (!ok) break;
       const int j0 = key_of_tile<C::TILE>(s, unit_from + u);
       // Keys on pages that are not there are masked like those that no row may see.
@@ -430,19 +456,18 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
     // -------- join the warps that shared the unit's keys; write rows, or a piece for the join kernel
     const bool whole = unit_from == 0 && unit_tiles == s.n;
     if (unit_from == 0 && tid == 0 && !p.cluster) {
-      const uint32_t u0 = w - unit_tiles;  // (after an abandoned wait the pieces do not matter)
-      const int last = whole ? static_cast<int>(blockIdx.x) : static_cast<int>(owner_of(total, gridDim.x, u0 + s.n - 1));
-      p.pieces[walk.g * p.kv_heads + h] = Pieces{static_cast<int>(blockIdx.x), last, u0 != w0, 0};
+      const int last = whole ? static_cast<int>(blockIdx.x) : static_cast<int>(owner_of(total, gridDim.x, w + s.n - 1));
+      p.pieces[walk.g * p.kv_heads + h] = Pieces{static_cast<int>(blockIdx.x), last, w != w0, 0};
     }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      if (!ok) l[x] = __int_as_float(0x7FC00000);
       if (c4 == 0) ml[warp * 16 + g8 + 8 * x] = make_float2(m[x], l[x]);
     }
     ok = vote_barrier(1, kConsumers, ok && *abort_flag == 0);  // the same answer in every warp: they leave together
-    const int slot = blockIdx.x * 2 + (unit_from == 0 && w - unit_tiles != w0 && !p.cluster ? 1 : 0);
+    if (!ok) break;
+    const int slot = blockIdx.x * 2 + (unit_from == 0 && w != w0 && !p.cluster ? 1 : 0);
     float* piece = p.partial + static_cast<int64_t>(slot) * C::ROWS * (D + 4);
     // thread -> (row, four consecutive columns) of the CTA's rows; a row's columns belong to 8 neighbouring threads
     bool bad[WM];
@@ -518,9 +543,11 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
       }
     }
     // the next unit
+    w += unit_tiles;
     walk.tile = unit_from + unit_tiles - 1;
     walk.next(p);
   }
+  if (w < w1) leave_undone<T, I8, D, WM, TREE>(p, walk, w, w0, w1, total);
   if (tid == 0 && *abort_flag != 0 && p.host_status != nullptr) atomicCAS_system(p.host_status, 0, *abort_flag);
 }
 
@@ -578,6 +605,7 @@ int launch(AttendParams p, int device, cudaStream_t st) {
   using C = Few<T, I8, D, WM>;
   static_assert(C::SMEM <= 113 * 1024, "two CTAs share an SM");
   p.row_blocks = (p.rows + C::ROWS - 1) / C::ROWS;
+  if (p.wait_cycles == 0) p.wait_cycles = kWaitCycleLimit;
   p.key_align = p.table ? (p.page < C::TILE ? p.page : C::TILE) : 8;
   CUtensorMap tk, tv;
   int rc;

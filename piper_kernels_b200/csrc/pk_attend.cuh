@@ -54,6 +54,8 @@ struct AttendParams {
   int workers, first_unit;
   int cluster;  // few rows: CTAs that share one unit and join its pieces themselves, or 0
   int32_t* host_status;  // pinned word that takes the site of an abandoned wait
+  long long wait_cycles;  // a wait inside a kernel is given up after this many cycles
+  int skip_copy;          // drill: every CTA leaves out its copy of this number, so that a wait runs out (-1: none)
   const CUtensorMap* maps;  // host: K and V maps for 64- and 128-key tiles of few rows and for many rows, or null
 };
 
@@ -386,6 +388,19 @@ struct Pieces {
   int c0, c1, late, pad;
 };
 
+// What a CTA that gave up a wait has not finished, for other code to see: rows of NaN, and pieces whose sum is
+// negative, from which the join makes rows of NaN.
+constexpr float kUndone = -1.f;
+// Features [first, first + N) of a query row.
+template <typename T, int D, int N>
+__device__ __forceinline__ void nan_row(const AttendParams& p, int b, int kvh, int row, int first) {
+  const int t = token_of(p, row), head = kvh * p.group + row - t * p.group;
+  T* out = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.heads + head) * p.tokens + t) * D + first;
+  const uint32_t w = pack2<T>(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
+#pragma unroll 1
+  for (int i = 0; i < N; i += 8) *reinterpret_cast<uint4*>(out + i) = make_uint4(w, w, w, w);
+}
+
 template <bool TREE, int TILE, int ROWS>
 struct Walk {  // position in the list of tiles
   Span s;
@@ -420,7 +435,16 @@ __device__ __forceinline__ void join_row(const AttendParams& p, const Pieces at,
   float2 first = make_float2(-INFINITY, 0.f);  // maximum and sum of this lane's first piece
   if (at.c0 + lane <= at.c1) first = *reinterpret_cast<const float2*>(p.partial + slot(at.c0 + lane) + D);
   mx = first.x;
-  for (int c = at.c0 + 32 + lane; c <= at.c1; c += 32) mx = fmaxf(mx, p.partial[slot(c) + D]);
+  bool undone = first.y < 0.f;
+  for (int c = at.c0 + 32 + lane; c <= at.c1; c += 32) {
+    const float2 st = *reinterpret_cast<const float2*>(p.partial + slot(c) + D);
+    mx = fmaxf(mx, st.x);
+    undone |= st.y < 0.f;
+  }
+  if (__any_sync(0xffffffffu, undone)) {
+    if (lane < D / 8) nan_row<T, D, 8>(p, g / p.row_blocks, h, row, lane * 8);
+    return;
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
 #pragma unroll

@@ -70,7 +70,7 @@ struct Wide {
   static constexpr int OFF_RING = 2 * TILE_BYTES;
   static constexpr int OFF_TOP = OFF_RING + STAGES * TILE_BYTES;  // [row tile][half][128]: maxima, then sums
   static constexpr int OFF_BAR = OFF_TOP + 2 * 2 * 128 * 4;
-  static constexpr int BARS = 2 * STAGES + 8;  // ring full / empty; q_full, s_full, p_full, o_done per row tile
+  static constexpr int BARS = 2 * STAGES + 9;  // ring full / empty; q_full, s_full, p_full, o_done per row tile; drained
   static constexpr int OFF_RED = OFF_BAR + (BARS + 1) / 2 * 16;
   static constexpr int OFF_THERE = OFF_RED + 64;
   static constexpr int OFF_MISC = OFF_THERE + kThere * 4;
@@ -136,14 +136,13 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
 // A bounded wait with little code (it is in every role's loop): gives up after some seconds, or when
 // another wait has been given up.  The limit is generous because a softmax warp may be away evaluating
 // rows one by one (plain_row) while the others wait for it.
-constexpr long long kWideWaitCycles = 4 * kWaitCycleLimit;
-__device__ __forceinline__ bool wide_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int where) {
+__device__ __forceinline__ bool wide_wait(const AttendParams& p, uint32_t bar, uint32_t parity, volatile int* abort_flag, int where) {
   long long since = 0;
   for (int n = 0; !mbar_try_wait(bar, parity); ++n) {
     if ((n & 63) != 63) continue;
     const long long now = clock64();
     if (since == 0) since = now;
-    if (*abort_flag != 0 || now - since > kWideWaitCycles) {
+    if (*abort_flag != 0 || now - since > p.wait_cycles) {
       *abort_flag = where;
       return false;
     }
@@ -222,6 +221,48 @@ __device__ __forceinline__ uint32_t seen_bits(const RowView& v, int j, int off, 
   return bits;
 }
 
+// Where a row tile's warps stopped, for what they leave undone after a wait was given up.
+struct Stopped {
+  int unit;
+  uint32_t at;
+};
+
+// Rows of NaN and marked pieces for what the CTA has not finished; by the whole CTA, which finds its place in the
+// list of units anew (carrying it to the end of the kernel cost the softmax registers and 2 % of the time).
+template <typename T, int D, bool TREE>
+__device__ __noinline__ void leave_undone(const AttendParams& p, const Stopped* stopped, uint32_t* red, Found* found) {
+  const int tid = threadIdx.x, i = (tid >> 7) & 1, half = tid >> 8, row = i * 128 + (tid & 127);
+  Segments<TREE> seg;
+  seg.unit = stopped[i].unit;
+  seg.units = p.first_unit;
+  seg.at = seg.end = 0;
+  uint32_t total = 0, share_from = 0;
+  if (p.workers) {
+    const int g0 = p.first_unit / p.kv_heads;
+    total = sum_tiles<TREE, kWideTile, kWideRows>(p, g0, p.batch * p.row_blocks, red);
+    share_from = share_begin(total, p.workers, blockIdx.x);
+    seg.at = stopped[i].at;
+    seg.end = share_begin(total, p.workers, blockIdx.x + 1);
+    for (int x = 0; x < 2; ++x) {
+      if (stopped[x].at >= seg.end) continue;  // the same for the whole CTA
+      const Found f = find_group<TREE, kWideTile, kWideRows>(p, g0, stopped[x].at, red, found);
+      if (x == i) seg.found = f;
+      __syncthreads();
+    }
+  }
+  if (tid >= 512) return;  // the other threads stand for a half row each
+  for (seg.take(p); seg.more(); seg.advance(p)) {
+    const Span& s = seg.walk.s;
+    const int r = s.rb * kWideRows + row, slot = blockIdx.x * 2 + (!seg.whole() && seg.at != share_from ? 1 : 0);
+    if (r < p.rows) {
+      if (seg.whole() || (seg.walk.tile == 0 && seg.count() == s.n)) nan_row<T, D, D / 2>(p, s.b, seg.walk.h, r, half * (D / 2));
+      else if (half == 0) *reinterpret_cast<float2*>(p.partial + (static_cast<int64_t>(slot) * kWideRows + row) * (D + 4) + D) = make_float2(-INFINITY, kUndone);
+    }
+    if (!seg.whole() && seg.walk.tile == 0 && tid == 0)
+      p.pieces[seg.walk.g * p.kv_heads + seg.walk.h] = Pieces{static_cast<int>(blockIdx.x), static_cast<int>(owner_of(total, p.workers, seg.at + s.n - 1)), seg.at != share_from, 0};
+  }
+}
+
 template <typename T, int D, bool TREE>
 __global__ void __launch_bounds__(kWideThreads, 1)
 wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttendParams p) {
@@ -234,6 +275,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   volatile uint32_t* there = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_THERE);
   uint32_t* red = reinterpret_cast<uint32_t*>(smem + C::OFF_RED);
   Found* found = reinterpret_cast<Found*>(smem + C::OFF_RED + 32);
+  Stopped* stopped = reinterpret_cast<Stopped*>(smem + C::OFF_RED + 48);
   const uint32_t bars = base + C::OFF_BAR;
   auto full = [&](int i) { return bars + 8 * i; };
   auto empty = [&](int i) { return bars + 8 * (ST + i); };
@@ -241,6 +283,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   auto s_full = [&](int i) { return bars + 8 * (2 * ST + 2 + i); };
   auto p_full = [&](int i) { return bars + 8 * (2 * ST + 4 + i); };
   auto o_done = [&](int i) { return bars + 8 * (2 * ST + 6 + i); };  // the products of a segment
+  const uint32_t drained = bars + 8 * (2 * ST + 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int MMA_WARP = 16, COPY_WARP = 17;
 
@@ -299,12 +342,13 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         if (lane == 0) there[(n / 2) % kThere] = mask;
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv, ++n) {
-          if (n >= ST && !(ok = WIDE_ALL(wide_wait(empty(st), ph, abort_flag, 71)))) break;
+          if (n >= ST && !(ok = WIDE_ALL(wide_wait(p, empty(st), ph, abort_flag, 71)))) break;
           const uint32_t dst = base + C::OFF_RING + st * C::TILE_BYTES;
           const CUtensorMap* tmap = kv ? &tm_v : &tm_k;
           if (lane == 0) mbar_expect_tx(full(st), C::TILE_BYTES);
           __syncwarp();
-          if (p.table) {
+          if (n == p.skip_copy) {  // drill
+          } else if (p.table) {
             // a page that is not there, or lies behind the sequence, reads as zeros (outside the map)
             if (mine)
               tma_load_5d(dst + hf * C::HALF + x * box * 128, tmap, full(st), 0, (j0 + x * box) & (p.page - 1), hf, h, page >= 0 ? p.page_base + page : 0x7fffffff);
@@ -317,9 +361,9 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         page = next;
       }
     }
-    if (*abort_flag != 0) {  // let the copies that were issued land before the CTA returns
-      for (int i = max(0, n - ST); i < n; ++i) mbar_wait_quiet(full(i % ST), (i / ST) & 1, 100000);
-    }
+    // When the CTA gives up a wait it ends early: not before the copies that were issued have landed (nor, below, the
+    // products that were issued).
+    for (int i = max(0, n - ST); i < n; ++i) mbar_wait_quiet(full(i % ST), (i / ST) & 1, 100000);
   } else if (warp == MMA_WARP) {
     // ---------------------------------------------------------------- products
     // Scalars only, descriptors built once: this warp is in everybody's chain.
@@ -366,13 +410,13 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         if (u + 1 < count) {
           const int j0 = key_of_tile<kWideTile>(s, from + u + 1);
           x0 = width_of(r0, j0, p.sinks), x1 = width_of(r1, j0, p.sinks);
-          ok = WIDE_ALL(wide_wait(full(k_st), k_ph, abort_flag, 73));
+          ok = WIDE_ALL(wide_wait(p, full(k_st), k_ph, abort_flag, 73));
         }
-        if (ok && u >= 0) ok = WIDE_ALL(wide_wait(full(v_st), v_ph, abort_flag, 72));
+        if (ok && u >= 0) ok = WIDE_ALL(wide_wait(p, full(v_st), v_ph, abort_flag, 72));
         if (!ok) break;
         const uint64_t kd = k_desc + k_st * (C::TILE_BYTES >> 4), vd = v_desc0 + v_st * (C::TILE_BYTES >> 4);
         if (w0) {
-          ok = WIDE_ALL(wide_wait(p_full(0), ph0, abort_flag, 74));
+          ok = WIDE_ALL(wide_wait(p, p_full(0), ph0, abort_flag, 74));
           if (!ok) break;
           ph0 ^= 1;
           tc_fence_after();
@@ -380,18 +424,18 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           more0 = true;
         }
         if (u + 1 == count && elect_one()) tc_commit(o_done(0));
-        if (u < 0 && !(ok = WIDE_ALL(wide_wait(q_full(0), nq & 1, abort_flag, 75)))) break;
+        if (u < 0 && !(ok = WIDE_ALL(wide_wait(p, q_full(0), nq & 1, abort_flag, 75)))) break;
         tc_fence_after();
         if (x0) scores(0, x0, kd);
         if (w1) {
-          ok = WIDE_ALL(wide_wait(p_full(1), ph1, abort_flag, 79));
+          ok = WIDE_ALL(wide_wait(p, p_full(1), ph1, abort_flag, 79));
           if (!ok) break;
           ph1 ^= 1;
           tc_fence_after();
           values(1, w1, vd, more1);
           more1 = true;
         }
-        if (u < 0 && !(ok = WIDE_ALL(wide_wait(q_full(1), nq & 1, abort_flag, 75)))) break;
+        if (u < 0 && !(ok = WIDE_ALL(wide_wait(p, q_full(1), nq & 1, abort_flag, 75)))) break;
         tc_fence_after();
         if (x1) scores(1, x1, kd);
         if (elect_one()) {  // complete with everything issued so far
@@ -404,6 +448,8 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         w0 = x0, w1 = x1;
       }
     }
+    if (elect_one()) tc_commit(drained);
+    mbar_wait_quiet(drained, 0, 100000);
   } else if (warp < 16) {
     // ---------------------------------------------------------------- softmax
     // Row tile i; of each key tile the 64 keys of half `half`, of its features (query rows in, output
@@ -470,7 +516,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const int j0 = key_of_tile<kWideTile>(s, from + u);
         const int width = width_of(reach, j0, p.sinks), mine = width - 64 * half;  // the same for the whole warpgroup
         if (width == 0) continue;
-        ok = WIDE_ALL(wide_wait(s_full(i), ns & 1, abort_flag, 76));
+        ok = WIDE_ALL(wide_wait(p, s_full(i), ns & 1, abort_flag, 76));
         ++ns;
         tc_fence_after();
         const uint32_t held = there[nt % kThere];
@@ -524,7 +570,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         // thread's arrival, for which the product waits.  All warpgroups write the same zeros.
         if (j0 + width > s.len) {
           const uint32_t vn = 2 * nt + 1;
-          ok = ok && WIDE_ALL(wide_wait(full(vn % ST), (vn / ST) & 1, abort_flag, 80));
+          ok = ok && WIDE_ALL(wide_wait(p, full(vn % ST), (vn / ST) & 1, abort_flag, 80));
           uint8_t* vt = smem + C::OFF_RING + vn % ST * C::TILE_BYTES;
           if (ok && j0 + row >= s.len) {
 #pragma unroll
@@ -581,10 +627,10 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       ok = vote_barrier(1 + i, 256, ok && *abort_flag == 0);  // and the maxima have been read
       if (!ok) break;
       tops[half * 128] = l;
-      asm volatile("bar.sync %0, 256;" ::"r"(1 + i) : "memory");
+      ok = vote_barrier(1 + i, 256, WIDE_ALL(wide_wait(p, o_done(i), nq & 1, abort_flag, 78)));
+      if (!ok) break;
       const float m = ref;
       l = tops[0] + tops[128];
-      if (!WIDE_ALL(wide_wait(o_done(i), nq & 1, abort_flag, 78))) l = __int_as_float(0x7fc00000);
       ++nq;
       tc_fence_after();
       const int idx = s.off + t;
@@ -659,9 +705,11 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         plain_row<T, false, D>(p, s.b, h, rr, s.off, s.len, row_view(p, s.off, s.len, token_of(p, rr), TREE ? tm : nullptr), TREE, half * FEATURES, half * FEATURES + FEATURES);
       }
     }
+    if (half == 0 && row == 0) stopped[i] = Stopped{seg.unit, seg.at};
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag != 0) leave_undone<T, D, TREE>(p, stopped, red, found);
   if (warp == MMA_WARP) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -692,6 +740,7 @@ int launch_wide(AttendParams p, int device, cudaStream_t st) {
   using C = Wide<D, TREE>;
   static_assert(C::SMEM <= 227 * 1024, "shared memory of one CTA");
   p.row_blocks = (p.rows + kWideRows - 1) / kWideRows;
+  if (p.wait_cycles == 0) p.wait_cycles = 4 * kWaitCycleLimit;
   p.key_align = p.table ? (p.page < kWideTile ? p.page : kWideTile) : 8;
   CUtensorMap tk, tv;
   int rc;

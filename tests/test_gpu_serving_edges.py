@@ -2,6 +2,7 @@
 values that are not finite side by side, values near the type's largest, shared pages when the pool runs
 out, waits that run out."""
 
+import ctypes as C
 import random
 import subprocess
 import sys
@@ -13,6 +14,7 @@ import torch
 import piper_kernels_b200 as pk
 from _serving import attend, check, tree_visible, window_visible
 from _serving_edges import LongestKeeps, unequal_owners
+from piper_kernels_b200 import _cabi, _ops
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
@@ -238,3 +240,95 @@ def test_largest_number_of_float16_in_prompt_rows(n_q, n_k):
     for got in (pk.window_attention(q, k, v, window=n_k, scale=1.0), pk.cache_attention(q, cache_of(k, v, n_q), scale=1.0)):
         assert got.isfinite().all()
         check_rows(got, q, k, v, window=n_k, scale=1.0, heads=range(0, heads, 17))
+
+
+SENTINEL = 777.0
+
+
+def window_stall(q, k, v, window, cycles, copy):
+    """pk_debug_window_stall into rows that hold a number of their own."""
+    lib, n, out = _cabi.lib(), C.c_uint64(), torch.full_like(q, SENTINEL)
+    p = _cabi.PkWindowProblem(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], _ops._DTYPE[q.dtype], window, 0, q.shape[3] ** -0.5,
+                              q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride()[:3], k.stride()[:3], v.stride()[:3], None, out.data_ptr(),
+                              None, 0, 0, torch.cuda.current_stream().cuda_stream)
+    _cabi.check(lib.pk_window_workspace_bytes(C.byref(p), C.byref(n)))
+    ws = torch.full((n.value,), 255, dtype=torch.uint8, device="cuda")
+    p.workspace, p.workspace_bytes = ws.data_ptr(), n.value
+    _cabi.check(lib.pk_debug_window_stall(C.byref(p), cycles, copy))
+    torch.cuda.synchronize()
+    return out
+
+
+def cache_stall(q, cache, cycles, copy, tree=None, scale=None):
+    lib, n, out = _cabi.lib(), C.c_uint64(), torch.full_like(q, SENTINEL)
+    c = cache.mapped_handle()
+    query = _cabi.PkCacheQuery(q.shape[1], q.shape[2], 0, _ops._DTYPE[q.dtype], 0, 0, q.shape[3] ** -0.5 if scale is None else scale, q.data_ptr(),
+                               q.stride()[:3], None if tree is None else tree.data_ptr(), 0, out.data_ptr(), None, 0)
+    _cabi.check(lib.pk_cache_attention_workspace_bytes(C.byref(c), C.byref(query), C.byref(n)))
+    ws = torch.full((n.value,), 255, dtype=torch.uint8, device="cuda")
+    query.workspace, query.workspace_bytes = ws.data_ptr(), n.value
+    _cabi.check(lib.pk_debug_cache_stall(C.byref(c), C.byref(query), cycles, copy))
+    torch.cuda.synchronize()
+    return out
+
+
+def check_stalled(stall, run, copies, site):
+    """``stall(copy)`` leaves rows of NaN and rows as ``run`` makes them, nothing else; the wait is reported once, and
+    the next call is as before."""
+    want = run()
+    lost = []
+    for copy in copies:
+        got = stall(copy)
+        nan = got.isnan().all(-1)
+        assert torch.equal(got[~nan], want[~nan]), copy
+        lost.append(int(nan.sum()))
+        if lost[-1]:
+            with pytest.raises(_cabi.PiperB200Error, match=f"wait site ({site});"):
+                run()
+        assert torch.equal(run(), want)
+    return lost
+
+
+CYCLES = 2_000_000  # about a millisecond
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("batch,heads,n_q,n_k", [
+    (1, 32, 1, 4000),   # a cluster for every key head
+    (300, 2, 1, 300),   # units shared by all CTAs
+    (3, 4, 32, 3000),   # the same, 64 rows
+    (2, 8, 20, 40),     # a CTA for every key head
+])
+def test_stalled_wait_of_few_rows(dim, dtype, batch, heads, n_q, n_k):
+    q = normal(batch, heads, n_q, dim, dtype=dtype, seed=8)
+    k, v = (normal(batch, heads // 2, n_k, dim, dtype=dtype, seed=s) for s in (9, 10))
+    lost = check_stalled(lambda copy: window_stall(q, k, v, n_k, CYCLES, copy), lambda: pk.window_attention(q, k, v, window=n_k), (0, 1, 4, -1, 10**6), "61|62")
+    assert lost[0] == batch * q.shape[1] * n_q and lost[3:] == [0, 0]
+
+
+@pytest.mark.parametrize("store", [F16, torch.int8])
+@pytest.mark.parametrize("tokens,room", [(1, None), (16, None), (16, 40000), (64, 40000)])
+def test_stalled_wait_over_a_cache(store, tokens, room):
+    lengths, page, dim = [1500, 700, tokens], 32, 128
+    cache = pk.PageCache(3, 90, page, 2, dim, dtype=store, max_length=room or 1504)
+    for counts in ([n - tokens for n in lengths], [tokens] * 3):
+        cache.extend(ints(counts))
+        rows = normal(2, 3, 2, max(counts), dim, dtype=F16, seed=11)
+        cache.write(rows[0], rows[1], layer=0)
+    q, tree = normal(3, 8, tokens, dim, dtype=F16, seed=12), ints([-1] + [(t - 1) // 2 for t in range(1, tokens)])
+    lost = check_stalled(lambda copy: cache_stall(q, cache, CYCLES, copy, tree), lambda: pk.cache_attention(q, cache, tree=tree), (0, 1, 3, -1), "61|62|7[0-9]|80")
+    assert lost[0] == q[..., 0].numel() and lost[3] == 0
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("batch,heads,n_q,n_k", [
+    (1, 8, 300, 300),      # units of few key tiles
+    (1, 2, 1500, 3000),    # all units shared
+    (10, 16, 100, 333),    # more units than SMs, the rest of them shared
+    (40, 16, 80, 200),     # several rounds, none shared
+])
+def test_stalled_wait_of_prompt_rows(dim, dtype, batch, heads, n_q, n_k):
+    q = normal(batch, heads, n_q, dim, dtype=dtype, seed=13)
+    k, v = (normal(batch, heads, n_k, dim, dtype=dtype, seed=s) for s in (14, 15))
+    lost = check_stalled(lambda copy: window_stall(q, k, v, n_k, CYCLES, copy), lambda: pk.window_attention(q, k, v, window=n_k), (0, 1, 2, 3, 7, 12, -1, 10**6), "7[0-9]|80")
+    assert lost[0] == lost[1] == q[..., 0].numel() and lost[6:] == [0, 0]

@@ -89,3 +89,12 @@ def test_copy_maps_of_two_threads_are_one(monkeypatch):
     assert outer.maps == inner[0].maps == cache.mapped_handle().maps and outer.maps in given
     start = C.addressof(cache._maps[0])
     assert start <= outer.maps <= start + 64 and outer.maps % 64 == 0
+
+
+def test_stalled_wait_drill_refuses_before_the_device():
+    lib = _cabi.lib()
+    p, c, q = _cabi.PkWindowProblem(), _cabi.PkCache(), _cabi.PkCacheQuery()
+    for cycles, copy in ((0, 1), (-5, 1), (2 * 10**9, 1), (1000, -2)):
+        assert lib.pk_debug_window_stall(C.byref(p), cycles, copy) == _cabi.PK_ERR_BAD_ARG and b"stall" in lib.pk_last_error()
+        assert lib.pk_debug_cache_stall(C.byref(c), C.byref(q), cycles, copy) == _cabi.PK_ERR_BAD_ARG and b"stall" in lib.pk_last_error()
+    assert lib.pk_debug_window_stall(C.byref(p), 1000, 1) == _cabi.PK_ERR_BAD_ARG and b"batch" in lib.pk_last_error()
