@@ -207,7 +207,7 @@ int validate_query(const pk_cache* c, const pk_cache_query* q, bool launching) {
 }
 
 struct Drill {  // the stalled-wait drill: see pk_debug_window_stall
-  int64_t wait_cycles = 0;
+  int64_t wait_cycles = 4 * kWaitCycleLimit;  // some seconds
   int skip_copy = -1;
 };
 

@@ -69,7 +69,7 @@ struct Few {
   static constexpr int OFF_TREE = OFF_ML + 4 * 16 * 8;
   static constexpr int OFF_BAR = OFF_TREE + static_cast<int>(sizeof(TreeMasks));
   static constexpr int OFF_RED = OFF_BAR + 2 * kStages * 8;
-  static constexpr int OFF_MISC = OFF_RED + 4 * 8 + 24;
+  static constexpr int OFF_MISC = OFF_RED + 4 * 8 + 24;  // (sums, the group found, when rows were last evaluated one by one)
   static constexpr int OFF_THERE = OFF_MISC + 4;  // per stage: which of its pages exist, one bit each
   static constexpr int SMEM = OFF_THERE + kStages * 4;
 };
@@ -144,6 +144,7 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
   Found* found = reinterpret_cast<Found*>(smem + C::OFF_RED + 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC);
   volatile uint32_t* there = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_THERE);
+  volatile long long* busy = reinterpret_cast<volatile long long*>(smem + C::OFF_RED + 48);
   const uint32_t bars = base + C::OFF_BAR;  // full[kStages], empty[kStages]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -151,7 +152,7 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
     mbar_init(bars + 8 * tid, tid < kStages ? 1 : 4);
     fence_barrier_init();
   }
-  if (tid == 0) *abort_flag = 0;
+  if (tid == 0) *abort_flag = 0, *busy = 0;
   if (tid == kConsumers) { prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
   cudaGridDependencySynchronize();
   __syncthreads();
@@ -186,7 +187,7 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
       const int i = static_cast<int>(w - w0), st = i % kStages, j0 = walk.key(), h = walk.h, b = walk.s.b;
       walk.next(p);
       const int next = w + 1 < w1 ? look_up() : -1;
-      if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * (kStages + st), ((i / kStages) - 1) & 1, abort_flag, 61, p.wait_cycles))) break;
+      if (i >= kStages && !__all_sync(0xffffffffu, attend_wait(p, bars + 8 * (kStages + st), ((i / kStages) - 1) & 1, abort_flag, busy, 61))) break;
       const uint32_t full = bars + 8 * st, dst = base + st * C::STAGE;
       const uint32_t mask = p.table ? __ballot_sync(0xffffffffu, page >= 0) : 1u;
       if (lane == 0) {
@@ -288,7 +289,7 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
     const int box = p.table ? min(p.page, C::TILE) : C::TILE;
     for (int u = 0; u < unit_tiles; ++u, ++i) {
       const int st = i % kStages;
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * st, (i / kStages) & 1, abort_flag, 62, p.wait_cycles));
+      ok = __all_sync(0xffffffffu, attend_wait(p, bars + 8 * st, (i / kStages) & 1, abort_flag, busy, 62));
       if (!ok) break;
       const int j0 = key_of_tile<C::TILE>(s, unit_from + u);
       // Keys on pages that are not there are masked like those that no row may see.
@@ -539,7 +540,7 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
       for (int r = 0; vote && r < 4; ++r) {
         if (!(vote & (0xffu << (8 * r)))) continue;
         const int row = s.rb * C::ROWS + it * 16 + warp * 4 + r;
-        plain_row<T, I8, D>(p, s.b, h, row, s.off, s.len, row_view(p, s.off, s.len, token_of(p, row), TREE ? tm : nullptr), TREE);
+        plain_row<T, I8, D>(p, s.b, h, row, s.off, s.len, row_view(p, s.off, s.len, token_of(p, row), TREE ? tm : nullptr), TREE, busy);
       }
     }
     // the next unit
@@ -605,7 +606,6 @@ int launch(AttendParams p, int device, cudaStream_t st) {
   using C = Few<T, I8, D, WM>;
   static_assert(C::SMEM <= 113 * 1024, "two CTAs share an SM");
   p.row_blocks = (p.rows + C::ROWS - 1) / C::ROWS;
-  if (p.wait_cycles == 0) p.wait_cycles = kWaitCycleLimit;
   p.key_align = p.table ? (p.page < C::TILE ? p.page : C::TILE) : 8;
   CUtensorMap tk, tv;
   int rc;

@@ -128,6 +128,25 @@ __device__ __forceinline__ void build_tree(const AttendParams& p, int b, int off
   __syncwarp();
 }
 
+// A bounded wait with little code (it is in every role's loop): gives up after p.wait_cycles, or when another wait has
+// been given up.  While a warp is away evaluating rows one by one (plain_row), which may take longer, it keeps the time
+// at `busy`, and the wait counts from there.
+__device__ __forceinline__ bool attend_wait(const AttendParams& p, uint32_t bar, uint32_t parity, volatile int* abort_flag, volatile long long* busy, int where) {
+  long long since = 0;
+  for (int n = 0; !mbar_try_wait(bar, parity); ++n) {
+    if ((n & 63) != 63) continue;
+    if (*abort_flag != 0) return false;
+    const long long now = clock64();
+    if (since == 0) since = now;
+    if (now - since <= p.wait_cycles) continue;
+    since = *busy;
+    if (now - since <= p.wait_cycles) continue;
+    *abort_flag = where;
+    return false;
+  }
+  return true;
+}
+
 // Barrier of all threads of a cluster; what they wrote before it, they all read after it.
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
@@ -215,9 +234,11 @@ __device__ __forceinline__ bool holds<__nv_bfloat16>(float x) { return fabsf(x) 
 // features [i * D/32, (i+1) * D/32).  The tiled kernels multiply whole tiles, so that an infinity
 // or NaN in a V row that this query row must not see would still reach it (0 * NaN); a row that
 // comes out of them with a value that its type does not hold is evaluated again here (its features
-// [first, last) are written).  Rare, and slow.
+// [first, last) are written).  Rare, and slow: some 1800 cycles a key.  `busy` (if any) takes the time meanwhile, for
+// the waits of other warps.
 template <typename T, bool I8, int D>
-__device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, int row, int off, int len, RowView view, bool tree, int first = 0, int last = D) {
+__device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, int row, int off, int len, RowView view, bool tree, volatile long long* busy = nullptr,
+                                       int first = 0, int last = D) {
   constexpr int E = D / 32;
   const int lane = threadIdx.x & 31, t = token_of(p, row), head = kvh * p.group + row - t * p.group;
   const T* q = static_cast<const T*>(p.q) + b * p.q_stride[0] + head * p.q_stride[1] + t * p.q_stride[2] + lane * E;
@@ -226,6 +247,7 @@ __device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, in
   for (int e = 0; e < E; ++e) qf[e] = to_f32(q[e]) * p.scale_log2, acc[e] = 0.f;
   const int end = tree ? min(len, off + kMaxTreeTokens) : min(len, view.lim);
   for (int j = 0; j < end; ++j) {
+    if (busy && lane == 0 && (j & 63) == 0) *busy = clock64();
     const bool visible = tree ? sees<true>(view, j, off, p.sinks) : sees<false>(view, j, off, p.sinks);
     if (!visible) continue;  // the same for all lanes
     int64_t at_k, at_v, at_s = 0;
@@ -264,6 +286,11 @@ __device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, in
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = acc[e] * keep + w * vf[e];
     m = mn;
+    // A row that is NaN throughout stays so: inputs full of NaN are done with soon.
+    bool nan = true;
+#pragma unroll
+    for (int e = 0; e < E; ++e) nan = nan && acc[e] != acc[e];
+    if (__all_sync(0xffffffffu, nan)) break;
   }
   T* out = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.heads + head) * p.tokens + t) * D + lane * E;
 #pragma unroll

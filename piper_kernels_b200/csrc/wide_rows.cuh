@@ -133,23 +133,6 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// A bounded wait with little code (it is in every role's loop): gives up after some seconds, or when
-// another wait has been given up.  The limit is generous because a softmax warp may be away evaluating
-// rows one by one (plain_row) while the others wait for it.
-__device__ __forceinline__ bool wide_wait(const AttendParams& p, uint32_t bar, uint32_t parity, volatile int* abort_flag, int where) {
-  long long since = 0;
-  for (int n = 0; !mbar_try_wait(bar, parity); ++n) {
-    if ((n & 63) != 63) continue;
-    const long long now = clock64();
-    if (since == 0) since = now;
-    if (*abort_flag != 0 || now - since > p.wait_cycles) {
-      *abort_flag = where;
-      return false;
-    }
-  }
-  return true;
-}
-
 // What one CTA does next.  Every role walks the same list: first every gridDim.x-th of the whole units
 // [0, first_unit), from the back (causal rows see the most keys there), then an equal, contiguous share
 // of the tiles of the units from first_unit on.
@@ -275,6 +258,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   volatile uint32_t* there = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_THERE);
   uint32_t* red = reinterpret_cast<uint32_t*>(smem + C::OFF_RED);
   Found* found = reinterpret_cast<Found*>(smem + C::OFF_RED + 32);
+  volatile long long* busy = reinterpret_cast<volatile long long*>(smem + C::OFF_RED + 40);
   Stopped* stopped = reinterpret_cast<Stopped*>(smem + C::OFF_RED + 48);
   const uint32_t bars = base + C::OFF_BAR;
   auto full = [&](int i) { return bars + 8 * i; };
@@ -292,7 +276,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     mbar_init(bars + 8 * tid, at < 0 || at == 2 || at == 3 || at >= 6 ? 1 : 256);  // q_full, p_full: two warpgroups
     fence_barrier_init();
   }
-  if (tid == 0) *abort_flag = 0;
+  if (tid == 0) *abort_flag = 0, *busy = 0;
   if (warp == MMA_WARP) {
     tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
     tmem_relinquish();
@@ -342,7 +326,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         if (lane == 0) there[(n / 2) % kThere] = mask;
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv, ++n) {
-          if (n >= ST && !(ok = WIDE_ALL(wide_wait(p, empty(st), ph, abort_flag, 71)))) break;
+          if (n >= ST && !(ok = WIDE_ALL(attend_wait(p, empty(st), ph, abort_flag, busy, 71)))) break;
           const uint32_t dst = base + C::OFF_RING + st * C::TILE_BYTES;
           const CUtensorMap* tmap = kv ? &tm_v : &tm_k;
           if (lane == 0) mbar_expect_tx(full(st), C::TILE_BYTES);
@@ -410,13 +394,13 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         if (u + 1 < count) {
           const int j0 = key_of_tile<kWideTile>(s, from + u + 1);
           x0 = width_of(r0, j0, p.sinks), x1 = width_of(r1, j0, p.sinks);
-          ok = WIDE_ALL(wide_wait(p, full(k_st), k_ph, abort_flag, 73));
+          ok = WIDE_ALL(attend_wait(p, full(k_st), k_ph, abort_flag, busy, 73));
         }
-        if (ok && u >= 0) ok = WIDE_ALL(wide_wait(p, full(v_st), v_ph, abort_flag, 72));
+        if (ok && u >= 0) ok = WIDE_ALL(attend_wait(p, full(v_st), v_ph, abort_flag, busy, 72));
         if (!ok) break;
         const uint64_t kd = k_desc + k_st * (C::TILE_BYTES >> 4), vd = v_desc0 + v_st * (C::TILE_BYTES >> 4);
         if (w0) {
-          ok = WIDE_ALL(wide_wait(p, p_full(0), ph0, abort_flag, 74));
+          ok = WIDE_ALL(attend_wait(p, p_full(0), ph0, abort_flag, busy, 74));
           if (!ok) break;
           ph0 ^= 1;
           tc_fence_after();
@@ -424,18 +408,18 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           more0 = true;
         }
         if (u + 1 == count && elect_one()) tc_commit(o_done(0));
-        if (u < 0 && !(ok = WIDE_ALL(wide_wait(p, q_full(0), nq & 1, abort_flag, 75)))) break;
+        if (u < 0 && !(ok = WIDE_ALL(attend_wait(p, q_full(0), nq & 1, abort_flag, busy, 75)))) break;
         tc_fence_after();
         if (x0) scores(0, x0, kd);
         if (w1) {
-          ok = WIDE_ALL(wide_wait(p, p_full(1), ph1, abort_flag, 79));
+          ok = WIDE_ALL(attend_wait(p, p_full(1), ph1, abort_flag, busy, 79));
           if (!ok) break;
           ph1 ^= 1;
           tc_fence_after();
           values(1, w1, vd, more1);
           more1 = true;
         }
-        if (u < 0 && !(ok = WIDE_ALL(wide_wait(p, q_full(1), nq & 1, abort_flag, 75)))) break;
+        if (u < 0 && !(ok = WIDE_ALL(attend_wait(p, q_full(1), nq & 1, abort_flag, busy, 75)))) break;
         tc_fence_after();
         if (x1) scores(1, x1, kd);
         if (elect_one()) {  // complete with everything issued so far
@@ -516,7 +500,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const int j0 = key_of_tile<kWideTile>(s, from + u);
         const int width = width_of(reach, j0, p.sinks), mine = width - 64 * half;  // the same for the whole warpgroup
         if (width == 0) continue;
-        ok = WIDE_ALL(wide_wait(p, s_full(i), ns & 1, abort_flag, 76));
+        ok = WIDE_ALL(attend_wait(p, s_full(i), ns & 1, abort_flag, busy, 76));
         ++ns;
         tc_fence_after();
         const uint32_t held = there[nt % kThere];
@@ -570,7 +554,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         // thread's arrival, for which the product waits.  All warpgroups write the same zeros.
         if (j0 + width > s.len) {
           const uint32_t vn = 2 * nt + 1;
-          ok = ok && WIDE_ALL(wide_wait(p, full(vn % ST), (vn / ST) & 1, abort_flag, 80));
+          ok = ok && WIDE_ALL(attend_wait(p, full(vn % ST), (vn / ST) & 1, abort_flag, busy, 80));
           uint8_t* vt = smem + C::OFF_RING + vn % ST * C::TILE_BYTES;
           if (ok && j0 + row >= s.len) {
 #pragma unroll
@@ -627,7 +611,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       ok = vote_barrier(1 + i, 256, ok && *abort_flag == 0);  // and the maxima have been read
       if (!ok) break;
       tops[half * 128] = l;
-      ok = vote_barrier(1 + i, 256, WIDE_ALL(wide_wait(p, o_done(i), nq & 1, abort_flag, 78)));
+      ok = vote_barrier(1 + i, 256, WIDE_ALL(attend_wait(p, o_done(i), nq & 1, abort_flag, busy, 78)));
       if (!ok) break;
       const float m = ref;
       l = tops[0] + tops[128];
@@ -702,7 +686,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       while (vote) {  // rows with a value that their type does not hold, evaluated again from their own keys
         const int src = __ffs(vote) - 1, rr = row0 + w4 * 32 + src;
         vote &= vote - 1;
-        plain_row<T, false, D>(p, s.b, h, rr, s.off, s.len, row_view(p, s.off, s.len, token_of(p, rr), TREE ? tm : nullptr), TREE, half * FEATURES, half * FEATURES + FEATURES);
+        plain_row<T, false, D>(p, s.b, h, rr, s.off, s.len, row_view(p, s.off, s.len, token_of(p, rr), TREE ? tm : nullptr), TREE, busy, half * FEATURES, half * FEATURES + FEATURES);
       }
     }
     if (half == 0 && row == 0) stopped[i] = Stopped{seg.unit, seg.at};
@@ -740,7 +724,6 @@ int launch_wide(AttendParams p, int device, cudaStream_t st) {
   using C = Wide<D, TREE>;
   static_assert(C::SMEM <= 227 * 1024, "shared memory of one CTA");
   p.row_blocks = (p.rows + kWideRows - 1) / kWideRows;
-  if (p.wait_cycles == 0) p.wait_cycles = 4 * kWaitCycleLimit;
   p.key_align = p.table ? (p.page < kWideTile ? p.page : kWideTile) : 8;
   CUtensorMap tk, tv;
   int rc;

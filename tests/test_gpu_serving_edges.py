@@ -247,7 +247,7 @@ SENTINEL = 777.0
 
 def window_stall(q, k, v, window, cycles, copy):
     """pk_debug_window_stall into rows that hold a number of their own."""
-    lib, n, out = _cabi.lib(), C.c_uint64(), torch.full_like(q, SENTINEL)
+    lib, n, out = _cabi.lib(), C.c_uint64(), torch.full(q.shape, SENTINEL, dtype=q.dtype, device="cuda")
     p = _cabi.PkWindowProblem(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], _ops._DTYPE[q.dtype], window, 0, q.shape[3] ** -0.5,
                               q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride()[:3], k.stride()[:3], v.stride()[:3], None, out.data_ptr(),
                               None, 0, 0, torch.cuda.current_stream().cuda_stream)
@@ -260,7 +260,7 @@ def window_stall(q, k, v, window, cycles, copy):
 
 
 def cache_stall(q, cache, cycles, copy, tree=None, scale=None):
-    lib, n, out = _cabi.lib(), C.c_uint64(), torch.full_like(q, SENTINEL)
+    lib, n, out = _cabi.lib(), C.c_uint64(), torch.full(q.shape, SENTINEL, dtype=q.dtype, device="cuda")
     c = cache.mapped_handle()
     query = _cabi.PkCacheQuery(q.shape[1], q.shape[2], 0, _ops._DTYPE[q.dtype], 0, 0, q.shape[3] ** -0.5 if scale is None else scale, q.data_ptr(),
                                q.stride()[:3], None if tree is None else tree.data_ptr(), 0, out.data_ptr(), None, 0)
@@ -332,3 +332,25 @@ def test_stalled_wait_of_prompt_rows(dim, dtype, batch, heads, n_q, n_k):
     k, v = (normal(batch, heads, n_k, dim, dtype=dtype, seed=s) for s in (14, 15))
     lost = check_stalled(lambda copy: window_stall(q, k, v, n_k, CYCLES, copy), lambda: pk.window_attention(q, k, v, window=n_k), (0, 1, 2, 3, 7, 12, -1, 10**6), "7[0-9]|80")
     assert lost[0] == lost[1] == q[..., 0].numel() and lost[6:] == [0, 0]
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("batch,n_q,n_k", [
+    (592, 16, 20000),  # few rows, two units for each of 296 CTAs
+    (592, 100, 4000),  # prompt rows, four units for each of 148 CTAs
+])
+def test_waits_for_rows_that_are_evaluated_one_by_one(dim, dtype, batch, n_q, n_k):
+    """A NaN in the last value row reaches the tiles of tokens that do not see it: these are evaluated one by one, which
+    takes some hundred times as long as the other warps' waits may last here."""
+    q = normal(1, 1, n_q, dim, dtype=dtype, seed=16).expand(batch, 1, n_q, dim)
+    k, v = (normal(1, 1, n_k, dim, dtype=dtype, seed=s) for s in (17, 18))
+    clean = v.clone()
+    v[0, 0, -1] = float("nan")
+    visible = window_visible(n_q, n_k, n_k, 0, n_k).cuda()
+    want, off = attend(q[0, 0], k[0, 0], clean[0, 0], visible, dim**-0.5, dtype)
+    got = window_stall(q, k.expand(batch, 1, n_k, dim), v.expand(batch, 1, n_k, dim), n_k, 1_000_000, -1)
+    assert torch.equal(got[1:, :, :-1], got[:1, :, :-1].expand_as(got[1:, :, :-1])) and got[:, :, -1].isnan().all()
+    check(got[0, 0, :-1], want[:-1], off[:-1])
+    code = C.c_int32(0)
+    _cabi.check(_cabi.lib().pk_poll_device_fault(0, C.byref(code)))
+    assert code.value == 0
