@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(kPlan) extend_kernel(const Pages c, const int3
   int* tail = plan;                  // last, partly filled page of a sequence that grows; -1: none
   int* before = plan + c.batch;      // new pages of the sequences in front (batch + 1 entries)
   int* copies = before + c.batch + 1;  // whether the last page is replaced
+  int* order = before;                 // until `before` is written: rows on the last page, the first sequence ahead among equals
   __shared__ int warp_sums[32];
   __shared__ int n_copies;
   const int tid = threadIdx.x;
@@ -88,6 +89,7 @@ __global__ void __launch_bounds__(kPlan) extend_kernel(const Pages c, const int3
     int page = -1;
     if (add > 0 && add <= row_limit(c) - len && (len & (c.page - 1))) page = c.table[static_cast<int64_t>(b) * c.width + (len >> c.shift)];
     tail[b] = is_page(c, page) ? page : -1;
+    order[b] = (len & (c.page - 1)) * kMaxBatch + kMaxBatch - 1 - b;
   }
   __syncthreads();
   // A last page that others name too is replaced; when all that name it grow, the longest of them keeps it (the
@@ -98,16 +100,12 @@ __global__ void __launch_bounds__(kPlan) extend_kernel(const Pages c, const int3
     if (page >= 0) {
       const int users = c.uses[page];
       if (users > 1) {
-        const int held = length_of(c, b) & (c.page - 1);
-        int growing = 0;
-        bool keeps = true;
+        int growing = 0, longest = 0;
         for (int o = 0; o < c.batch; ++o) {
-          if (tail[o] != page) continue;
-          ++growing;
-          const int other = length_of(c, o) & (c.page - 1);
-          keeps = keeps && (other < held || (other == held && o >= b));
+          const int at = order[o];
+          if (tail[o] == page) ++growing, longest = max(longest, at);
         }
-        copy = growing < users || !keeps;
+        copy = growing < users || longest != order[b];
       }
     }
     copies[b] = copy;
