@@ -468,10 +468,6 @@ __device__ __forceinline__ void join_row(const AttendParams& p, const Pieces at,
     mx = fmaxf(mx, st.x);
     undone |= st.y < 0.f;
   }
-  if (__any_sync(0xffffffffu, undone)) {
-    if (lane < D / 8) nan_row<T, D, 8>(p, g / p.row_blocks, h, row, lane * 8);
-    return;
-  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
 #pragma unroll
@@ -499,6 +495,8 @@ __device__ __forceinline__ void join_row(const AttendParams& p, const Pieces at,
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  undone = __any_sync(0xffffffffu, undone);
+  if (undone) sum = __int_as_float(0x7fc00000);
   const int b = g / p.row_blocks, len = attend_len(p, b), off = attend_off(p, b, len);
   const int t = token_of(p, row), idx = off + t;
   const bool valid = idx >= 0 && idx < len;
@@ -512,7 +510,7 @@ __device__ __forceinline__ void join_row(const AttendParams& p, const Pieces at,
     *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(x, y);
   }
   __syncwarp();
-  if (!__any_sync(0xffffffffu, bad)) return;
+  if (undone || !__any_sync(0xffffffffu, bad)) return;
   if (TREE) build_tree(p, b, off, lane, tm);  // warps of one CTA write the same values
   plain_row<T, I8, D>(p, b, h, row, off, len, row_view(p, off, len, t, TREE ? tm : nullptr), TREE);
 }
