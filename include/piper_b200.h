@@ -272,9 +272,10 @@ PK_API int pk_cache_write(const pk_cache* c, int32_t layer, const void* key, con
  * [0, lengths[b]) read as zero. */
 PK_API int pk_cache_read(const pk_cache* c, int32_t layer, const int32_t* first, int32_t count, void* key, void* value, int32_t dtype);
 /* Sequence b becomes what sequence parents[b] was before the call (shares its pages); negative:
- * empty.  parents[b] >= batch is refused (the sequence stays as it was). */
+ * empty.  parents[b] >= batch is refused (the sequence keeps its rows).  starts = lengths for all. */
 PK_API int pk_cache_fork(const pk_cache* c, const int32_t* parents);
-/* Every sequence keeps its first min(length, max(lengths[b], 0)) rows; pages behind them are released. */
+/* Every sequence keeps its first min(length, max(lengths[b], 0)) rows; pages behind them are released;
+ * starts = lengths. */
 PK_API int pk_cache_truncate(const pk_cache* c, const int32_t* lengths);
 /* Of the rows added last keeps paths[b, i], i < counts[b], in this order: row starts + paths[b, i]
  * moves to starts + i, the rest is released (as by truncate).  paths is [batch, most]; it must rise

@@ -224,14 +224,15 @@ class PageCache:
 
         ``parents[b] = b`` keeps it, a negative one empties it, several may name the same parent.  Pages are
         shared, not copied; :meth:`extend` copies a shared last page when it has to.  ``parents[b] >= batch`` is
-        refused: the sequence stays.  ``starts`` becomes ``lengths``: rows added before are no longer the latest.
+        refused: the sequence keeps its rows.  ``starts`` becomes ``lengths`` everywhere: rows added before are no
+        longer the latest.
         """
         check_lengths(_OP, "parents", parents, self.batch, self.device, optional=False)
         _cabi.check(_cabi.lib().pk_cache_fork(C.byref(self.handle()), parents.data_ptr()))
 
     def truncate(self, lengths: torch.Tensor) -> None:
         """Every sequence keeps its first ``lengths[b]`` rows (int32 ``[batch]``; 0 or less: none; more than it
-        has: all) and releases the pages behind them."""
+        has: all) and releases the pages behind them; ``starts`` becomes ``lengths``."""
         check_lengths(_OP, "lengths", lengths, self.batch, self.device, optional=False)
         _cabi.check(_cabi.lib().pk_cache_truncate(C.byref(self.handle()), lengths.data_ptr()))
 

@@ -23,7 +23,7 @@
 //   - A few of the exponentials are evaluated on the FMA pipe beside the exponential unit.
 // Measured: 4 prompts of 8192 tokens, 32 query and 8 key heads of 128 features, window 1024, float16:
 // 697 us, 743 TFLOP/s of visible pairs (0.45 of the measured 1652); the last 2048 tokens of 32760, 40 / 8
-// heads, window 4096, bfloat16: 182 us, 957 TFLOP/s (0.58).  A tile's chain takes some 3600 cycles where the two
+// heads, window 4096, bfloat16: 184 us, 947 TFLOP/s (0.57); SM clock 1875 to 1965 MHz.  A tile's chain takes some 3600 cycles where the two
 // row tiles' products fill 2048; two thirds of it are in the softmax, most of that latency (taking the
 // exponentials out altogether makes the kernel 6 % faster), the rest in the products and the hand-overs.
 // A unit's query rows in, first scores and rows out take about 9000 cycles, partly beside the other row tile.
@@ -184,7 +184,7 @@ __device__ __forceinline__ Reach reach_of(const AttendParams& p, const Span& s, 
   r.lo = max(0, (TREE ? s.off : s.off + t0) - p.window + 1);
   return r;
 }
-// How many of a tile's keys, from its first on, a row tile has to look at (a multiple of 32; 0: none).
+// How many of a tile's keys, from its first on, a row tile has to look at (a multiple of 64; 0: none).
 __device__ __forceinline__ int width_of(const Reach& r, int j0, int sinks) {
   const int end = j0 + kWideTile > r.lo ? r.hi : min(sinks, r.hi);
   return max(0, min((end - j0 + 63) & ~63, kWideTile));

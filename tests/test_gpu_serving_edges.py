@@ -354,3 +354,25 @@ def test_waits_for_rows_that_are_evaluated_one_by_one(dim, dtype, batch, n_q, n_
     code = C.c_int32(0)
     _cabi.check(_cabi.lib().pk_poll_device_fault(0, C.byref(code)))
     assert code.value == 0
+
+
+@pytest.mark.parametrize("dim,dtype,store", [(64, F16, F16), (128, BF16, BF16), (128, F16, torch.int8), (64, BF16, torch.int8)])
+@pytest.mark.parametrize("tokens", [1, 16, 100])
+def test_pages_of_256_rows(dim, dtype, store, tokens):
+    """The largest pages: longer than a key tile."""
+    n = 500 + tokens
+    cache = pk.PageCache(2, 6, 256, 2, dim, dtype=store, max_length=n)
+    rows = normal(2, 2, 2, n, dim, dtype=dtype, seed=19)
+    cache.extend(ints([n, n]))
+    cache.write(rows[0], rows[1], layer=0)
+    cache.starts.fill_(500)
+    q = normal(2, 4, tokens, dim, dtype=dtype, seed=20)
+    k, v = cache.read(ints([0, 0]), n, layer=0)
+    step = float(cache.value_scales.max()) * 127 if store is torch.int8 else 0.0
+    for window, sinks in ((None, 0), (200, 5)):
+        got = pk.cache_attention(q, cache, window=window, sinks=sinks)
+        visible = window_visible(tokens, n, window or n, sinks, n).cuda()
+        for b in range(2):
+            for h in range(4):
+                want, off = attend(q[b, h], k[b, h // 2], v[b, h // 2], visible, dim**-0.5, dtype, step)
+                check(got[b, h], want, off, f"sequence {b} head {h}")
