@@ -143,8 +143,8 @@ PK_API int pk_sage2pp_attention_fwd(const pk_problem* p);
 PK_API int pk_device_status(const pk_problem* p, int32_t status[16]);
 
 /* Non-blocking check for the same condition, for callers that do not keep the workspace (the
- * torch operators): every fused kernel also writes its wait-site code into one pinned host word
- * per device; this call reads and clears it without touching the device or any stream.  Returns
+ * torch operators): every fused kernel, and every attention kernel of the second half of this file,
+ * also writes its wait-site code into one pinned host word per device; this call reads and clears it without touching the device or any stream.  Returns
  * PK_ERR_DEVICE_STATUS with *code != 0 when a kernel launched earlier on `device` gave up a
  * wait, PK_OK with *code == 0 otherwise.  The reference has no counterpart (its kernels cannot
  * give up a wait); it stands where the reference relies on CUDA's own launch errors. */

@@ -234,8 +234,8 @@ __device__ __forceinline__ bool holds<__nv_bfloat16>(float x) { return fabsf(x) 
 // features [i * D/32, (i+1) * D/32).  The tiled kernels multiply whole tiles, so that an infinity
 // or NaN in a V row that this query row must not see would still reach it (0 * NaN); a row that
 // comes out of them with a value that its type does not hold is evaluated again here (its features
-// [first, last) are written).  Rare, and slow: some 1800 cycles a key.  `busy` (if any) takes the time meanwhile, for
-// the waits of other warps.
+// [first, last) are written).  Rare, and slow: 1000 to 2000 cycles a key.  `busy` (if any) takes the time
+// meanwhile, for the waits of other warps.
 template <typename T, bool I8, int D>
 __device__ __noinline__ void plain_row(const AttendParams& p, int b, int kvh, int row, int off, int len, RowView view, bool tree, volatile long long* busy = nullptr,
                                        int first = 0, int last = D) {
