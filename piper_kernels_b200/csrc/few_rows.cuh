@@ -540,7 +540,7 @@ __device__ __forceinline__ void attend_share(const CUtensorMap& tm_k, const CUte
       for (int r = 0; vote && r < 4; ++r) {
         if (!(vote & (0xffu << (8 * r)))) continue;
         const int row = s.rb * C::ROWS + it * 16 + warp * 4 + r;
-        plain_row<T, I8, D>(p, s.b, h, row, s.off, s.len, row_view(p, s.off, s.len, token_of(p, row), TREE ? tm : nullptr), TREE, busy);
+        plain_row<T, I8, D, true>(p, s.b, h, row, s.off, s.len, row_view(p, s.off, s.len, token_of(p, row), TREE ? tm : nullptr), TREE, busy);
       }
     }
     // the next unit

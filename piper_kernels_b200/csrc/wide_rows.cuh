@@ -686,7 +686,7 @@ wide_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       while (vote) {  // rows with a value that their type does not hold, evaluated again from their own keys
         const int src = __ffs(vote) - 1, rr = row0 + w4 * 32 + src;
         vote &= vote - 1;
-        plain_row<T, false, D>(p, s.b, h, rr, s.off, s.len, row_view(p, s.off, s.len, token_of(p, rr), TREE ? tm : nullptr), TREE, busy, half * FEATURES, half * FEATURES + FEATURES);
+        plain_row<T, false, D, true>(p, s.b, h, rr, s.off, s.len, row_view(p, s.off, s.len, token_of(p, rr), TREE ? tm : nullptr), TREE, busy, half * FEATURES, half * FEATURES + FEATURES);
       }
     }
     if (half == 0 && row == 0) stopped[i] = Stopped{seg.unit, seg.at};
